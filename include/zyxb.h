@@ -97,7 +97,8 @@ typedef struct {
  * them (zyx/src/backend/mod.rs:974, zyx/src/runtime.rs:2285-2291).
  * ---------------------------------------------------------------------------------- */
 enum { ZYXB_KIND_ROWREDUCE = 1, ZYXB_KIND_GEMM = 2, ZYXB_KIND_ELTWISE = 3, ZYXB_KIND_OPTIM = 4, ZYXB_KIND_ATTENTION = 5, ZYXB_KIND_ATTENTION_BWD = 6,
-       ZYXB_KIND_CONV = 7, ZYXB_KIND_CONV_WGRAD = 8, ZYXB_KIND_CONV_DGRAD = 9 };
+       ZYXB_KIND_CONV = 7, ZYXB_KIND_CONV_WGRAD = 8, ZYXB_KIND_CONV_DGRAD = 9,
+       ZYXB_KIND_EMBEDDING = 10, ZYXB_KIND_EMBEDDING_BWD = 11, ZYXB_KIND_RMSNORM = 12, ZYXB_KIND_RMSNORM_BWD = 13, ZYXB_KIND_MUON = 14 };
 
 /* Row kernels: an elementwise chain with a trailing reduce over the last axis.
  * Semantics: Tensor::reduce_impl (zyx/src/tensor/reduce_ops.rs:45-157), softmax /
@@ -278,6 +279,72 @@ typedef struct {
  *                       bf16 / f16 with enough work run per tap as a matmul over the output positions on the tensor cores
  *                       (dy by tiled TMA, x by im2col-mode TMA, positions split over CTAs, f32 partials added in a fixed order) */
 
+/* Embedding: rows of a table picked by token number, and the gradient of the table.  No counterpart in the reference, which
+ * would multiply a one-hot matrix: as there, a token number outside [0, vocab) (padding, say -1) picks a row of zeros and gives
+ * no gradient.
+ *   EMBEDDING      out[i,:] = scale * table[ids[i],:]          (scale 1: the table's bits)
+ *   EMBEDDING_BWD  dtable[v,:] = scale * sum over the i with ids[i] = v of dout[i,:]   (+ dtable[v,:] when accumulate is set)
+ * The sums are f32, over the tokens in an order that depends on ids alone: the same input gives the same bits.  Without accumulate
+ * every row of dtable is written (zeros where no token names it); with it only the named rows are read and written. */
+typedef struct {
+  int32_t  dtype;        /* table, out, dout, dtable: bf16 / f16 / f32 */
+  int32_t  id_dtype;     /* ZYXB_I32 or ZYXB_I64 */
+  uint64_t tokens, vocab, dim;   /* each below 2^31 */
+  uint64_t ld_table, ld_out;     /* row pitch of table / dtable and of out / dout in elements; 0 = dim.  What lies between dim and
+                                    the pitch is neither read nor written */
+  float    scale;        /* 0 means 1 */
+  int32_t  accumulate;   /* EMBEDDING_BWD only */
+} zyxb_embedding_desc;
+/* ZYXB_KIND_EMBEDDING      args: ids, table -> out
+ * ZYXB_KIND_EMBEDDING_BWD  args: ids, dout -> dtable */
+
+/* Root-mean-square norm of rows, with the residual stream's addition in front of it.
+ *   h = x + residual (f32; the stored h is rounded once, the norm reads the unrounded sum)
+ *   y = h / sqrt(mean(h^2) + eps) * weight
+ * quant: y is stored as 8-bit floats (e4m3, 4 exponent and 3 mantissa bits, largest 448) with one f32 scale per `group` columns of
+ * a row: scale = max(max|y|, 1e-30) / 448, q = e4m3(y / scale) rounded to nearest even; y stands for q * scale.
+ * Backward (h as stored): xh = h / sqrt(mean(h^2) + eps), g = dy * weight, dx = (g - xh * mean(g * xh)) / sqrt(mean(h^2) + eps) [+ dh],
+ * dweight = sum over rows of dy * xh (f32, in a fixed order).  dx is the gradient of x and of residual alike; dh is the gradient
+ * that reaches the residual stream behind the norm.
+ * An output may be the buffer of an input of its type and shape. */
+typedef struct {
+  int32_t  dtype;        /* bf16 / f16 / f32; weight, dweight too */
+  int32_t  quant;        /* RMSNORM only: 1 = y as e4m3 bytes [rows, cols] (dense) and scales [rows, ceil(cols / group)] */
+  uint64_t rows, cols;   /* cols <= 16384 */
+  uint64_t ld;           /* row pitch of x, residual, h, y, dy, dh, dx in elements; 0 = cols */
+  float    eps;
+  int32_t  has_residual, has_weight;
+  int32_t  has_dh;       /* RMSNORM_BWD only */
+  uint32_t group;        /* quant: columns that share a scale, at least 16; 0 = the whole row */
+} zyxb_rmsnorm_desc;
+/* ZYXB_KIND_RMSNORM      args: x [,residual] [,weight] -> [h when has_residual,] y [,scales when quant]
+ * ZYXB_KIND_RMSNORM_BWD  args: h, dy [,weight] [,dh] -> dx [,dweight when has_weight] */
+
+/* Muon: the update of weight matrices whose step is the momentum made (nearly) orthogonal by Newton-Schulz products.  Per matrix
+ *   buf = momentum * buf + g;  u = nesterov ? g + momentum * buf : buf          (buf as stored)
+ *   X = u / (|u|_F + eps);  `steps` times  X = a X + (b A + c A^2) X  with A = X X^T  (X^T X, from the right, when rows > cols)
+ *   p = p * (1 - lr * weight_decay) - lr * adjust * X
+ * f32 matrices carry X, A as pairs of f16 (22 bits) and add the products in f32; 16-bit ones as single f16 (11 bits).
+ * Nothing depends on a step counter: buf starts as zeros, and a launch may be captured. */
+enum { ZYXB_MUON_ADJUST_RATIO = 0,   /* sqrt(max(1, rows / cols)) */
+       ZYXB_MUON_ADJUST_RMS = 1 };   /* 0.2 * sqrt(max(rows, cols)): the root mean square of an Adam step */
+typedef struct {
+  int32_t  dtype;          /* params, grads, buf: bf16 / f16 / f32 */
+  int32_t  n_tensors;
+  const uint64_t* rows;    /* [n_tensors]; copied at program creation */
+  const uint64_t* cols;    /* [n_tensors]; each extent at most 32768 */
+  float    lr, weight_decay, momentum;
+  int32_t  nesterov;
+  int32_t  steps;          /* 0 means 5; at most 32 */
+  float    a, b, c;        /* all 0 means 3.4445, -4.7750, 2.0315; a x + b x^3 + c x^5 has to map [0, 1.25] into [-1.25, 1.25] */
+  float    eps;            /* 0 means 1e-7 */
+  float    grad_scale;     /* gradients are multiplied by this first; 0 means 1 */
+  int32_t  adjust;         /* ZYXB_MUON_ADJUST_* */
+} zyxb_muon_desc;
+/* ZYXB_KIND_MUON  args (updated in place): p[0..n), g[0..n) [, buf[0..n) when momentum != 0]; p and buf each name n different buffers.
+ * The program owns the memory its products need (allocated at creation, given back at release): a graph that captured its launch
+ * must be released before it. */
+
 typedef struct {
   int32_t kind;  /* ZYXB_KIND_* */
   union {
@@ -287,6 +354,9 @@ typedef struct {
     zyxb_optim_desc     optim;
     zyxb_attention_desc attention;   /* both attention kinds */
     zyxb_conv_desc      conv;
+    zyxb_embedding_desc embedding;   /* both embedding kinds */
+    zyxb_rmsnorm_desc   rmsnorm;     /* both RMS norm kinds */
+    zyxb_muon_desc      muon;
   } u;
 } zyxb_kernel_desc;
 
@@ -330,6 +400,12 @@ int32_t zyxb_buffer_bytes(zyxb_ctx* ctx, int32_t dev, uint32_t buf, uint64_t* ou
  * plan's `Alias` instruction shares storage (zyx/src/graph/plan.rs:47-54).  Freeing a view releases
  * only the id; the parent must outlive its views. */
 int32_t zyxb_buffer_view(zyxb_ctx* ctx, int32_t dev, uint32_t parent, uint64_t offset, uint64_t bytes, uint32_t* out_buf);
+/* An id for device memory that another library of this process owns (a tensor of it, say): programs then read and write it in
+ * place.  device_ptr is 256-byte aligned and [device_ptr, device_ptr + bytes) lies inside one allocation on this device.
+ * zyxb_free releases only the id; the owner keeps the memory alive until this library's work on it has finished.  The library's
+ * streams know nothing of the owner's: synchronise with the owner's stream before a launch, and with this device (zyxb_sync /
+ * zyxb_device_sync) before the owner reads what a launch wrote. */
+int32_t zyxb_buffer_import(zyxb_ctx* ctx, int32_t dev, void* device_ptr, uint64_t bytes, uint32_t* out_buf);
 /* blocking; destroys the events */
 int32_t zyxb_sync(zyxb_ctx* ctx, int32_t dev, const zyxb_event* events, int32_t n);
 /* non-blocking destroy */

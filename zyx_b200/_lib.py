@@ -20,6 +20,7 @@ ERR_NAMES_INV = {name: code for code, name in ERR_NAMES.items()}
 BF16, F16, F32, F64, U8, U16, U32, U64, I8, I16, I32, I64, BOOL = range(13)
 DTYPE_SIZE = {BF16: 2, F16: 2, F32: 4, F64: 8, U8: 1, U16: 2, U32: 4, U64: 8, I8: 1, I16: 2, I32: 4, I64: 8, BOOL: 1}
 KIND_ROWREDUCE, KIND_GEMM, KIND_ELTWISE, KIND_OPTIM, KIND_ATTENTION, KIND_ATTENTION_BWD, KIND_CONV, KIND_CONV_WGRAD, KIND_CONV_DGRAD = 1, 2, 3, 4, 5, 6, 7, 8, 9
+KIND_EMBEDDING, KIND_EMBEDDING_BWD, KIND_RMSNORM, KIND_RMSNORM_BWD, KIND_MUON = 10, 11, 12, 13, 14
 (RR_SUM, RR_MAX, RR_MIN, RR_MEAN, RR_VAR, RR_STD, RR_SOFTMAX, RR_LN_SOFTMAX, RR_LAYERNORM, RR_CROSS_ENTROPY,
  RR_CROSS_ENTROPY_BWD, RR_SOFTMAX_BWD, RR_LAYERNORM_BWD, RR_COLSUM, RR_MSE, RR_LAYERNORM_DYXHAT) = range(16)
 EPI_NONE, EPI_BIAS, EPI_BIAS_RELU, EPI_BIAS_GELU, EPI_MUL_RELU_GRAD, EPI_MUL_GELU_GRAD, EPI_ADD = range(7)
@@ -27,6 +28,7 @@ TRI_NONE, TRI_OUT_LOWER, TRI_A_LOWER, TRI_AT_LOWER = range(4)
 (EW_RELU, EW_GELU, EW_ADD, EW_SUB, EW_MUL, EW_SCALE, EW_RELU_BWD, EW_GELU_BWD, EW_MSE_BWD, EW_CAST, EW_TANH, EW_SIGMOID,
  EW_EXP, EW_BIAS_ADD) = range(14)
 OPT_SGD, OPT_ADAM, OPT_ADAMW = range(3)
+MUON_ADJUST_RATIO, MUON_ADJUST_RMS = range(2)
 
 
 # ---- structs ---------------------------------------------------------------------------------
@@ -84,9 +86,26 @@ class ConvDesc(C.Structure):
                 ("pad_right", C.c_uint32), ("has_bias", C.c_int32), ("channels_last", C.c_int32), ("flip_filter", C.c_int32)]
 
 
+class EmbeddingDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("id_dtype", C.c_int32), ("tokens", C.c_uint64), ("vocab", C.c_uint64), ("dim", C.c_uint64),
+                ("ld_table", C.c_uint64), ("ld_out", C.c_uint64), ("scale", C.c_float), ("accumulate", C.c_int32)]
+
+
+class RmsnormDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("quant", C.c_int32), ("rows", C.c_uint64), ("cols", C.c_uint64), ("ld", C.c_uint64),
+                ("eps", C.c_float), ("has_residual", C.c_int32), ("has_weight", C.c_int32), ("has_dh", C.c_int32), ("group", C.c_uint32)]
+
+
+class MuonDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("n_tensors", C.c_int32), ("rows", C.POINTER(C.c_uint64)), ("cols", C.POINTER(C.c_uint64)),
+                ("lr", C.c_float), ("weight_decay", C.c_float), ("momentum", C.c_float), ("nesterov", C.c_int32), ("steps", C.c_int32),
+                ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float), ("grad_scale", C.c_float), ("adjust", C.c_int32)]
+
+
 class _DescUnion(C.Union):
     _fields_ = [("rowreduce", RowReduceDesc), ("gemm", GemmDesc), ("eltwise", EltwiseDesc), ("optim", OptimDesc),
-                ("attention", AttentionDesc), ("conv", ConvDesc)]
+                ("attention", AttentionDesc), ("conv", ConvDesc), ("embedding", EmbeddingDesc), ("rmsnorm", RmsnormDesc),
+                ("muon", MuonDesc)]
 
 
 class KernelDesc(C.Structure):
@@ -115,6 +134,7 @@ SIGNATURES = {
     "zyxb_memset": (C.c_int32, [_CTX, C.c_int32, C.c_uint32, C.c_uint64, C.c_int32, C.c_uint64]),
     "zyxb_buffer_bytes": (C.c_int32, [_CTX, C.c_int32, C.c_uint32, C.POINTER(C.c_uint64)]),
     "zyxb_buffer_view": (C.c_int32, [_CTX, C.c_int32, C.c_uint32, C.c_uint64, C.c_uint64, _U32_P]),
+    "zyxb_buffer_import": (C.c_int32, [_CTX, C.c_int32, C.c_void_p, C.c_uint64, _U32_P]),
     "zyxb_sync": (C.c_int32, [_CTX, C.c_int32, _EV_P, C.c_int32]),
     "zyxb_release_events": (C.c_int32, [_CTX, C.c_int32, _EV_P, C.c_int32]),
     "zyxb_device_sync": (C.c_int32, [_CTX, C.c_int32]),

@@ -147,6 +147,13 @@ class MemoryPool:
         self.be._check(self.be.lib.zyxb_buffer_view(self.be.ctx, self.dev, parent, int(offset), int(nbytes), C.byref(buf)))
         return buf.value
 
+    def import_device(self, device_ptr, nbytes):
+        """An id for device memory that another library of this process owns (256-byte aligned, on this device); the caller keeps it
+        alive and orders its own stream against this library's (zyxb_buffer_import).  deallocate releases only the id."""
+        buf = C.c_uint32()
+        self.be._check(self.be.lib.zyxb_buffer_import(self.be.ctx, self.dev, C.c_void_p(int(device_ptr)), int(nbytes), C.byref(buf)))
+        return buf.value
+
     def buffer_bytes(self, buffer_id):
         v = C.c_uint64()
         self.be._check(self.be.lib.zyxb_buffer_bytes(self.be.ctx, self.dev, buffer_id, C.byref(v)))
@@ -401,4 +408,38 @@ def optim_desc(algo, dtype, numels, lr, weight_decay=0.0, momentum=0.0, dampenin
     o.algo, o.dtype, o.n_tensors, o.numel = algo, dtype, len(numels), arr
     o.lr, o.weight_decay, o.momentum, o.dampening, o.nesterov, o.maximize = lr, weight_decay, momentum, dampening, int(nesterov), int(maximize)
     o.beta1, o.beta2, o.eps, o.grad_scale, o.standard = beta1, beta2, eps, grad_scale, int(standard)
+    return d
+
+
+def embedding_desc(dtype, tokens, vocab, dim, scale=0.0, id_dtype=L.I32, ld_table=0, ld_out=0, backward=False, accumulate=False):
+    d = L.KernelDesc()
+    d.kind = L.KIND_EMBEDDING_BWD if backward else L.KIND_EMBEDDING
+    e = d.u.embedding
+    e.dtype, e.id_dtype, e.tokens, e.vocab, e.dim, e.ld_table, e.ld_out = dtype, id_dtype, tokens, vocab, dim, ld_table, ld_out
+    e.scale, e.accumulate = scale, int(accumulate)
+    return d
+
+
+def rmsnorm_desc(dtype, rows, cols, eps=1e-6, has_residual=False, has_weight=False, ld=0, quant=False, group=0, backward=False,
+                 has_dh=False):
+    d = L.KernelDesc()
+    d.kind = L.KIND_RMSNORM_BWD if backward else L.KIND_RMSNORM
+    r = d.u.rmsnorm
+    r.dtype, r.quant, r.rows, r.cols, r.ld, r.eps = dtype, int(quant), rows, cols, ld, eps
+    r.has_residual, r.has_weight, r.has_dh, r.group = int(has_residual), int(has_weight), int(has_dh), group
+    return d
+
+
+def muon_desc(dtype, shapes, lr, weight_decay=0.0, momentum=0.95, nesterov=True, steps=0, coefficients=(0.0, 0.0, 0.0), eps=0.0,
+              grad_scale=0.0, adjust=L.MUON_ADJUST_RATIO):
+    """shapes: [(rows, cols)] of the matrices that one launch updates."""
+    d = L.KernelDesc()
+    d.kind = L.KIND_MUON
+    m = d.u.muon
+    rows, cols = (C.c_uint64 * len(shapes))(*[s[0] for s in shapes]), (C.c_uint64 * len(shapes))(*[s[1] for s in shapes])
+    d._shapes_keepalive = rows, cols
+    m.dtype, m.n_tensors, m.rows, m.cols = dtype, len(shapes), rows, cols
+    m.lr, m.weight_decay, m.momentum, m.nesterov, m.steps = lr, weight_decay, momentum, int(nesterov), steps
+    m.a, m.b, m.c = coefficients
+    m.eps, m.grad_scale, m.adjust = eps, grad_scale, adjust
     return d

@@ -8,6 +8,7 @@
 //   compute : every kernel, d2h, memset            (in-order: a launch sees all earlier launches)
 //   copy    : h2d, so uploads can overlap kernels  (ordered against compute by events)
 //   comm    : NCCL collectives                      (ordered against compute by events)
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdio.h>
 #include <string.h>
@@ -39,7 +40,9 @@ struct Buffer {
 
 struct Program {
   zyxb_kernel_desc desc{};
-  std::vector<uint64_t> numel;  // optimizer programs: copy of desc.u.optim.numel
+  std::vector<uint64_t> numel;  // optimizer programs: copy of desc.u.optim.numel; Muon: rows, then cols of its matrices
+  void* workspace = nullptr;    // Muon: memory of its products, owned by the program
+  uint64_t workspace_bytes = 0;
   uint64_t step = 0;            // optimizer programs: AdamW::t
   bool live = false;
 };
@@ -67,6 +70,7 @@ struct Device {
   uint64_t launch_count = 0;
   void* tma_encode = nullptr;
   void* tma_encode_im2col = nullptr;
+  void* address_range = nullptr;          // cuMemGetAddressRange
   Comm* comm = nullptr;
   PeerComm* peer = nullptr;               // allreduce over peer memory (peer_allreduce.cu); created with the communicator
   int comm_latency = 0;                   // ZYXB_COMM_OPT_LATENCY: allreduces take the communicator's own path
@@ -197,6 +201,19 @@ cudaError_t device_malloc(Device& D, uint64_t capacity, void** out) {
   return e;
 }
 
+// A block goes back to the cache and may be handed out again at once: kernels already queued on the compute stream are in order
+// with later ones; the event keeps the other streams behind them.
+void recycle_block(Device& D, void* ptr, uint64_t capacity) {
+  cudaEvent_t ready = nullptr;
+  if (cudaEventCreateWithFlags(&ready, cudaEventDisableTiming) != cudaSuccess || cudaEventRecord(ready, D.compute) != cudaSuccess) {
+    cudaGetLastError();
+    if (ready) { cudaEventDestroy(ready); ready = nullptr; }
+    cudaStreamSynchronize(D.compute);      // no event to hand on: the block is idle before it enters the cache
+  }
+  D.cache.emplace(capacity, Device::CachedBlock{ptr, ready});
+  D.cached_bytes += capacity;
+}
+
 LaunchCtx make_launch_ctx(zyxb_ctx* ctx, Device& D) {
   LaunchCtx lc{};
   lc.stream = D.compute; lc.round_nearest = ctx->round_nearest; lc.sm_count = D.prop.multiProcessorCount;
@@ -265,6 +282,10 @@ int32_t zyxb_init(const zyxb_config* config, zyxb_ctx** out_ctx) {
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeIm2col", &fn, cudaEnableDefault, &qres) == cudaSuccess && qres == cudaDriverEntryPointSuccess)
       D.tma_encode_im2col = fn;
     else cudaGetLastError();
+    fn = nullptr;
+    if (cudaGetDriverEntryPoint("cuMemGetAddressRange", &fn, cudaEnableDefault, &qres) == cudaSuccess && qres == cudaDriverEntryPointSuccess)
+      D.address_range = fn;
+    else cudaGetLastError();
     D.buffers.emplace_back();   // id 0 is never handed out
     D.programs.emplace_back();
     if (ctx->debug & 1) fprintf(stderr, "[zyxb] device %d: %s, %d SMs, %.1f GB\n", id, D.prop.name, D.prop.multiProcessorCount, D.prop.totalGlobalMem / 1e9);
@@ -285,6 +306,7 @@ int32_t zyxb_shutdown(zyxb_ctx* ctx) {
     for (auto& g : D.graphs) if (g.first) cudaGraphExecDestroy(g.first);
     for (auto& kv : D.events) cudaEventDestroy(kv.second);
     for (auto& b : D.buffers) if (b.live && b.ptr && !b.is_view && !b.is_variable) cudaFree(b.ptr);
+    for (auto& P : D.programs) if (P.workspace) cudaFree(P.workspace);
     for (auto& kv : D.cache) { if (kv.second.ready) cudaEventDestroy(kv.second.ready); cudaFree(kv.second.ptr); }
     if (D.scratch) cudaFree(D.scratch);
     if (D.status_word) cudaFree(D.status_word);
@@ -379,14 +401,7 @@ int32_t zyxb_free(zyxb_ctx* ctx, int32_t dev, uint32_t buf, const zyxb_event* wa
   } else if (!b->is_variable && !b->is_view) {
     if ((st = order_streams(ctx, D.copy, D.compute, ZYXB_ERR_MEMORY_DEALLOCATION))) return st;
     if ((st = order_streams(ctx, D.comm_stream, D.compute, ZYXB_ERR_MEMORY_DEALLOCATION))) return st;
-    cudaEvent_t ready = nullptr;
-    if (cudaEventCreateWithFlags(&ready, cudaEventDisableTiming) != cudaSuccess || cudaEventRecord(ready, D.compute) != cudaSuccess) {
-      cudaGetLastError();
-      if (ready) { cudaEventDestroy(ready); ready = nullptr; }
-      cudaStreamSynchronize(D.compute);      // no event to hand on: the block is idle before it enters the cache
-    }
-    D.cache.emplace(b->capacity, Device::CachedBlock{b->ptr, ready});
-    D.cached_bytes += b->capacity;
+    recycle_block(D, b->ptr, b->capacity);
   }
   *b = Buffer();
   D.free_buffer_ids.push_back(buf);
@@ -407,6 +422,32 @@ int32_t zyxb_buffer_view(zyxb_ctx* ctx, int32_t dev, uint32_t parent, uint64_t o
   b = Buffer();
   b.ptr = ptr; b.bytes = bytes; b.capacity = bytes; b.live = true; b.is_view = true;
   b.parent = D.buffers[parent].is_view ? D.buffers[parent].parent : parent;
+  *out_buf = id;
+  return ZYXB_OK;
+}
+
+int32_t zyxb_buffer_import(zyxb_ctx* ctx, int32_t dev, void* device_ptr, uint64_t bytes, uint32_t* out_buf) {
+  DEV_OR_FAIL(ZYXB_ERR_MEMORY_ALLOCATION);
+  if (!device_ptr || !bytes || !out_buf) return fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "buffer_import: null argument or no bytes");
+  if ((uintptr_t)device_ptr % 256 != 0) return fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "buffer_import: the address must be a multiple of 256 bytes");
+  cudaPointerAttributes at{};
+  cudaError_t e = cudaPointerGetAttributes(&at, device_ptr);
+  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "buffer_import", e); }
+  if (at.type != cudaMemoryTypeDevice || at.device != D.cuda_id) return fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "buffer_import: not memory of this device");
+  if (D.address_range) {      // the whole range belongs to the allocation the address lies in
+    CUdeviceptr base = 0;
+    size_t size = 0;
+    if (reinterpret_cast<CUresult (*)(CUdeviceptr*, size_t*, CUdeviceptr)>(D.address_range)(&base, &size, (CUdeviceptr)device_ptr) != CUDA_SUCCESS ||
+        !range_ok((uint64_t)((CUdeviceptr)device_ptr - base), bytes, size))
+      return fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "buffer_import: range exceeds the allocation");
+  }
+  uint32_t id;
+  if (!D.free_buffer_ids.empty()) { id = D.free_buffer_ids.back(); D.free_buffer_ids.pop_back(); }
+  else { id = (uint32_t)D.buffers.size(); D.buffers.emplace_back(); }
+  Buffer& b = D.buffers[id];
+  b = Buffer();
+  b.ptr = device_ptr; b.bytes = bytes; b.capacity = bytes; b.live = true;
+  b.is_view = true; b.parent = id;       // like a view: freeing it releases the id, the owner keeps the memory
   *out_buf = id;
   return ZYXB_OK;
 }
@@ -582,9 +623,20 @@ int32_t zyxb_program_create(zyxb_ctx* ctx, int32_t dev, const zyxb_kernel_desc* 
     case ZYXB_KIND_OPTIM: st = validate_optim(desc->u.optim, err); break;
     case ZYXB_KIND_ATTENTION: case ZYXB_KIND_ATTENTION_BWD: st = validate_attention(desc->u.attention, err); break;
     case ZYXB_KIND_CONV: case ZYXB_KIND_CONV_WGRAD: case ZYXB_KIND_CONV_DGRAD: st = validate_conv(desc->u.conv, err); break;
+    case ZYXB_KIND_EMBEDDING: case ZYXB_KIND_EMBEDDING_BWD: st = validate_embedding(desc->u.embedding, desc->kind == ZYXB_KIND_EMBEDDING_BWD, err); break;
+    case ZYXB_KIND_RMSNORM: case ZYXB_KIND_RMSNORM_BWD: st = validate_rmsnorm(desc->u.rmsnorm, desc->kind == ZYXB_KIND_RMSNORM_BWD, err); break;
+    case ZYXB_KIND_MUON: st = validate_muon(desc->u.muon, err); break;
     default: st = ZYXB_ERR_KERNEL_COMPILATION; err = "unknown kernel kind";
   }
   if (st) return fail(ctx, st, err);
+  void* workspace = nullptr;
+  uint64_t workspace_bytes = 0;
+  if (desc->kind == ZYXB_KIND_MUON) {
+    NOT_WHILE_CAPTURING("zyxb_program_create of a Muon program", ZYXB_ERR_KERNEL_COMPILATION);
+    workspace_bytes = round_up(muon_workspace_bytes(desc->u.muon, desc->u.muon.rows, desc->u.muon.cols), 512);
+    cudaError_t e = device_malloc(D, workspace_bytes, &workspace);
+    if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "program_create: workspace", e); }
+  }
   uint32_t id;
   if (!D.free_program_ids.empty()) { id = D.free_program_ids.back(); D.free_program_ids.pop_back(); }
   else { id = (uint32_t)D.programs.size(); D.programs.emplace_back(); }
@@ -595,6 +647,13 @@ int32_t zyxb_program_create(zyxb_ctx* ctx, int32_t dev, const zyxb_kernel_desc* 
     P.numel.assign(desc->u.optim.numel, desc->u.optim.numel + desc->u.optim.n_tensors);
     P.desc.u.optim.numel = nullptr;   // the caller's array need not outlive this call
   }
+  if (desc->kind == ZYXB_KIND_MUON) {
+    const zyxb_muon_desc& m = desc->u.muon;
+    P.numel.assign(m.rows, m.rows + m.n_tensors);
+    P.numel.insert(P.numel.end(), m.cols, m.cols + m.n_tensors);
+    P.desc.u.muon.rows = P.desc.u.muon.cols = nullptr;
+    P.workspace = workspace; P.workspace_bytes = workspace_bytes;
+  }
   *out_prog = id;
   return ZYXB_OK;
 }
@@ -602,6 +661,10 @@ int32_t zyxb_program_create(zyxb_ctx* ctx, int32_t dev, const zyxb_kernel_desc* 
 int32_t zyxb_program_release(zyxb_ctx* ctx, int32_t dev, uint32_t prog) {
   DEV_OR_FAIL(ZYXB_ERR_KERNEL_COMPILATION);
   if (prog == 0 || prog >= D.programs.size() || !D.programs[prog].live) return fail(ctx, ZYXB_ERR_KERNEL_COMPILATION, "release: unknown program");
+  if (D.programs[prog].workspace) {
+    NOT_WHILE_CAPTURING("zyxb_program_release of a Muon program", ZYXB_ERR_KERNEL_COMPILATION);
+    recycle_block(D, D.programs[prog].workspace, D.programs[prog].workspace_bytes);
+  }
   D.programs[prog] = Program();
   D.free_program_ids.push_back(prog);
   return ZYXB_OK;
@@ -659,6 +722,13 @@ int32_t zyxb_launch(zyxb_ctx* ctx, int32_t dev, uint32_t prog, const uint32_t* a
     case ZYXB_KIND_CONV: st = launch_conv(P.desc.u.conv, ptrs.data(), sizes.data(), n_args, lc, err); break;
     case ZYXB_KIND_CONV_DGRAD: st = launch_conv_dgrad(P.desc.u.conv, ptrs.data(), sizes.data(), n_args, lc, err); break;
     case ZYXB_KIND_CONV_WGRAD: st = launch_conv_wgrad(P.desc.u.conv, ptrs.data(), sizes.data(), n_args, lc, err); break;
+    case ZYXB_KIND_EMBEDDING: st = launch_embedding(P.desc.u.embedding, ptrs.data(), sizes.data(), n_args, lc, err); break;
+    case ZYXB_KIND_EMBEDDING_BWD: st = launch_embedding_bwd(P.desc.u.embedding, ptrs.data(), sizes.data(), n_args, lc, err); break;
+    case ZYXB_KIND_RMSNORM: st = launch_rmsnorm(P.desc.u.rmsnorm, ptrs.data(), sizes.data(), n_args, lc, err); break;
+    case ZYXB_KIND_RMSNORM_BWD: st = launch_rmsnorm_bwd(P.desc.u.rmsnorm, ptrs.data(), sizes.data(), n_args, lc, err); break;
+    case ZYXB_KIND_MUON:
+      st = launch_muon(P.desc.u.muon, P.numel.data(), P.numel.data() + P.numel.size() / 2, P.workspace, ptrs.data(), sizes.data(), n_args, lc, err);
+      break;
     case ZYXB_KIND_OPTIM:
       st = launch_optim(P.desc.u.optim, P.numel.data(), P.step + 1, ptrs.data(), sizes.data(), n_args, lc, err);
       if (st == ZYXB_OK && !D.capturing) P.step += 1;     // a captured launch has not run

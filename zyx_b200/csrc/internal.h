@@ -47,6 +47,18 @@ int validate_conv(const zyxb_conv_desc& d, std::string& err);
 int launch_conv_dgrad(const zyxb_conv_desc& d, void* const* args, const uint64_t* arg_bytes, int n_args, const LaunchCtx& lc, std::string& err);
 int launch_conv_wgrad(const zyxb_conv_desc& d, void* const* args, const uint64_t* arg_bytes, int n_args, const LaunchCtx& lc, std::string& err);
 
+int validate_embedding(const zyxb_embedding_desc& d, bool backward, std::string& err);
+int launch_embedding(const zyxb_embedding_desc& d, void* const* args, const uint64_t* arg_bytes, int n_args, const LaunchCtx& lc, std::string& err);
+int launch_embedding_bwd(const zyxb_embedding_desc& d, void* const* args, const uint64_t* arg_bytes, int n_args, const LaunchCtx& lc, std::string& err);
+int validate_rmsnorm(const zyxb_rmsnorm_desc& d, bool backward, std::string& err);
+int launch_rmsnorm(const zyxb_rmsnorm_desc& d, void* const* args, const uint64_t* arg_bytes, int n_args, const LaunchCtx& lc, std::string& err);
+int launch_rmsnorm_bwd(const zyxb_rmsnorm_desc& d, void* const* args, const uint64_t* arg_bytes, int n_args, const LaunchCtx& lc, std::string& err);
+// Muon: extents of the program's matrices; the workspace is owned by the program
+int validate_muon(const zyxb_muon_desc& d, std::string& err);
+uint64_t muon_workspace_bytes(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols);
+int launch_muon(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols, void* workspace, void* const* args,
+                const uint64_t* arg_bytes, int n_args, const LaunchCtx& lc, std::string& err);
+
 // column sums with the partials in a fixed device array (no allocation anywhere on the path)
 int launch_colsum_static(int dtype, const void* x, void* y, uint64_t rows, uint64_t cols, const LaunchCtx& lc, std::string& err);
 uint64_t colsum_static_capacity();

@@ -1,0 +1,516 @@
+// Root-mean-square norm with the residual's addition, its 8-bit output, and its adjoint.
+//   h = x + r,  y = h * rstd * w,  rstd = 1 / sqrt(mean(h^2) + eps)
+//   adjoint: with the row sums  S = sum h^2  and  P = sum dy w h  taken in one pass,
+//     dx = rstd * dy w - h * rstd^3 * P / cols (+ dh),   dw = sum over rows of dy h rstd
+// Bound by HBM: every element is read once, kept in registers between the sum and the store, and written once.
+//
+// A group of `tpr` threads (a power of two, 8..1024) holds one row as 16-byte vectors, PACKS per thread.  Rows whose start is not
+// on a 16-byte boundary (odd pitches) are covered by the aligned vectors that contain them: vectors inside the row move as a
+// whole, the two that hang over its ends element by element.  Sums are f32.
+#include <algorithm>
+
+#include "internal.h"
+#include "rounding.cuh"
+
+namespace zyxb {
+
+namespace {
+
+constexpr uint64_t RMS_MAX_COLS = 16384;
+
+struct RmsParams {
+  const void *x, *residual, *weight, *dy, *dh;
+  void *h, *y, *dweight;
+  float *scales, *partial;
+  uint64_t rows, ld;
+  uint32_t cols, group, n_groups;
+  float eps;
+  int log_tpr, rn, residual_on, weight_on, dh_on;
+};
+
+// sum over the group's threads of up to two values; `parity` alternates between calls, so one barrier per call is enough
+template <int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int log_tpr, float (*buf)[32][N], int parity) {
+  const int width = min(32, 1 << log_tpr);
+  for (int o = width >> 1; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
+  if (log_tpr > 5) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wpr = 1 << (log_tpr - 5);
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) buf[parity][warp][i] = v[i];
+    }
+    __syncthreads();
+    const int first = warp & ~(wpr - 1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lane < wpr ? buf[parity][first + lane][i] : 0.0f;
+    for (int o = wpr >> 1; o > 0; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, v[i], 0);
+  }
+}
+
+// One row seen through aligned vectors: element 0 of vector 0 is `off` elements before the row.
+template <typename T, bool ALIGNED>
+struct RowView {
+  using S = typename Elem<T>::store_t;
+  static constexpr int VEC = 16 / (int)sizeof(S);
+  uint64_t start;      // element index of vector 0 (a multiple of VEC)
+  int off, cols;
+  __device__ __forceinline__ RowView(uint64_t row, uint64_t ld, uint32_t cols_) : cols((int)cols_) {
+    const uint64_t at = row * ld;
+    off = ALIGNED ? 0 : (int)(at % VEC);
+    start = at - off;
+  }
+  __device__ __forceinline__ bool has(int pack) const { return pack * VEC < off + cols; }
+  __device__ __forceinline__ int col(int pack) const { return pack * VEC - off; }                 // may be negative
+  __device__ __forceinline__ bool whole(int pack) const { return ALIGNED || (col(pack) >= 0 && col(pack) + VEC <= cols); }
+  __device__ __forceinline__ bool inside(int c) const { return ALIGNED || ((unsigned)c < (unsigned)cols); }
+  // zeros outside the row
+  __device__ __forceinline__ void load(RawVec<T, VEC>& r, const void* base, int pack) const {
+    const S* p = reinterpret_cast<const S*>(base) + start + (uint64_t)pack * VEC;
+    if (whole(pack)) { r.load_stream(p); return; }
+    float v[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = inside(col(pack) + k) ? Elem<T>::load(p[k]) : 0.0f;
+    r.encode(v, false);          // exact: the values are of the storage type
+  }
+  __device__ __forceinline__ void store(const float (&v)[VEC], void* base, int pack, bool rn) const {
+    S* p = reinterpret_cast<S*>(base) + start + (uint64_t)pack * VEC;
+    if (whole(pack)) {
+      RawVec<T, VEC> r;
+      round_encode<T, VEC>(r, v, rn);
+      r.store_stream(p);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      if (inside(col(pack) + k)) p[k] = round_store<T>(v[k], rn);
+  }
+  // the weight's entries under a vector (the weight itself starts on a boundary, the row need not)
+  __device__ __forceinline__ void weight(float (&v)[VEC], const void* w, int pack) const {
+    const S* p = reinterpret_cast<const S*>(w);
+    if constexpr (ALIGNED) {
+      RawVec<T, VEC> r;
+      r.load(p + pack * VEC);
+      r.decode(v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[k] = inside(col(pack) + k) ? Elem<T>::load(p[col(pack) + k]) : 0.0f;
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+constexpr float E4M3_MAX = 448.0f, AMAX_FLOOR = 1e-30f;
+
+template <typename T, int PACKS, bool ALIGNED, bool QUANT>
+__global__ void __launch_bounds__(1024) rmsnorm_kernel(RmsParams p) {
+  using View = RowView<T, ALIGNED>;
+  constexpr int VEC = View::VEC;
+  __shared__ float red[2][32][1];
+  extern __shared__ uint32_t amax_bits[];            // QUANT: largest |y| of each column group, per row of the CTA, as its bits
+  const int tpr = 1 << p.log_tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & (tpr - 1);
+  const uint64_t row = (uint64_t)blockIdx.x * (blockDim.x >> p.log_tpr) + in_cta;
+  const bool live = row < p.rows;
+  const View view(live ? row : 0, p.ld, p.cols);
+  float h[PACKS][VEC];
+  float sum[1] = {0.0f};
+  {
+    RawVec<T, VEC> rx[PACKS], rr[PACKS];
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      const int pack = t + i * tpr;
+      rx[i].zero(); rr[i].zero();
+      if (live && view.has(pack)) {
+        view.load(rx[i], p.x, pack);
+        if (p.residual_on) view.load(rr[i], p.residual, pack);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      const int pack = t + i * tpr;
+      rx[i].decode(h[i]);
+      if (p.residual_on) {
+        float r[VEC];
+        rr[i].decode(r);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) h[i][k] += r[k];
+        if (live && view.has(pack)) view.store(h[i], p.h, pack, p.rn != 0);
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum[0] += h[i][k] * h[i][k];
+    }
+  }
+  if constexpr (QUANT) {
+    for (uint32_t g = threadIdx.x; g < (blockDim.x >> p.log_tpr) * p.n_groups; g += blockDim.x) amax_bits[g] = __float_as_uint(AMAX_FLOOR);
+    if (p.log_tpr <= 5) __syncthreads();             // wider rows pass a barrier in row_sum
+  }
+  row_sum(sum, p.log_tpr, red, 0);
+  const float rstd = 1.0f / sqrtf(sum[0] / (float)p.cols + p.eps);
+#pragma unroll
+  for (int i = 0; i < PACKS; ++i) {
+    const int pack = t + i * tpr;
+    if (!live || !view.has(pack)) continue;
+    if (p.weight_on) {
+      float w[VEC];
+      view.weight(w, p.weight, pack);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * rstd * w[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) h[i][k] *= rstd;
+    }
+    if constexpr (!QUANT) view.store(h[i], p.y, pack, p.rn != 0);
+  }
+  if constexpr (QUANT) {
+    // The bits of |y| order like the values, and a NaN above all of them: it becomes its group's scale.
+    uint32_t* mine = amax_bits + in_cta * p.n_groups;
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      const int pack = t + i * tpr;
+      if (!live || !view.has(pack)) continue;
+      const int c0 = max(0, view.col(pack)), c1 = min((int)p.cols, view.col(pack) + VEC) - 1;
+      const uint32_t g0 = (uint32_t)c0 / p.group, g1 = (uint32_t)c1 / p.group;
+      uint32_t m0 = 0, m1 = 0;                       // a vector meets at most two groups
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const int c = view.col(pack) + k;
+        if (!view.inside(c)) continue;
+        const uint32_t b = __float_as_uint(h[i][k]) & 0x7fffffffu;
+        if ((uint32_t)c < (g0 + 1) * p.group) m0 = max(m0, b); else m1 = max(m1, b);
+      }
+      atomicMax(&mine[g0], m0);
+      if (g1 != g0) atomicMax(&mine[g1], m1);
+    }
+    __syncthreads();
+    uint8_t* y = reinterpret_cast<uint8_t*>(p.y) + row * p.cols;
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      const int pack = t + i * tpr;
+      if (!live || !view.has(pack)) continue;
+      const int c0 = view.col(pack);
+      float q[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const int c = min(max(c0 + k, 0), (int)p.cols - 1);
+        q[k] = h[i][k] / (__uint_as_float(mine[(uint32_t)c / p.group]) / E4M3_MAX);
+      }
+      uint32_t w[VEC / 4];
+#pragma unroll
+      for (int k = 0; k < VEC / 4; ++k) w[k] = e4m3x2(q[4 * k], q[4 * k + 1]) | (e4m3x2(q[4 * k + 2], q[4 * k + 3]) << 16);
+      if (ALIGNED) {
+        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(y + c0) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(y + c0) = w[0];
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          if (view.inside(c0 + k)) y[c0 + k] = (uint8_t)(w[k / 4] >> (8 * (k % 4)));
+      }
+    }
+    if (live)
+      for (uint32_t g = t; g < p.n_groups; g += tpr) p.scales[row * p.n_groups + g] = __uint_as_float(mine[g]) / E4M3_MAX;
+  }
+}
+
+// Rows are dealt to the groups of a persistent grid, so that a thread keeps the weight gradient of its columns in registers (or,
+// where rows start at odd places and a column wanders between threads, in shared memory) until its last row.
+template <typename T, int PACKS, bool ALIGNED>
+__global__ void __launch_bounds__(1024) rmsnorm_bwd_kernel(RmsParams p) {
+  using View = RowView<T, ALIGNED>;
+  constexpr int VEC = View::VEC;
+  __shared__ float red[2][32][2];
+  extern __shared__ float dw_shared[];               // [group of the CTA][cols]
+  const int tpr = 1 << p.log_tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & (tpr - 1), groups = blockDim.x >> p.log_tpr;
+  float* dw_mine = dw_shared + (size_t)in_cta * p.cols;
+  float dw[PACKS][VEC];
+#pragma unroll
+  for (int i = 0; i < PACKS; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) dw[i][k] = 0.0f;
+  if (!ALIGNED && p.weight_on)
+    for (uint32_t c = t; c < p.cols; c += tpr) dw_mine[c] = 0.0f;
+  const uint64_t step = (uint64_t)gridDim.x * groups;
+  int parity = 0;
+  for (uint64_t row0 = (uint64_t)blockIdx.x * groups; row0 < p.rows; row0 += step, parity ^= 1) {
+    const uint64_t row = row0 + in_cta;
+    const bool live = row < p.rows;
+    const View view(live ? row : 0, p.ld, p.cols);
+    RawVec<T, VEC> rh[PACKS], rg[PACKS], rd[PACKS];
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      const int pack = t + i * tpr;
+      rh[i].zero(); rg[i].zero(); rd[i].zero();
+      if (live && view.has(pack)) {
+        view.load(rh[i], p.h, pack);
+        view.load(rg[i], p.dy, pack);
+        if (p.dh_on) view.load(rd[i], p.dh, pack);
+      }
+    }
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      const int pack = t + i * tpr;
+      float h[VEC], g[VEC];
+      rh[i].decode(h);
+      rg[i].decode(g);
+      if (p.weight_on && live && view.has(pack)) {
+        float w[VEC];
+        view.weight(w, p.weight, pack);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) g[k] *= w[k];
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) { s[0] += h[k] * h[k]; s[1] += g[k] * h[k]; }
+    }
+    row_sum(s, p.log_tpr, red, parity);
+    const float rstd = 1.0f / sqrtf(s[0] / (float)p.cols + p.eps);
+    const float pull = rstd * rstd * (s[1] / (float)p.cols);          // dx = rstd * (dy w - h * pull)
+    if (!ALIGNED) __syncwarp();
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      const int pack = t + i * tpr;
+      if (!live || !view.has(pack)) continue;
+      float h[VEC], g[VEC], o[VEC];
+      rh[i].decode(h);
+      rg[i].decode(g);
+      if (p.weight_on) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const float d = g[k] * (h[k] * rstd);
+          if constexpr (ALIGNED) dw[i][k] += d;
+          else if (view.inside(view.col(pack) + k)) dw_mine[view.col(pack) + k] += d;
+        }
+        float w[VEC];
+        view.weight(w, p.weight, pack);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) g[k] *= w[k];
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) o[k] = rstd * (g[k] - h[k] * pull);
+      if (p.dh_on) {
+        float d[VEC];
+        rd[i].decode(d);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o[k] += d[k];
+      }
+      view.store(o, p.y, pack, p.rn != 0);
+    }
+  }
+  if (!p.weight_on) return;
+  // the CTA's groups are added in order, then one row of partials per CTA
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      const int pack = t + i * tpr;
+      if ((uint32_t)pack * VEC < p.cols) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) dw_mine[pack * VEC + k] = dw[i][k];
+      }
+    }
+  }
+  __syncthreads();
+  for (uint32_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
+    float sum = 0.0f;
+    for (int g = 0; g < groups; ++g) sum += dw_shared[(size_t)g * p.cols + c];
+    p.partial[(uint64_t)blockIdx.x * p.cols + c] = sum;
+  }
+}
+
+// dweight[c] = sum over the CTAs' partials, in order: 32 columns per CTA, 8 warps share the list
+template <typename T>
+__global__ void __launch_bounds__(256) rmsnorm_dweight_kernel(const float* __restrict__ partial, uint32_t n, uint32_t cols, typename Elem<T>::store_t* dweight, int rn) {
+  __shared__ float part[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t c = blockIdx.x * 32 + lane;
+  float sum = 0.0f;
+  if (c < cols) {
+#pragma unroll 16
+    for (uint32_t i = warp; i < n; i += 8) sum += partial[(uint64_t)i * cols + c];
+  }
+  part[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && c < cols) {
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += part[w][lane];
+    dweight[c] = round_store<T>(v, rn != 0);
+  }
+}
+
+int log2_up(uint64_t v) {
+  int l = 0;
+  while ((1ull << l) < v) ++l;
+  return l;
+}
+
+struct RmsShape { bool aligned; int log_tpr, packs, threads; };
+
+// vectors that cover a row, one per thread up to `most` threads; a row's group is at least 8 threads wide
+template <typename T>
+RmsShape rms_shape(const RmsParams& p, int most_log) {
+  constexpr int VEC = 16 / (int)sizeof(typename Elem<T>::store_t);
+  RmsShape s{};
+  s.aligned = p.cols % VEC == 0 && p.ld % VEC == 0;
+  const uint64_t vectors = s.aligned ? p.cols / VEC : (p.cols + 2 * VEC - 2) / VEC;
+  s.log_tpr = std::min(most_log, std::max(3, log2_up(vectors)));
+  const int need = (int)((vectors + (1u << s.log_tpr) - 1) >> s.log_tpr);
+  s.packs = 1;
+  while (s.packs < need) s.packs *= 2;
+  s.threads = std::max(256, 1 << s.log_tpr);
+  return s;
+}
+
+template <typename T, int PACKS, bool ALIGNED>
+cudaError_t run_rms(const RmsParams& p, const RmsShape& s, bool quant, const LaunchCtx& lc) {
+  const uint64_t per_cta = (uint64_t)(s.threads >> s.log_tpr);
+  const unsigned grid = (unsigned)((p.rows + per_cta - 1) / per_cta);
+  if (quant) rmsnorm_kernel<T, PACKS, ALIGNED, true><<<grid, s.threads, per_cta * p.n_groups * 4, lc.stream>>>(p);
+  else rmsnorm_kernel<T, PACKS, ALIGNED, false><<<grid, s.threads, 0, lc.stream>>>(p);
+  return cudaSuccess;
+}
+
+template <typename T, int PACKS, bool ALIGNED>
+cudaError_t run_rms_bwd(RmsParams& p, const RmsShape& s, unsigned* grid_out, const LaunchCtx& lc) {
+  const int groups = s.threads >> s.log_tpr;
+  const size_t smem = p.weight_on ? (size_t)groups * p.cols * 4 : 0;
+  static uint64_t configured = 0;
+  cudaError_t e = ensure_dynamic_smem(rmsnorm_bwd_kernel<T, PACKS, ALIGNED>, 80 << 10, &configured);
+  if (e != cudaSuccess) return e;
+  const uint64_t work = (p.rows + groups - 1) / groups;
+  *grid_out = (unsigned)std::min<uint64_t>(work, (uint64_t)lc.sm_count * std::max(1, 2048 / s.threads / 2));
+  rmsnorm_bwd_kernel<T, PACKS, ALIGNED><<<*grid_out, s.threads, smem, lc.stream>>>(p);
+  return cudaSuccess;
+}
+
+// 16384 columns are 1024 threads x 2 vectors of 16-bit elements or x 4 of f32; rows off the boundary can need one vector more
+#define ZYXB_RMS_PACKS(CALL)                                                                       \
+  constexpr bool wide = sizeof(T) == 4;                                                            \
+  if (s.packs == 1) e = s.aligned ? CALL(1, true) : CALL(1, false);                                \
+  else if (s.packs == 2) e = s.aligned ? CALL(2, true) : CALL(2, false);                           \
+  else if (s.packs == 4 && !s.aligned) e = CALL(4, false);                                         \
+  else if constexpr (wide) { if (s.packs == 4) e = CALL(4, true); else e = CALL(8, false); }
+
+template <typename T>
+cudaError_t rms_forward(const RmsParams& p, bool quant, const LaunchCtx& lc) {
+  RmsParams q = p;
+  const RmsShape s = rms_shape<T>(p, 10);
+  q.log_tpr = s.log_tpr;
+  cudaError_t e = cudaSuccess;
+#define ZYXB_RMS_FWD(P, A) (run_rms<T, P, A>(q, s, quant, lc))
+  ZYXB_RMS_PACKS(ZYXB_RMS_FWD)
+#undef ZYXB_RMS_FWD
+  return e;
+}
+
+template <typename T>
+cudaError_t rms_backward(const RmsParams& p, const LaunchCtx& lc) {
+  using S = typename Elem<T>::store_t;
+  RmsParams q = p;
+  const RmsShape s = rms_shape<T>(p, 10);
+  q.log_tpr = s.log_tpr;
+  unsigned grid = 0;
+  cudaError_t e = cudaSuccess;
+#define ZYXB_RMS_BWD(P, A) (run_rms_bwd<T, P, A>(q, s, &grid, lc))
+  ZYXB_RMS_PACKS(ZYXB_RMS_BWD)
+#undef ZYXB_RMS_BWD
+  if (e == cudaSuccess && p.weight_on)
+    rmsnorm_dweight_kernel<T><<<(p.cols + 31) / 32, 256, 0, lc.stream>>>(q.partial, grid, p.cols, (S*)q.dweight, q.rn);
+  return e;
+}
+
+bool rows_fit(const zyxb_rmsnorm_desc& d, uint64_t ld, uint64_t bytes) {
+  return (unsigned __int128)dtype_size(d.dtype) * ((unsigned __int128)(d.rows - 1) * ld + d.cols) <= bytes;
+}
+
+}  // namespace
+
+int validate_rmsnorm(const zyxb_rmsnorm_desc& d, bool backward, std::string& err) {
+  auto bad = [&](const char* m) { err = m; return (int)ZYXB_ERR_KERNEL_COMPILATION; };
+  if (d.dtype != ZYXB_F32 && d.dtype != ZYXB_BF16 && d.dtype != ZYXB_F16) return bad("rmsnorm: dtype must be f32, bf16 or f16");
+  if (d.rows == 0 || d.cols == 0) return bad("rmsnorm: rows and cols must be positive");
+  if (d.cols > RMS_MAX_COLS) return bad("rmsnorm: cols must be at most 16384");
+  if (d.rows > 0x7fffffffull) return bad("rmsnorm: rows must be below 2^31");
+  if ((d.ld && d.ld < d.cols) || d.ld > (1ull << 40)) return bad("rmsnorm: row pitch smaller than the row, or too large");
+  if (!(d.eps >= 0.0f)) return bad("rmsnorm: eps must not be negative");
+  if (d.quant != 0 && d.quant != 1) return bad("rmsnorm: quant must be 0 or 1");
+  if (backward && (d.quant || d.has_residual)) return bad("rmsnorm backward: takes h, the stored sum; quant and has_residual are options of the forward");
+  if (!backward && d.has_dh) return bad("rmsnorm: has_dh is an option of the backward");
+  if (d.group && (!d.quant || d.group < 16)) return bad("rmsnorm: group needs quant and must be at least 16");
+  return ZYXB_OK;
+}
+
+int launch_rmsnorm(const zyxb_rmsnorm_desc& d, void* const* args, const uint64_t* arg_bytes, int n_args, const LaunchCtx& lc, std::string& err) {
+  const int want = 1 + (d.has_residual ? 2 : 0) + (d.has_weight ? 1 : 0) + 1 + (d.quant ? 1 : 0);
+  ZYXB_CHECK_ARG(n_args == want, "rmsnorm: expected args x [,residual] [,weight] -> [h,] y [,scales]");
+  const uint64_t es = dtype_size(d.dtype);
+  RmsParams p{};
+  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.eps = d.eps; p.rn = lc.round_nearest ? 1 : 0;
+  p.residual_on = d.has_residual ? 1 : 0; p.weight_on = d.has_weight ? 1 : 0;
+  p.group = d.group ? std::min<uint32_t>(d.group, p.cols) : p.cols;
+  p.n_groups = (p.cols + p.group - 1) / p.group;
+  int i = 0;
+  ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm: x too small"); p.x = args[i++];
+  if (d.has_residual) { ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm: residual too small"); p.residual = args[i++]; }
+  if (d.has_weight) { ZYXB_CHECK_ARG(arg_bytes[i] >= d.cols * es, "rmsnorm: weight too small"); p.weight = args[i++]; }
+  if (d.has_residual) { ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm: h too small"); p.h = args[i++]; }
+  if (d.quant) {
+    ZYXB_CHECK_ARG(arg_bytes[i] >= d.rows * d.cols, "rmsnorm: y too small"); p.y = args[i++];
+    ZYXB_CHECK_ARG(arg_bytes[i] >= d.rows * p.n_groups * 4, "rmsnorm: scales too small"); p.scales = (float*)args[i++];
+    ZYXB_CHECK_ARG(p.y != p.x && p.y != p.residual && p.y != p.h && (void*)p.scales != p.y && (const void*)p.scales != p.x &&
+                   (const void*)p.scales != p.residual && (void*)p.scales != p.h, "rmsnorm: 8-bit y and scales must be buffers of their own");
+  } else {
+    ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm: y too small"); p.y = args[i++];
+    ZYXB_CHECK_ARG(!d.has_residual || p.y != p.h, "rmsnorm: h and y must be different buffers");
+  }
+  ZYXB_CHECK_ARG(!d.has_weight || (p.weight != p.y && p.weight != p.h && p.weight != (const void*)p.scales), "rmsnorm: an output must not be the weight's buffer");
+  cudaError_t e;
+  switch (d.dtype) {
+    case ZYXB_F32: e = rms_forward<float>(p, d.quant != 0, lc); break;
+    case ZYXB_BF16: e = rms_forward<bf16_t>(p, d.quant != 0, lc); break;
+    default: e = rms_forward<f16_t>(p, d.quant != 0, lc); break;
+  }
+  if (e != cudaSuccess) { err = std::string("rmsnorm: ") + cudaGetErrorString(e); return ZYXB_ERR_KERNEL_LAUNCH; }
+  return check_launch(lc, err, "rmsnorm");
+}
+
+int launch_rmsnorm_bwd(const zyxb_rmsnorm_desc& d, void* const* args, const uint64_t* arg_bytes, int n_args, const LaunchCtx& lc, std::string& err) {
+  const int want = 2 + (d.has_weight ? 2 : 0) + (d.has_dh ? 1 : 0) + 1;
+  ZYXB_CHECK_ARG(n_args == want, "rmsnorm backward: expected args h, dy [,weight] [,dh] -> dx [,dweight]");
+  const uint64_t es = dtype_size(d.dtype);
+  RmsParams p{};
+  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.eps = d.eps; p.rn = lc.round_nearest ? 1 : 0;
+  p.weight_on = d.has_weight ? 1 : 0; p.dh_on = d.has_dh ? 1 : 0;
+  int i = 0;
+  ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm backward: h too small"); p.h = args[i++];
+  ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm backward: dy too small"); p.dy = args[i++];
+  if (d.has_weight) { ZYXB_CHECK_ARG(arg_bytes[i] >= d.cols * es, "rmsnorm backward: weight too small"); p.weight = args[i++]; }
+  if (d.has_dh) { ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm backward: dh too small"); p.dh = args[i++]; }
+  ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm backward: dx too small"); p.y = args[i++];
+  if (d.has_weight) {
+    ZYXB_CHECK_ARG(arg_bytes[i] >= d.cols * es, "rmsnorm backward: dweight too small"); p.dweight = args[i++];
+    ZYXB_CHECK_ARG(p.y != p.weight && p.dweight != p.y && p.dweight != p.h && p.dweight != p.dy && p.dweight != p.dh,
+                   "rmsnorm backward: dx must not be the weight's buffer, dweight no other argument's but the weight's");
+  }
+  p.partial = (float*)lc.scratch;
+  cudaError_t e;
+  switch (d.dtype) {
+    case ZYXB_F32: e = rms_backward<float>(p, lc); break;
+    case ZYXB_BF16: e = rms_backward<bf16_t>(p, lc); break;
+    default: e = rms_backward<f16_t>(p, lc); break;
+  }
+  if (e != cudaSuccess) { err = std::string("rmsnorm backward: ") + cudaGetErrorString(e); return ZYXB_ERR_KERNEL_LAUNCH; }
+  return check_launch(lc, err, "rmsnorm backward", d.has_weight ? 2 : 1);
+}
+
+}  // namespace zyxb

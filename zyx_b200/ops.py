@@ -10,6 +10,7 @@ from . import _lib as L
 from . import backend as B
 
 NP_DTYPE = {L.BF16: np.uint16, L.F16: np.uint16, L.F32: np.float32, L.I32: np.int32}
+ID_DTYPE = {np.dtype(np.int32): L.I32, np.dtype(np.int64): L.I64}
 
 
 class Session:
@@ -94,6 +95,37 @@ class Session:
     def mse(self, dtype, y, t):
         rows, cols = y.shape
         return float(self.run(B.rowreduce_desc(L.RR_MSE, dtype, rows, cols), [y, t], [((1,), np.float32)])[0][0])
+
+    def rmsnorm(self, dtype, x, residual=None, weight=None, eps=1e-6, quant=False, group=0):
+        """y = h / sqrt(mean(h^2) + eps) * weight with h = x + residual; -> y, or (h, y) with a residual; with quant y is (e4m3 bytes,
+        f32 scales [rows, ceil(cols / group)]), group 0 = one scale per row."""
+        rows, cols = x.shape
+        d = B.rmsnorm_desc(dtype, rows, cols, eps=eps, has_residual=residual is not None, has_weight=weight is not None, quant=quant, group=group)
+        outs = [(x.shape, x.dtype)] if residual is not None else []
+        outs += [(x.shape, np.uint8), ((rows, -(-cols // (group or cols))), np.float32)] if quant else [(x.shape, x.dtype)]
+        r = self.run(d, [a for a in (x, residual, weight) if a is not None], outs)
+        y = tuple(r[-2:]) if quant else r[-1]
+        return (r[0], y) if residual is not None else y
+
+    def rmsnorm_bwd(self, dtype, h, dy, weight=None, dh=None, eps=1e-6):
+        """h: the normed sum as stored; -> dx (dh, the residual stream's gradient, added), or (dx, dweight) with a weight."""
+        rows, cols = h.shape
+        d = B.rmsnorm_desc(dtype, rows, cols, eps=eps, has_weight=weight is not None, backward=True, has_dh=dh is not None)
+        outs = [(h.shape, h.dtype)] + ([(weight.shape, weight.dtype)] if weight is not None else [])
+        r = self.run(d, [a for a in (h, dy, weight, dh) if a is not None], outs)
+        return tuple(r) if weight is not None else r[0]
+
+    # ---- embedding -----------------------------------------------------------------------------
+    def embedding(self, dtype, ids, table, scale=0.0):
+        """ids [tokens] (int32 / int64), table [vocab, dim] -> scale * table[ids]; ids outside the table give rows of zeros."""
+        d = B.embedding_desc(dtype, ids.size, table.shape[0], table.shape[1], scale=scale, id_dtype=ID_DTYPE[ids.dtype])
+        return self.run(d, [ids, table], [((ids.size, table.shape[1]), table.dtype)])[0]
+
+    def embedding_bwd(self, dtype, ids, dout, vocab, scale=0.0, accumulate_into=None):
+        """-> the table's gradient [vocab, dim]; accumulate_into: a gradient of that shape to which it is added."""
+        d = B.embedding_desc(dtype, ids.size, vocab, dout.shape[1], scale=scale, id_dtype=ID_DTYPE[ids.dtype], backward=True,
+                             accumulate=accumulate_into is not None)
+        return self.run(d, [ids, dout], [((vocab, dout.shape[1]), dout.dtype)], out_init=accumulate_into)[0]
 
     # ---- elementwise ---------------------------------------------------------------------------
     def eltwise(self, op, dtype, a, b=None, p0=0.0, dtype_out=None, cols=0):
@@ -182,4 +214,22 @@ class Session:
             for grp in bufs:
                 for b in grp:
                     self.pool.deallocate(b)
+            self.device.release(prog)
+
+    def muon_step(self, desc_kw, dtype, tensors):
+        """tensors: list of [p, g (, buf when momentum != 0)] of host matrices; p and buf are updated in place."""
+        groups = len(tensors[0])
+        prog = self.device.create_program(B.muon_desc(dtype, [t[0].shape for t in tensors], **desc_kw))
+        bufs = [[self.pool.upload(t[g]) for t in tensors] for g in range(groups)]
+        try:
+            self.device.launch(prog, [b for grp in bufs for b in grp])
+            if self.check_guards:
+                self.device.check_guards()
+            for g in range(groups):
+                if g != 1:
+                    for t, b in zip(tensors, bufs[g]):
+                        t[g][...] = self.pool.download(b, t[g].shape, t[g].dtype)
+        finally:
+            for b in [b for grp in bufs for b in grp]:
+                self.pool.deallocate(b)
             self.device.release(prog)
