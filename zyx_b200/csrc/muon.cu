@@ -1,9 +1,14 @@
 // Muon: momentum, then the update made nearly orthogonal by Newton-Schulz products, then the weight's step.
+//   momentum   buf = momentum * buf + g, and the sum of squares of the direction (f64)
+//   normalize  X = direction / (norm + eps) as f16 parts, transposed where rows > cols: the products see rows <= cols
+//   products   three per step (muon_gemm.cuh)
+//   step       p = p (1 - lr wd) - lr adjust X
+// Matrices of equal extents (or transposes of each other) go through every launch together.
 #include <algorithm>
 #include <cmath>
 #include <vector>
 
-#include "gemm.h"
+#include "muon_gemm.cuh"
 #include "rounding.cuh"
 
 namespace zyxb {
@@ -11,42 +16,57 @@ namespace zyxb {
 namespace {
 
 constexpr uint64_t MUON_MAX_EXTENT = 32768;
-constexpr int MUON_THREADS = 256, MUON_PARTIALS = 512;
+constexpr int MUON_THREADS = 256, MUON_PARTIALS = 512, MUON_TABLE = 32, TILE = 64;
+constexpr uint64_t MUON_GROUP_BYTES = 1ull << 30;      // matrices that go together: their operands stay below this, or go alone
 
-struct MuonMatrix {
-  void* p;
-  const void* g;
-  void* buf;
-  uint32_t rows, cols;
+struct MuonMatrix { void* p; const void* g; void* buf; uint32_t tall; };
+struct MuonGroup {
+  MuonMatrix m[MUON_TABLE];
+  uint32_t lo, hi;                // extents of the products' X: lo <= hi
   float momentum, grad_scale;
   int nesterov, rn;
 };
 
-// the step before it is made orthogonal, from the stored momentum
-__device__ __forceinline__ float muon_direction(float g, float buf, const MuonMatrix& m) {
-  if (!m.buf) return g;
-  return m.nesterov ? g + m.momentum * buf : buf;
-}
+// the direction that is made orthogonal, from the stored momentum
+__device__ __forceinline__ float muon_direction(float g, float buf, const MuonGroup& k) { return k.nesterov ? g + k.momentum * buf : buf; }
 
-// buf = momentum * buf + g and the sum of squares of the direction, in 64 bits: a gradient's square leaves f32 at 1e19 and 1e-23
+// Sum of squares in 64 bits: a gradient's square leaves f32 at 1e19 and 1e-23.
 template <typename T>
-__global__ void __launch_bounds__(MUON_THREADS) muon_momentum_kernel(MuonMatrix m, double* __restrict__ partial) {
+__global__ void __launch_bounds__(MUON_THREADS) muon_momentum_kernel(const __grid_constant__ MuonGroup k, double* __restrict__ partial) {
   using S = typename Elem<T>::store_t;
+  constexpr int VEC = 16 / (int)sizeof(S);
   __shared__ double part[MUON_THREADS / 32];
-  const uint64_t n = (uint64_t)m.rows * m.cols;
+  const MuonMatrix& m = k.m[blockIdx.y];
+  const uint64_t n = (uint64_t)k.lo * k.hi, vectors = n / VEC;
   const S* g = (const S*)m.g;
   S* b = (S*)m.buf;
   double sum = 0.0;
-  for (uint64_t i = (uint64_t)blockIdx.x * MUON_THREADS + threadIdx.x; i < n; i += (uint64_t)gridDim.x * MUON_THREADS) {
-    const float gv = Elem<T>::load(g[i]) * m.grad_scale;
-    float bv = 0.0f;
+  auto one = [&](float gv, float bv, float& stored) {     // -> the momentum to store; adds the direction's square
+    gv *= k.grad_scale;
+    float u = gv;
     if (b) {
-      const S s = round_store<T>(m.momentum * Elem<T>::load(b[i]) + gv, m.rn != 0);
-      b[i] = s;
-      bv = Elem<T>::load(s);
+      const S s = round_store<T>(k.momentum * bv + gv, k.rn != 0);
+      stored = Elem<T>::load(s);
+      u = muon_direction(gv, stored, k);
     }
-    const double u = muon_direction(gv, bv, m);
-    sum += u * u;
+    sum += (double)u * (double)u;
+  };
+  for (uint64_t i = (uint64_t)blockIdx.x * MUON_THREADS + threadIdx.x; i < vectors; i += (uint64_t)gridDim.x * MUON_THREADS) {
+    RawVec<T, VEC> rg, rb;
+    rg.load(g + i * VEC);
+    if (b) rb.load(b + i * VEC); else rb.zero();
+    float fg[VEC], fb[VEC];
+    rg.decode(fg);
+    rb.decode(fb);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) one(fg[j], fb[j], fb[j]);
+    if (b) { round_encode<T, VEC>(rb, fb, true); rb.store(b + i * VEC); }      // exact: the values are rounded already
+  }
+  if (blockIdx.x == 0 && threadIdx.x < n - vectors * VEC) {
+    const uint64_t i = vectors * VEC + threadIdx.x;
+    float s = 0.0f;
+    one(Elem<T>::load(g[i]), b ? Elem<T>::load(b[i]) : 0.0f, s);
+    if (b) b[i] = round_store<T>(s, true);
   }
   sum = warp_reduce(sum, OpSum());
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
@@ -54,59 +74,121 @@ __global__ void __launch_bounds__(MUON_THREADS) muon_momentum_kernel(MuonMatrix 
   if (threadIdx.x == 0) {
     double s = 0.0;
     for (int w = 0; w < MUON_THREADS / 32; ++w) s += part[w];
-    partial[blockIdx.x] = s;
+    partial[blockIdx.y * MUON_PARTIALS + blockIdx.x] = s;
   }
 }
 
-// X = direction / (norm + eps), lying down: rows <= cols after a transposition where needed
-template <typename T>
-__global__ void __launch_bounds__(MUON_THREADS) muon_normalize_kernel(MuonMatrix m, const double* __restrict__ partial, int n_partial, float eps, float* __restrict__ x) {
+// A 64 x 64 tile of a stored matrix [rows, cols]: f(row in tile, column in tile, first element's index, count) per vector
+template <int VEC, class F>
+__device__ __forceinline__ void muon_tile(uint32_t r0, uint32_t c0, uint32_t rows, uint32_t cols, bool vector, F f) {
+  if (vector) {
+    for (int i = threadIdx.x; i < TILE * (TILE / VEC); i += MUON_THREADS) {
+      const uint32_t r = i / (TILE / VEC), c = i % (TILE / VEC) * VEC;
+      if (r0 + r < rows && c0 + c < cols) f(r, c, (uint64_t)(r0 + r) * cols + c0 + c, true);
+    }
+  } else {
+    for (int i = threadIdx.x; i < TILE * TILE; i += MUON_THREADS) {
+      const uint32_t r = i / TILE, c = i % TILE;
+      if (r0 + r < rows && c0 + c < cols) f(r, c, (uint64_t)(r0 + r) * cols + c0 + c, false);
+    }
+  }
+}
+
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(MUON_THREADS) muon_normalize_kernel(const __grid_constant__ MuonGroup k, const double* __restrict__ partial, int n_partial, float eps,
+                                                                      muon::Operand x) {
   using S = typename Elem<T>::store_t;
+  constexpr int VEC = 16 / (int)sizeof(S);
   __shared__ double total;
-  __shared__ float tile[32][33];
+  __shared__ float tile[TILE][TILE + 1];
+  const MuonMatrix& m = k.m[blockIdx.z];
+  const uint32_t x0 = blockIdx.x * TILE, y0 = blockIdx.y * TILE;       // of X
+  const uint32_t rows = m.tall ? k.hi : k.lo, cols = m.tall ? k.lo : k.hi, r0 = m.tall ? x0 : y0, c0 = m.tall ? y0 : x0;
+  const S* g = (const S*)m.g;
+  const S* b = (const S*)m.buf;
   if (threadIdx.x < 32) {
     double s = 0.0;
-    for (int i = threadIdx.x; i < n_partial; i += 32) s += partial[i];
+    for (int i = threadIdx.x; i < n_partial; i += 32) s += partial[blockIdx.z * MUON_PARTIALS + i];
     s = warp_reduce(s, OpSum());
     if (threadIdx.x == 0) total = s;
   }
+  muon_tile<VEC>(r0, c0, rows, cols, cols % VEC == 0, [&](uint32_t r, uint32_t c, uint64_t i, bool vector) {
+    if (vector) {
+      RawVec<T, VEC> rg, rb;
+      rg.load(g + i);
+      if (b) rb.load(b + i); else rb.zero();
+      float fg[VEC], fb[VEC];
+      rg.decode(fg);
+      rb.decode(fb);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) tile[r][c + j] = b ? muon_direction(fg[j] * k.grad_scale, fb[j], k) : fg[j] * k.grad_scale;
+    } else {
+      const float gv = Elem<T>::load(g[i]) * k.grad_scale;
+      tile[r][c] = b ? muon_direction(gv, Elem<T>::load(b[i]), k) : gv;
+    }
+  });
   __syncthreads();
-  const float inv = 1.0f / ((float)sqrt(total) + eps);
-  const bool tall = m.rows > m.cols;
-  const uint32_t c0 = blockIdx.x * 32, r0 = blockIdx.y * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const S* g = (const S*)m.g;
-  const S* b = (const S*)m.buf;
-  for (int j = ty; j < 32; j += 8) {
-    const uint32_t r = r0 + j, c = c0 + tx;
-    if (r >= m.rows || c >= m.cols) continue;
-    const uint64_t i = (uint64_t)r * m.cols + c;
-    const float v = muon_direction(Elem<T>::load(g[i]) * m.grad_scale, b ? Elem<T>::load(b[i]) : 0.0f, m) * inv;
-    if (tall) tile[j][tx] = v; else x[i] = v;
-  }
-  if (!tall) return;
-  __syncthreads();
-  for (int j = ty; j < 32; j += 8) {
-    const uint32_t r = r0 + tx, c = c0 + j;
-    if (r < m.rows && c < m.cols) x[(uint64_t)c * m.rows + r] = tile[tx][j];
+  const float norm = (float)sqrt(total) + eps;
+  uint16_t* out = x.ptr + blockIdx.z * x.part() * PARTS;
+  for (int i = threadIdx.x; i < TILE * (TILE / 8); i += MUON_THREADS) {
+    const uint32_t y = i / (TILE / 8), q = i % (TILE / 8) * 8;
+    if (y0 + y >= k.lo || x0 + q >= k.hi) continue;
+    uint32_t w[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float u = m.tall ? tile[q + 2 * j][y] : tile[y][q + 2 * j], v = m.tall ? tile[q + 2 * j + 1][y] : tile[y][q + 2 * j + 1];
+      muon::split2(u / norm * muon::SCALE, v / norm * muon::SCALE, w[0][j], w[1][j]);      // behind the last column: spare
+    }
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s)
+      *reinterpret_cast<uint4*>(out + s * x.part() + (uint64_t)(y0 + y) * x.ld + x0 + q) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
   }
 }
 
-// B = a I + b A + c A^2 (A^2 given)
-__global__ void muon_polynomial_kernel(const float* __restrict__ a1, float* __restrict__ a2, uint32_t m, float a, float b, float c) {
-  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (uint64_t)m * m; i += (uint64_t)gridDim.x * blockDim.x)
-    a2[i] = (i % (m + 1) == 0 ? a : 0.0f) + b * a1[i] + c * a2[i];
-}
-
-template <typename T>
-__global__ void muon_step_kernel(MuonMatrix m, const float* __restrict__ x, float decay, float step) {
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(MUON_THREADS) muon_step_kernel(const __grid_constant__ MuonGroup k, muon::Operand x, float decay, float step_flat, float step_tall) {
   using S = typename Elem<T>::store_t;
-  S* p = (S*)m.p;
-  const bool tall = m.rows > m.cols;
-  for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (uint64_t)m.rows * m.cols; i += (uint64_t)gridDim.x * blockDim.x) {
-    const float o = tall ? x[(i % m.cols) * m.rows + i / m.cols] : x[i];
-    p[i] = round_store<T>(Elem<T>::load(p[i]) * decay - step * o, m.rn != 0);
+  constexpr int VEC = 16 / (int)sizeof(S);
+  __shared__ float tile[TILE][TILE + 1];
+  const MuonMatrix& m = k.m[blockIdx.z];
+  const uint32_t x0 = blockIdx.x * TILE, y0 = blockIdx.y * TILE;
+  const uint32_t rows = m.tall ? k.hi : k.lo, cols = m.tall ? k.lo : k.hi, r0 = m.tall ? x0 : y0, c0 = m.tall ? y0 : x0;
+  const uint16_t* in = x.ptr + blockIdx.z * x.part() * PARTS;
+  const float step = (m.tall ? step_tall : step_flat) * muon::UNSCALE;
+  for (int i = threadIdx.x; i < TILE * (TILE / 8); i += MUON_THREADS) {
+    const uint32_t y = i / (TILE / 8), q = i % (TILE / 8) * 8;
+    if (y0 + y >= k.lo || x0 + q >= k.hi) continue;
+    float v[8];
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s) {
+      RawVec<f16_t, 8> r;
+      r.load_stream(in + s * x.part() + (uint64_t)(y0 + y) * x.ld + x0 + q);
+      float f[8];
+      r.decode(f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = s ? v[j] + f[j] : f[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (m.tall) tile[q + j][y] = v[j]; else tile[y][q + j] = v[j];
+    }
   }
+  __syncthreads();
+  S* p = (S*)m.p;
+  muon_tile<VEC>(r0, c0, rows, cols, cols % VEC == 0, [&](uint32_t r, uint32_t c, uint64_t i, bool vector) {
+    if (vector) {
+      RawVec<T, VEC> rp;
+      rp.load(p + i);
+      float f[VEC];
+      rp.decode(f);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = f[j] * decay - step * tile[r][c + j];
+      round_encode<T, VEC>(rp, f, k.rn != 0);
+      rp.store(p + i);
+    } else {
+      p[i] = round_store<T>(Elem<T>::load(p[i]) * decay - step * tile[r][c], k.rn != 0);
+    }
+  });
 }
 
 float muon_adjust(int kind, uint64_t rows, uint64_t cols) {
@@ -119,36 +201,90 @@ void muon_coefficients(const zyxb_muon_desc& d, float& a, float& b, float& c) {
   if (a == 0.0f && b == 0.0f && c == 0.0f) { a = 3.4445f; b = -4.7750f; c = 2.0315f; }
 }
 
-int muon_gemm(const float* a, const float* b, float* c, uint64_t m, uint64_t n, uint64_t k, bool trans_b, const LaunchCtx& lc, std::string& err) {
-  zyxb_gemm_desc g{};
-  g.dtype = ZYXB_F32; g.m = m; g.n = n; g.k = k; g.batch = 1; g.trans_b = trans_b ? 1 : 0;
-  void* args[3] = {(void*)a, (void*)b, (void*)c};
-  const uint64_t bytes[3] = {m * k * 4, n * k * 4, m * n * 4};
-  return launch_gemm(g, args, bytes, 3, lc, err);
+// 16-bit matrices come with at most 11 bits and are stored with them again; f32 ones take two parts
+int muon_parts(int dtype) { return dtype == ZYXB_F32 ? 2 : 1; }
+
+uint64_t up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
+
+struct MuonPlan { uint64_t lo, hi; std::vector<int> members; };
+
+uint64_t muon_bytes(uint64_t lo, uint64_t hi, uint64_t batch, int parts) {
+  return up(batch * MUON_PARTIALS * sizeof(double), 256) + 2 * up(batch * parts * lo * up(hi, 8) * 2, 256) + 2 * up(batch * parts * lo * up(lo, 8) * 2, 256);
 }
 
-template <typename T>
-int muon_update(const zyxb_muon_desc& d, const MuonMatrix& m, void* workspace, const LaunchCtx& lc, std::string& err) {
-  const uint64_t lo = std::min(m.rows, m.cols), hi = std::max(m.rows, m.cols), n = lo * hi;
-  double* partial = (double*)workspace;
-  float* x = (float*)(partial + MUON_PARTIALS);
-  float *y = x + n, *a1 = y + n, *a2 = a1 + lo * lo;
-  const unsigned sums = (unsigned)std::min<uint64_t>(MUON_PARTIALS, (n + MUON_THREADS * 8 - 1) / (MUON_THREADS * 8));
-  muon_momentum_kernel<T><<<sums, MUON_THREADS, 0, lc.stream>>>(m, partial);
-  muon_normalize_kernel<T><<<dim3((m.cols + 31) / 32, (m.rows + 31) / 32), MUON_THREADS, 0, lc.stream>>>(m, partial, (int)sums, d.eps == 0.0f ? 1e-7f : d.eps, x);
+// matrices that are updated together, in the order of their first members
+std::vector<MuonPlan> muon_plan(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols) {
+  std::vector<MuonPlan> plans;
+  for (int i = 0; i < d.n_tensors; ++i) {
+    const uint64_t lo = std::min(rows[i], cols[i]), hi = std::max(rows[i], cols[i]);
+    MuonPlan* to = nullptr;
+    for (auto& g : plans)
+      if (g.lo == lo && g.hi == hi && g.members.size() < MUON_TABLE && muon_bytes(lo, hi, g.members.size() + 1, muon_parts(d.dtype)) <= MUON_GROUP_BYTES) to = &g;
+    if (!to) { plans.push_back(MuonPlan{lo, hi, {}}); to = &plans.back(); }
+    to->members.push_back(i);
+  }
+  return plans;
+}
+
+template <typename T, int PARTS>
+int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols, const MuonPlan& pl, void* const* args, void* workspace, const LaunchCtx& lc, std::string& err) {
+  const uint32_t lo = (uint32_t)pl.lo, hi = (uint32_t)pl.hi, batch = (uint32_t)pl.members.size();
+  MuonGroup k{};
+  k.lo = lo; k.hi = hi; k.momentum = d.momentum; k.grad_scale = d.grad_scale == 0.0f ? 1.0f : d.grad_scale;
+  k.nesterov = d.nesterov ? 1 : 0; k.rn = lc.round_nearest ? 1 : 0;
+  const int n = d.n_tensors;
+  for (uint32_t j = 0; j < batch; ++j) {
+    const int i = pl.members[j];
+    k.m[j] = MuonMatrix{args[i], args[n + i], d.momentum != 0.0f ? args[2 * n + i] : nullptr, rows[i] > cols[i] ? 1u : 0u};
+  }
+  char* at = (char*)workspace;
+  double* partial = (double*)at;
+  at += up(batch * MUON_PARTIALS * sizeof(double), 256);
+  auto operand = [&](uint32_t rows, uint32_t cols) {
+    muon::Operand o{(uint16_t*)at, rows, cols, (uint32_t)up(cols, 8)};
+    at += up(batch * PARTS * o.part() * 2, 256);
+    return o;
+  };
+  muon::Operand x[2], gram, poly;
+  x[0] = operand(lo, hi); x[1] = operand(lo, hi); gram = operand(lo, lo); poly = operand(lo, lo);
+
+  const unsigned sums = (unsigned)std::min<uint64_t>(MUON_PARTIALS, ((uint64_t)lo * hi + MUON_THREADS * 16 - 1) / (MUON_THREADS * 16));
+  const dim3 tiles((hi + TILE - 1) / TILE, (lo + TILE - 1) / TILE, batch);
+  muon_momentum_kernel<T><<<dim3(sums, batch), MUON_THREADS, 0, lc.stream>>>(k, partial);
+  muon_normalize_kernel<T, PARTS><<<tiles, MUON_THREADS, 0, lc.stream>>>(k, partial, (int)sums, d.eps == 0.0f ? 1e-7f : d.eps, x[0]);
+
+  constexpr int BN = 256;
+  CUtensorMap x_rows[2], x_cols[2], x_k[2], gram_rows, gram_cols, poly_rows;
+  bool ok = true;
+  for (int j = 0; j < 2; ++j)
+    ok = ok && muon::encode(lc.tma_encode, &x_rows[j], x[j], PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &x_cols[j], x[j], PARTS, batch, BN) &&
+         muon::encode(lc.tma_encode, &x_k[j], x[j], PARTS, batch, 64);
+  ok = ok && muon::encode(lc.tma_encode, &gram_rows, gram, PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &gram_cols, gram, PARTS, batch, BN) &&
+       muon::encode(lc.tma_encode, &poly_rows, poly, PARTS, batch, muon::BM);
+  if (!ok) { err = "muon: cuTensorMapEncodeTiled rejected an operand"; return ZYXB_ERR_KERNEL_LAUNCH; }
   float a, b, c;
   muon_coefficients(d, a, b, c);
-  int launches = 3, st;
-  for (int i = 0; i < (d.steps ? d.steps : 5); ++i) {
-    if ((st = muon_gemm(x, x, a1, lo, lo, hi, true, lc, err))) return st;
-    if ((st = muon_gemm(a1, a1, a2, lo, lo, lo, true, lc, err))) return st;
-    muon_polynomial_kernel<<<(unsigned)std::min<uint64_t>(2048, (lo * lo + 255) / 256), 256, 0, lc.stream>>>(a1, a2, (uint32_t)lo, a, b, c);
-    ++launches;
-    if ((st = muon_gemm(a2, x, y, lo, hi, lo, false, lc, err))) return st;
-    std::swap(x, y);
+  auto gemm_args = [&](const muon::Operand& out, uint32_t contraction) {
+    muon::GemmArgs g{};
+    g.out = out.ptr; g.m = out.rows; g.n = out.cols; g.k = contraction; g.batch = batch; g.ld = out.ld; g.part = out.part(); g.stride = out.part() * PARTS;
+    return g;
+  };
+  const int steps = d.steps ? d.steps : 5;
+  cudaError_t e = cudaSuccess;
+  for (int i = 0; i < steps && e == cudaSuccess; ++i) {
+    const int from = i & 1;
+    e = muon::launch<PARTS, BN, true, false, false>(x_rows[from], x_cols[from], gemm_args(gram, hi), lc);
+    if (e != cudaSuccess) break;
+    muon::GemmArgs g = gemm_args(poly, lo);
+    g.gram = gram.ptr; g.a = a; g.b = b; g.c = c;
+    e = muon::launch<PARTS, BN, true, true, false>(gram_rows, gram_cols, g, lc);
+    if (e != cudaSuccess) break;
+    e = muon::launch<PARTS, BN, false, false, true>(poly_rows, x_k[from], gemm_args(x[from ^ 1], lo), lc);
   }
-  muon_step_kernel<T><<<(unsigned)std::min<uint64_t>(4096, (n + 255) / 256), 256, 0, lc.stream>>>(m, x, 1.0f - d.lr * d.weight_decay, d.lr * muon_adjust(d.adjust, m.rows, m.cols));
-  return check_launch(lc, err, "muon", launches);
+  if (e != cudaSuccess) { err = std::string("muon: ") + cudaGetErrorString(e); return ZYXB_ERR_KERNEL_LAUNCH; }
+  muon_step_kernel<T, PARTS><<<tiles, MUON_THREADS, 0, lc.stream>>>(k, x[steps & 1], 1.0f - d.lr * d.weight_decay, d.lr * muon_adjust(d.adjust, lo, hi),
+                                                                   d.lr * muon_adjust(d.adjust, hi, lo));
+  return check_launch(lc, err, "muon", 3 + 3 * steps);
 }
 
 }  // namespace
@@ -174,11 +310,8 @@ int validate_muon(const zyxb_muon_desc& d, std::string& err) {
 
 uint64_t muon_workspace_bytes(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols) {
   uint64_t most = 0;
-  for (int i = 0; i < d.n_tensors; ++i) {
-    const uint64_t lo = std::min(rows[i], cols[i]);
-    most = std::max(most, 4 * (2 * rows[i] * cols[i] + 2 * lo * lo));
-  }
-  return MUON_PARTIALS * sizeof(double) + most;
+  for (const MuonPlan& pl : muon_plan(d, rows, cols)) most = std::max(most, muon_bytes(pl.lo, pl.hi, pl.members.size(), muon_parts(d.dtype)));
+  return most;
 }
 
 int launch_muon(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols, void* workspace, void* const* args,
@@ -196,16 +329,13 @@ int launch_muon(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* c
   ZYXB_CHECK_ARG(std::adjacent_find(written.begin(), written.end()) == written.end(), "muon: the same buffer is given twice to be updated");
   for (int i = 0; i < n; ++i)
     ZYXB_CHECK_ARG(!std::binary_search(written.begin(), written.end(), (const void*)args[n + i]), "muon: a gradient is given as a buffer to be updated");
-  for (int i = 0; i < n; ++i) {
-    MuonMatrix m{};
-    m.p = args[i]; m.g = args[n + i]; m.buf = groups > 2 ? args[2 * n + i] : nullptr;
-    m.rows = (uint32_t)rows[i]; m.cols = (uint32_t)cols[i]; m.momentum = d.momentum;
-    m.grad_scale = d.grad_scale == 0.0f ? 1.0f : d.grad_scale; m.nesterov = d.nesterov ? 1 : 0; m.rn = lc.round_nearest ? 1 : 0;
+  if (!lc.tma_encode) { err = "muon: the driver offers no cuTensorMapEncodeTiled"; return ZYXB_ERR_KERNEL_LAUNCH; }
+  for (const MuonPlan& pl : muon_plan(d, rows, cols)) {
     int st;
     switch (d.dtype) {
-      case ZYXB_F32: st = muon_update<float>(d, m, workspace, lc, err); break;
-      case ZYXB_BF16: st = muon_update<bf16_t>(d, m, workspace, lc, err); break;
-      default: st = muon_update<f16_t>(d, m, workspace, lc, err); break;
+      case ZYXB_F32: st = muon_run<float, 2>(d, rows, cols, pl, args, workspace, lc, err); break;
+      case ZYXB_BF16: st = muon_run<bf16_t, 1>(d, rows, cols, pl, args, workspace, lc, err); break;
+      default: st = muon_run<f16_t, 1>(d, rows, cols, pl, args, workspace, lc, err); break;
     }
     if (st) return st;
   }

@@ -1,0 +1,362 @@
+// The three products of a Newton-Schulz step on the 5th-generation tensor cores.
+//   gram   A  = X X^T                      [m, m], symmetric
+//   poly   B  = a I + b A + c A A^T        [m, m], symmetric (A A^T = A^2)
+//   apply  X' = B X                        [m, n]
+// Operands and results are f16 in the program's workspace, carried as `PARTS` numbers whose sum is the value: one (11 bits) or two
+// (hi + lo, 22 bits).  All are multiplied by 2^10, which keeps the entries of a normed matrix (down to 2^-15 on average at the
+// largest extent) and their low halves inside f16's normal range, and the largest possible entry (5, by the bound that the
+// program puts on the coefficients) below its end.  Two parts take three products (the product of the low halves, 2^-22, is dropped).
+//
+// The pipeline is the 16-bit matmul's: one persistent CTA per SM, warp 0 loads tiles by TMA, warp 1 issues tcgen05.mma, warps 2..9
+// read the accumulators from TMEM while the next tile is multiplied.  What differs:
+//   symmetry  only tiles that touch the lower triangle are computed, and stored twice: half of the work of gram and poly.
+//   rounding  the tensor core adds with truncation, which over 1536 additions costs 1.5e-4 of the result: below the 2^-11 of one
+//             part, far above the 2^-22 of two.  With two parts an accumulator takes 24 additions (128 of k), and the epilogue warps add
+//             the accumulators in f32 registers.
+// Every wait is bounded, like the matmul's.
+#pragma once
+#include <algorithm>
+
+#include "common.cuh"
+#include "internal.h"
+#include "tc_ptx.cuh"
+
+namespace zyxb {
+namespace muon {
+
+constexpr int BM = 128, BK = 64, UMMA_K = 16, THREADS = 320, EPI_THREADS = 256;
+constexpr int CHUNK_BLOCKS = 2;        // two parts: k-blocks per accumulator
+constexpr float SCALE = 1024.0f, UNSCALE = 1.0f / 1024.0f;
+enum { ERR_PRODUCER = 0x20000u, ERR_MMA = 0x40000u, ERR_EPILOGUE = 0x80000u };
+
+// [batch][part][rows][ld] f16
+struct Operand {
+  uint16_t* ptr;
+  uint32_t rows, cols, ld;
+  __host__ __device__ uint64_t part() const { return (uint64_t)rows * ld; }
+};
+
+struct GemmArgs {
+  uint16_t* out;
+  const uint16_t* gram;     // poly: A, shaped like out
+  uint32_t m, n, k, batch, tiles_m, tiles_n, tiles, ld;
+  uint64_t part, stride;    // elements from hi to lo, from matrix to matrix, of out
+  float a, b, c;            // poly; c is 1 otherwise
+  uint32_t* status;
+};
+
+template <int PARTS, int BN> struct Smem {
+  static constexpr int A_PART = BM * BK * 2, B_PART = BN * BK * 2;
+  static constexpr int STAGE = PARTS * (A_PART + B_PART);
+  static constexpr int STAGES = 196608 / STAGE;
+  static constexpr int BAR = STAGES * STAGE;
+  static constexpr int TOTAL = BAR + 256 + 1024;
+};
+
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack2_t<false>(x, y);
+  const float hx = __half2float(__ushort_as_half((uint16_t)hi)), hy = __half2float(__ushort_as_half((uint16_t)(hi >> 16)));
+  lo = pack2_t<false>(x - hx, y - hy);
+}
+
+template <int PARTS, int BN, bool SYM, bool POLY, bool B_MN>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, GemmArgs p) {
+  using SM = Smem<PARTS, BN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - raw);
+  const uint32_t bars = base + SM::BAR;
+  auto full_bar = [&](int s) { return bars + 8u * s; };
+  auto empty_bar = [&](int s) { return bars + 8u * (SM::STAGES + s); };
+  auto tfull_bar = [&](int a) { return bars + 8u * (2 * SM::STAGES + a); };
+  auto tempty_bar = [&](int a) { return bars + 8u * (2 * SM::STAGES + 2 + a); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + SM::BAR + 8 * (2 * SM::STAGES + 4));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr uint32_t TMEM_COLS = 2 * BN;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SM::STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), EPI_THREADS / 32); }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const uint32_t total = p.tiles * p.batch, k_blocks = (p.k + BK - 1) / BK;
+  auto tile_coords = [&](uint32_t t, uint32_t& z, uint32_t& tm, uint32_t& tn) {
+    z = t / p.tiles;
+    const uint32_t r = t - z * p.tiles;
+    if constexpr (SYM) {
+      // row tm of tiles holds tm / W + 1 of them (W = BN / BM): W rows at a time, q + 1 tiles each, W q (q + 1) / 2 before them
+      constexpr uint32_t W = BN / BM;
+      uint32_t q = (uint32_t)((sqrtf(1.0f + 8.0f * (float)r / W) - 1.0f) * 0.5f);
+      while (W * q * (q + 1) / 2 > r) --q;
+      while (W * (q + 1) * (q + 2) / 2 <= r) ++q;
+      const uint32_t in = r - W * q * (q + 1) / 2;
+      tm = q * W + in / (q + 1);
+      tn = in % (q + 1);
+    } else {
+      constexpr uint32_t GROUP_M = 16;   // tiles that run together share panels in L2
+      const uint32_t group_size = GROUP_M * p.tiles_n, g = r / group_size, first_m = g * GROUP_M;
+      const uint32_t rows_in_group = min(GROUP_M, p.tiles_m - first_m), in_group = r % group_size;
+      tm = first_m + in_group % rows_in_group;
+      tn = in_group / rows_in_group;
+    }
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, issued = 0;
+      bool ok = true;
+      for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        uint32_t z, tm, tn;
+        tile_coords(t, z, tm, tn);
+        for (uint32_t kb = 0; kb < k_blocks; ++kb) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status, ERR_PRODUCER)) { ok = false; break; }
+          const uint32_t a_dst = base + stage * SM::STAGE, b_dst = a_dst + PARTS * SM::A_PART;
+          mbar_expect_tx(full_bar(stage), SM::STAGE);
+          const int k0 = (int)(kb * BK);
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) {
+            tma_load_4d(a_dst + q * SM::A_PART, &map_a, full_bar(stage), k0, (int)(tm * BM), q, (int)z);
+            if constexpr (B_MN) {
+#pragma unroll
+              for (int j = 0; j < BN / 64; ++j)
+                tma_load_4d(b_dst + q * SM::B_PART + j * (64 * BK * 2), &map_b, full_bar(stage), (int)(tn * BN) + j * 64, k0, q, (int)z);
+            } else {
+              tma_load_4d(b_dst + q * SM::B_PART, &map_b, full_bar(stage), k0, (int)(tn * BN), q, (int)z);
+            }
+          }
+          ++issued;
+          if (++stage == SM::STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) {     // copies in flight land before the CTA goes
+        uint32_t s = stage, ph = phase;
+        const uint32_t n_back = issued < (uint32_t)SM::STAGES ? issued : (uint32_t)SM::STAGES;
+        for (uint32_t i = 0; i < n_back; ++i) {
+          if (s == 0) { s = SM::STAGES - 1; ph ^= 1; } else --s;
+          const uint64_t t0 = global_timer_ns();
+          while (!mbar_try_wait(full_bar(s), ph) && global_timer_ns() - t0 < TC_WAIT_NS) {}
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc(false, false, B_MN, BM, BN);
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        for (uint32_t kb = 0; kb < k_blocks && ok; ++kb) {
+          const uint32_t in_chunk = PARTS == 2 ? kb % CHUNK_BLOCKS : kb;
+          if (in_chunk == 0) {
+            if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1, abort_flag, p.status, ERR_MMA)) { ok = false; break; }
+            tc_fence_after();
+          }
+          const uint32_t d_tmem = tmem_base + acc * BN;
+          if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, ERR_MMA)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_addr = base + stage * SM::STAGE, b_addr = a_addr + PARTS * SM::A_PART;
+#pragma unroll
+          for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+            auto adesc = [&](int q) { return make_smem_desc(a_addr + q * SM::A_PART + kk * (UMMA_K * 2), 16, 1024); };
+            auto bdesc = [&](int q) {
+              return B_MN ? make_smem_desc(b_addr + q * SM::B_PART + kk * (UMMA_K * 128), 64 * BK * 2, 1024)
+                          : make_smem_desc(b_addr + q * SM::B_PART + kk * (UMMA_K * 2), 16, 1024);
+            };
+            const uint32_t more = (in_chunk | (uint32_t)kk) != 0 ? 1u : 0u;
+            if constexpr (PARTS == 2) {     // the small products first
+              umma_f16(d_tmem, adesc(1), bdesc(0), idesc, more);
+              umma_f16(d_tmem, adesc(0), bdesc(1), idesc, 1u);
+              umma_f16(d_tmem, adesc(0), bdesc(0), idesc, 1u);
+            } else {
+              umma_f16(d_tmem, adesc(0), bdesc(0), idesc, more);
+            }
+          }
+          umma_commit(empty_bar(stage));
+          if (++stage == SM::STAGES) { stage = 0; phase ^= 1; }
+          if (kb + 1 == k_blocks || (PARTS == 2 && in_chunk == CHUNK_BLOCKS - 1)) {
+            umma_commit(tfull_bar(acc));
+            if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+          }
+        }
+      }
+    }
+  } else {
+    // lane = row; two warps per TMEM lane quarter, each with half of the columns
+    const int col_half = (warp - 2) >> 2;
+    const uint32_t quarter = (uint32_t)(warp & 3);
+    constexpr int HALF = BN / 2, CH = HALF / 32;
+    uint32_t acc = 0, acc_phase = 0;
+    bool ok = true;
+    const uint32_t n_chunks = PARTS == 2 ? (k_blocks + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS : 1;
+    for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      uint32_t z, tm, tn;
+      tile_coords(t, z, tm, tn);
+      uint16_t* out = p.out + z * p.stride;
+      const uint16_t* gram = POLY ? p.gram + z * p.stride : nullptr;
+      const uint32_t row0 = tm * BM + quarter * 32, row = row0 + lane;
+      // 32 columns from c on of this lane's row
+      auto finish = [&](float (&v)[32], uint32_t c) {
+        if (c >= p.n || row0 >= p.m) return;
+        if (SYM && c > row0 + 31) return;                      // wholly above the diagonal: the mirrored tile's
+        const uint64_t at = (uint64_t)row * p.ld + c;
+        const bool mine = row < p.m;
+        if constexpr (POLY) {
+          if (mine) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              if (c + q * 8 >= p.n) break;
+              float g[8];
+#pragma unroll
+              for (int s = 0; s < PARTS; ++s) {
+                const uint4 w = *reinterpret_cast<const uint4*>(gram + s * p.part + at + q * 8);
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float lo = __half2float(__ushort_as_half((uint16_t)ws[j])), hi = __half2float(__ushort_as_half((uint16_t)(ws[j] >> 16)));
+                  g[2 * j] = s ? g[2 * j] + lo : lo;
+                  g[2 * j + 1] = s ? g[2 * j + 1] + hi : hi;
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                v[q * 8 + j] = p.c * (v[q * 8 + j] * UNSCALE) + p.b * g[j];
+                if (c + q * 8 + j == row) v[q * 8 + j] += p.a * SCALE;
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= UNSCALE;
+        }
+        uint32_t w[PARTS][16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if constexpr (PARTS == 2) split2(v[2 * j], v[2 * j + 1], w[0][j], w[PARTS - 1][j]);
+          else w[0][j] = pack2_t<false>(v[2 * j], v[2 * j + 1]);
+        }
+        const bool below = !SYM || c + 31 < row0;              // no entry of the warp's block on or above the diagonal
+        if (below && mine) {
+#pragma unroll
+          for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (c + q * 8 < p.n)                             // ld is a multiple of 8: what lies behind n is spare
+                *reinterpret_cast<uint4*>(out + s * p.part + at + q * 8) = make_uint4(w[s][4 * q], w[s][4 * q + 1], w[s][4 * q + 2], w[s][4 * q + 3]);
+        }
+        if constexpr (SYM) {
+          if (below && row0 + 32 <= p.m) {
+            // mirrored: two neighbouring lanes trade halves, so that each stores two rows' entries of one column side by side
+            const bool odd = lane & 1;
+#pragma unroll
+            for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, w[s][j], 1);
+                const uint32_t pair = odd ? __byte_perm(other, w[s][j], 0x7632) : __byte_perm(w[s][j], other, 0x5410);
+                *reinterpret_cast<uint32_t*>(out + s * p.part + (uint64_t)(c + 2 * j + (odd ? 1 : 0)) * p.ld + (row & ~1u)) = pair;
+              }
+          } else if (mine) {
+#pragma unroll
+            for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const uint32_t col = c + j;
+                if (col > row) continue;
+                const uint16_t h = (uint16_t)(w[s][j / 2] >> (16 * (j & 1)));
+                if (!below) out[s * p.part + (uint64_t)row * p.ld + col] = h;
+                if (col < row) out[s * p.part + (uint64_t)col * p.ld + row] = h;
+              }
+          }
+        }
+      };
+      if constexpr (PARTS == 2) {
+        float sum[HALF];
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) sum[i] = 0.0f;
+        for (uint32_t ck = 0; ck < n_chunks && ok; ++ck) {
+          if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, ERR_EPILOGUE)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch) {
+            uint32_t r[32];
+            tmem_ld32(tmem_base + ((quarter * 32u) << 16) + acc * BN + (col_half * CH + ch) * 32, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sum[ch * 32 + i] += __uint_as_float(r[i]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tempty_bar(acc));
+          if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = sum[ch * 32 + i];
+          finish(v, tn * BN + (col_half * CH + ch) * 32);
+        }
+      } else {
+        if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, ERR_EPILOGUE)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll 1
+        for (int ch = 0; ch < CH; ++ch) {
+          uint32_t r[32];
+          tmem_ld32(tmem_base + ((quarter * 32u) << 16) + acc * BN + (col_half * CH + ch) * 32, r);
+          tmem_ld_wait();
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+          finish(v, tn * BN + (col_half * CH + ch) * 32);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty_bar(acc));
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// {contiguous, rows, parts, matrices} with a box of 64 x `box_rows`
+inline bool encode(void* fn, CUtensorMap* map, const Operand& o, int parts, uint32_t batch, uint32_t box_rows) {
+  return encode_map(fn, map, false, o.ptr, o.cols, o.rows, o.ld, (uint64_t)parts, parts > 1 ? o.part() : 0, batch, batch > 1 ? o.part() * parts : 0, box_rows);
+}
+
+template <int PARTS, int BN, bool SYM, bool POLY, bool B_MN>
+cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mb, GemmArgs p, const LaunchCtx& lc) {
+  using SM = Smem<PARTS, BN>;
+  static uint64_t configured = 0;
+  auto kern = gemm_kernel<PARTS, BN, SYM, POLY, B_MN>;
+  cudaError_t e = ensure_dynamic_smem(kern, SM::TOTAL, &configured);
+  if (e != cudaSuccess) return e;
+  p.tiles_m = (p.m + BM - 1) / BM;
+  p.tiles_n = (p.n + BN - 1) / BN;
+  if (SYM) {
+    p.tiles = 0;
+    for (uint32_t tm = 0; tm < p.tiles_m; ++tm) p.tiles += tm / (BN / BM) + 1;
+  } else {
+    p.tiles = p.tiles_m * p.tiles_n;
+  }
+  p.status = lc.status_word;
+  const unsigned grid = (unsigned)std::min<uint64_t>((uint64_t)p.tiles * p.batch, (uint64_t)lc.sm_count);
+  kern<<<grid, THREADS, SM::TOTAL, lc.stream>>>(ma, mb, p);
+  return cudaGetLastError();
+}
+
+}  // namespace muon
+}  // namespace zyxb

@@ -78,7 +78,7 @@ struct RowView {
     float v[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) v[k] = inside(col(pack) + k) ? Elem<T>::load(p[k]) : 0.0f;
-    r.encode(v, false);          // exact: the values are of the storage type
+    round_encode<T, VEC>(r, v, true);          // exact: the values are of the storage type
   }
   __device__ __forceinline__ void store(const float (&v)[VEC], void* base, int pack, bool rn) const {
     S* p = reinterpret_cast<S*>(base) + start + (uint64_t)pack * VEC;
