@@ -337,7 +337,7 @@ typedef struct {
   int32_t  nesterov;
   int32_t  steps;          /* 0 means 5; at most 32 */
   float    a, b, c;        /* all 0 means 3.4445, -4.7750, 2.0315; a x + b x^3 + c x^5 has to map [0, 1.25] into [-1.25, 1.25] */
-  float    eps;            /* 0 means 1e-7 */
+  float    eps;            /* 0 means 1e-7; otherwise at least 1e-30 */
   float    grad_scale;     /* gradients are multiplied by this first; 0 means 1 */
   int32_t  adjust;         /* ZYXB_MUON_ADJUST_* */
 } zyxb_muon_desc;

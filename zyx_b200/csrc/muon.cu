@@ -36,6 +36,7 @@ __global__ void __launch_bounds__(MUON_THREADS) muon_momentum_kernel(const __gri
   using S = typename Elem<T>::store_t;
   constexpr int VEC = 16 / (int)sizeof(S);
   __shared__ double part[MUON_THREADS / 32];
+  pdl_trigger();
   const MuonMatrix& m = k.m[blockIdx.y];
   const uint64_t n = (uint64_t)k.lo * k.hi, vectors = n / VEC;
   const S* g = (const S*)m.g;
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(MUON_THREADS) muon_momentum_kernel(const __gri
   }
 }
 
-// A 64 x 64 tile of a stored matrix [rows, cols]: f(row in tile, column in tile, first element's index, count) per vector
+// A 64 x 64 tile of a stored matrix [rows, cols]: f(row in tile, column in tile, element's index, whole vector or one element)
 template <int VEC, class F>
 __device__ __forceinline__ void muon_tile(uint32_t r0, uint32_t c0, uint32_t rows, uint32_t cols, bool vector, F f) {
   if (vector) {
@@ -94,25 +95,89 @@ __device__ __forceinline__ void muon_tile(uint32_t r0, uint32_t c0, uint32_t row
   }
 }
 
+// Eight neighbouring entries of X and where they lie in a stored matrix that is not transposed
+constexpr int EIGHTS = TILE * TILE / 8 / MUON_THREADS;       // per thread and tile
+
+// eight neighbouring elements of a row of `cols`, from element i (column c) on; zeros behind the row
+template <typename T> __device__ __forceinline__ void load8(float (&v)[8], const typename Elem<T>::store_t* p, uint64_t i, uint32_t c, uint32_t cols, bool vector) {
+  constexpr int VEC = 16 / (int)sizeof(typename Elem<T>::store_t);
+  if (vector) {
+#pragma unroll
+    for (int h = 0; h < 8 / VEC; ++h) {
+      RawVec<T, VEC> r;
+      r.load(p + i + h * VEC);
+      float f[VEC];
+      r.decode(f);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[h * VEC + j] = f[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? Elem<T>::load(p[i + j]) : 0.0f;
+  }
+}
+
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(MUON_THREADS) muon_normalize_kernel(const __grid_constant__ MuonGroup k, const double* __restrict__ partial, int n_partial, float eps,
                                                                       muon::Operand x) {
   using S = typename Elem<T>::store_t;
   constexpr int VEC = 16 / (int)sizeof(S);
-  __shared__ double total;
+  __shared__ double part[MUON_THREADS / 32];
   __shared__ float tile[TILE][TILE + 1];
   const MuonMatrix& m = k.m[blockIdx.z];
   const uint32_t x0 = blockIdx.x * TILE, y0 = blockIdx.y * TILE;       // of X
-  const uint32_t rows = m.tall ? k.hi : k.lo, cols = m.tall ? k.lo : k.hi, r0 = m.tall ? x0 : y0, c0 = m.tall ? y0 : x0;
   const S* g = (const S*)m.g;
   const S* b = (const S*)m.buf;
-  if (threadIdx.x < 32) {
+  uint16_t* out = x.ptr + blockIdx.z * x.part() * PARTS;
+  pdl_trigger();
+  pdl_wait();
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < MUON_PARTIALS; i += MUON_THREADS)
+    if ((int)threadIdx.x + i < n_partial) sum += partial[blockIdx.z * MUON_PARTIALS + threadIdx.x + i];
+  sum = warp_reduce(sum, OpSum());
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+  auto scale = [&] {                 // behind a barrier
     double s = 0.0;
-    for (int i = threadIdx.x; i < n_partial; i += 32) s += partial[blockIdx.z * MUON_PARTIALS + i];
-    s = warp_reduce(s, OpSum());
-    if (threadIdx.x == 0) total = s;
+#pragma unroll
+    for (int w = 0; w < MUON_THREADS / 32; ++w) s += part[w];
+    return muon::SCALE / ((float)sqrt(s) + eps);
+  };
+  auto put = [&](const float (&v)[8], uint32_t y, uint32_t q, float inv) {
+    uint32_t w[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) muon::split2(v[2 * j] * inv, v[2 * j + 1] * inv, w[0][j], w[1][j]);
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s)
+      *reinterpret_cast<uint4*>(out + s * x.part() + (uint64_t)y * x.ld + q) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+  };
+  if (!m.tall) {
+    float v[EIGHTS][8];
+    const bool vector = k.hi % 8 == 0;
+#pragma unroll
+    for (int e = 0; e < EIGHTS; ++e) {
+      const uint32_t i = threadIdx.x + e * MUON_THREADS, y = y0 + i / (TILE / 8), q = x0 + i % (TILE / 8) * 8;
+      if (y >= k.lo || q >= k.hi) continue;
+      const uint64_t at = (uint64_t)y * k.hi + q;
+      load8<T>(v[e], g, at, q, k.hi, vector);
+      float f[8];
+      if (b) load8<T>(f, b, at, q, k.hi, vector);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[e][j] *= k.grad_scale;
+        if (b) v[e][j] = muon_direction(v[e][j], f[j], k);
+      }
+    }
+    __syncthreads();
+    const float inv = scale();
+#pragma unroll
+    for (int e = 0; e < EIGHTS; ++e) {
+      const uint32_t i = threadIdx.x + e * MUON_THREADS, y = y0 + i / (TILE / 8), q = x0 + i % (TILE / 8) * 8;
+      if (y < k.lo && q < k.hi) put(v[e], y, q, inv);
+    }
+    return;
   }
-  muon_tile<VEC>(r0, c0, rows, cols, cols % VEC == 0, [&](uint32_t r, uint32_t c, uint64_t i, bool vector) {
+  muon_tile<VEC>(x0, y0, k.hi, k.lo, k.lo % VEC == 0, [&](uint32_t r, uint32_t c, uint64_t i, bool vector) {
     if (vector) {
       RawVec<T, VEC> rg, rb;
       rg.load(g + i);
@@ -128,20 +193,15 @@ __global__ void __launch_bounds__(MUON_THREADS) muon_normalize_kernel(const __gr
     }
   });
   __syncthreads();
-  const float norm = (float)sqrt(total) + eps;
-  uint16_t* out = x.ptr + blockIdx.z * x.part() * PARTS;
-  for (int i = threadIdx.x; i < TILE * (TILE / 8); i += MUON_THREADS) {
-    const uint32_t y = i / (TILE / 8), q = i % (TILE / 8) * 8;
+  const float inv = scale();
+#pragma unroll
+  for (int e = 0; e < EIGHTS; ++e) {
+    const uint32_t i = threadIdx.x + e * MUON_THREADS, y = i % TILE, q = i / TILE * 8;       // lanes down a column of the tile: no bank twice
     if (y0 + y >= k.lo || x0 + q >= k.hi) continue;
-    uint32_t w[2][4];
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float u = m.tall ? tile[q + 2 * j][y] : tile[y][q + 2 * j], v = m.tall ? tile[q + 2 * j + 1][y] : tile[y][q + 2 * j + 1];
-      muon::split2(u / norm * muon::SCALE, v / norm * muon::SCALE, w[0][j], w[1][j]);      // behind the last column: spare
-    }
-#pragma unroll
-    for (int s = 0; s < PARTS; ++s)
-      *reinterpret_cast<uint4*>(out + s * x.part() + (uint64_t)(y0 + y) * x.ld + x0 + q) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+    for (int j = 0; j < 8; ++j) v[j] = x0 + q + j < k.hi ? tile[q + j][y] : 0.0f;
+    put(v, y0 + y, x0 + q, inv);
   }
 }
 
@@ -152,30 +212,67 @@ __global__ void __launch_bounds__(MUON_THREADS) muon_step_kernel(const __grid_co
   __shared__ float tile[TILE][TILE + 1];
   const MuonMatrix& m = k.m[blockIdx.z];
   const uint32_t x0 = blockIdx.x * TILE, y0 = blockIdx.y * TILE;
-  const uint32_t rows = m.tall ? k.hi : k.lo, cols = m.tall ? k.lo : k.hi, r0 = m.tall ? x0 : y0, c0 = m.tall ? y0 : x0;
   const uint16_t* in = x.ptr + blockIdx.z * x.part() * PARTS;
   const float step = (m.tall ? step_tall : step_flat) * muon::UNSCALE;
-  for (int i = threadIdx.x; i < TILE * (TILE / 8); i += MUON_THREADS) {
-    const uint32_t y = i / (TILE / 8), q = i % (TILE / 8) * 8;
-    if (y0 + y >= k.lo || x0 + q >= k.hi) continue;
-    float v[8];
+  S* p = (S*)m.p;
+  pdl_wait();
+  auto get = [&](float (&v)[8], uint32_t y, uint32_t q) {
 #pragma unroll
     for (int s = 0; s < PARTS; ++s) {
       RawVec<f16_t, 8> r;
-      r.load_stream(in + s * x.part() + (uint64_t)(y0 + y) * x.ld + x0 + q);
+      r.load_stream(in + s * x.part() + (uint64_t)y * x.ld + q);
       float f[8];
       r.decode(f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = s ? v[j] + f[j] : f[j];
     }
+  };
+  if (!m.tall) {
+    float v[EIGHTS][8], f[EIGHTS][8];
+    const bool vector = k.hi % 8 == 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (m.tall) tile[q + j][y] = v[j]; else tile[y][q + j] = v[j];
+    for (int e = 0; e < EIGHTS; ++e) {
+      const uint32_t i = threadIdx.x + e * MUON_THREADS, y = y0 + i / (TILE / 8), q = x0 + i % (TILE / 8) * 8;
+      if (y >= k.lo || q >= k.hi) continue;
+      get(v[e], y, q);
+      load8<T>(f[e], p, (uint64_t)y * k.hi + q, q, k.hi, vector);
     }
+#pragma unroll
+    for (int e = 0; e < EIGHTS; ++e) {
+      const uint32_t i = threadIdx.x + e * MUON_THREADS, y = y0 + i / (TILE / 8), q = x0 + i % (TILE / 8) * 8;
+      if (y >= k.lo || q >= k.hi) continue;
+      S* to = p + (uint64_t)y * k.hi + q;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[e][j] = f[e][j] * decay - step * v[e][j];
+      if (vector) {
+#pragma unroll
+        for (int h = 0; h < 8 / VEC; ++h) {
+          RawVec<T, VEC> r;
+          float o[VEC];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) o[j] = f[e][h * VEC + j];
+          round_encode<T, VEC>(r, o, k.rn != 0);
+          r.store(to + h * VEC);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (q + j < k.hi) to[j] = round_store<T>(f[e][j], k.rn != 0);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < EIGHTS; ++e) {
+    const uint32_t i = threadIdx.x + e * MUON_THREADS, y = i / (TILE / 8), q = i % (TILE / 8) * 8;
+    if (y0 + y >= k.lo || x0 + q >= k.hi) continue;
+    float v[8];
+    get(v, y0 + y, x0 + q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) tile[q + j][y] = v[j];
   }
   __syncthreads();
-  S* p = (S*)m.p;
-  muon_tile<VEC>(r0, c0, rows, cols, cols % VEC == 0, [&](uint32_t r, uint32_t c, uint64_t i, bool vector) {
+  muon_tile<VEC>(x0, y0, k.hi, k.lo, k.lo % VEC == 0, [&](uint32_t r, uint32_t c, uint64_t i, bool vector) {
     if (vector) {
       RawVec<T, VEC> rp;
       rp.load(p + i);
@@ -251,15 +348,15 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
   const unsigned sums = (unsigned)std::min<uint64_t>(MUON_PARTIALS, ((uint64_t)lo * hi + MUON_THREADS * 16 - 1) / (MUON_THREADS * 16));
   const dim3 tiles((hi + TILE - 1) / TILE, (lo + TILE - 1) / TILE, batch);
   muon_momentum_kernel<T><<<dim3(sums, batch), MUON_THREADS, 0, lc.stream>>>(k, partial);
-  muon_normalize_kernel<T, PARTS><<<tiles, MUON_THREADS, 0, lc.stream>>>(k, partial, (int)sums, d.eps == 0.0f ? 1e-7f : d.eps, x[0]);
+  cudaError_t e = launch_pdl(muon_normalize_kernel<T, PARTS>, tiles, MUON_THREADS, 0, lc.stream, k, partial, (int)sums, d.eps == 0.0f ? 1e-7f : d.eps, x[0]);
 
-  constexpr int BN = 256;
+  const int bn_sym = muon::tile_width<PARTS, true>(lo, lo, batch, lc.sm_count), bn_apply = muon::tile_width<PARTS, false>(lo, hi, batch, lc.sm_count);
   CUtensorMap x_rows[2], x_cols[2], x_k[2], gram_rows, gram_cols, poly_rows;
   bool ok = true;
   for (int j = 0; j < 2; ++j)
-    ok = ok && muon::encode(lc.tma_encode, &x_rows[j], x[j], PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &x_cols[j], x[j], PARTS, batch, BN) &&
+    ok = ok && muon::encode(lc.tma_encode, &x_rows[j], x[j], PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &x_cols[j], x[j], PARTS, batch, bn_sym) &&
          muon::encode(lc.tma_encode, &x_k[j], x[j], PARTS, batch, 64);
-  ok = ok && muon::encode(lc.tma_encode, &gram_rows, gram, PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &gram_cols, gram, PARTS, batch, BN) &&
+  ok = ok && muon::encode(lc.tma_encode, &gram_rows, gram, PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &gram_cols, gram, PARTS, batch, bn_sym) &&
        muon::encode(lc.tma_encode, &poly_rows, poly, PARTS, batch, muon::BM);
   if (!ok) { err = "muon: cuTensorMapEncodeTiled rejected an operand"; return ZYXB_ERR_KERNEL_LAUNCH; }
   float a, b, c;
@@ -270,20 +367,23 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
     return g;
   };
   const int steps = d.steps ? d.steps : 5;
-  cudaError_t e = cudaSuccess;
   for (int i = 0; i < steps && e == cudaSuccess; ++i) {
     const int from = i & 1;
-    e = muon::launch<PARTS, BN, true, false, false>(x_rows[from], x_cols[from], gemm_args(gram, hi), lc);
+    e = bn_sym == 128 ? muon::launch<PARTS, 128, true, false, false>(x_rows[from], x_cols[from], gemm_args(gram, hi), lc)
+                      : muon::launch<PARTS, 256, true, false, false>(x_rows[from], x_cols[from], gemm_args(gram, hi), lc);
     if (e != cudaSuccess) break;
     muon::GemmArgs g = gemm_args(poly, lo);
     g.gram = gram.ptr; g.a = a; g.b = b; g.c = c;
-    e = muon::launch<PARTS, BN, true, true, false>(gram_rows, gram_cols, g, lc);
+    e = bn_sym == 128 ? muon::launch<PARTS, 128, true, true, false>(gram_rows, gram_cols, g, lc)
+                      : muon::launch<PARTS, 256, true, true, false>(gram_rows, gram_cols, g, lc);
     if (e != cudaSuccess) break;
-    e = muon::launch<PARTS, BN, false, false, true>(poly_rows, x_k[from], gemm_args(x[from ^ 1], lo), lc);
+    e = bn_apply == 128 ? muon::launch<PARTS, 128, false, false, true>(poly_rows, x_k[from], gemm_args(x[from ^ 1], lo), lc)
+                        : muon::launch<PARTS, 256, false, false, true>(poly_rows, x_k[from], gemm_args(x[from ^ 1], lo), lc);
   }
   if (e != cudaSuccess) { err = std::string("muon: ") + cudaGetErrorString(e); return ZYXB_ERR_KERNEL_LAUNCH; }
-  muon_step_kernel<T, PARTS><<<tiles, MUON_THREADS, 0, lc.stream>>>(k, x[steps & 1], 1.0f - d.lr * d.weight_decay, d.lr * muon_adjust(d.adjust, lo, hi),
-                                                                   d.lr * muon_adjust(d.adjust, hi, lo));
+  e = launch_pdl(muon_step_kernel<T, PARTS>, tiles, MUON_THREADS, 0, lc.stream, k, x[steps & 1], 1.0f - d.lr * d.weight_decay,
+                 d.lr * muon_adjust(d.adjust, lo, hi), d.lr * muon_adjust(d.adjust, hi, lo));
+  if (e != cudaSuccess) { err = std::string("muon: ") + cudaGetErrorString(e); return ZYXB_ERR_KERNEL_LAUNCH; }
   return check_launch(lc, err, "muon", 3 + 3 * steps);
 }
 
@@ -296,7 +396,7 @@ int validate_muon(const zyxb_muon_desc& d, std::string& err) {
   for (int i = 0; i < d.n_tensors; ++i)
     if (d.rows[i] == 0 || d.cols[i] == 0 || d.rows[i] > MUON_MAX_EXTENT || d.cols[i] > MUON_MAX_EXTENT) return bad("muon: extents must be between 1 and 32768");
   if (d.steps < 0 || d.steps > 32) return bad("muon: at most 32 steps");
-  if (!(d.eps >= 0.0f)) return bad("muon: eps must not be negative");
+  if (!(d.eps == 0.0f || d.eps >= 1e-30f)) return bad("muon: eps must be at least 1e-30 (0 means 1e-7)");
   if (d.adjust != ZYXB_MUON_ADJUST_RATIO && d.adjust != ZYXB_MUON_ADJUST_RMS) return bad("muon: unknown adjust");
   // The products keep X in 16-bit floats: a polynomial that lets singular values grow from step to step would leave their range.
   float a, b, c;

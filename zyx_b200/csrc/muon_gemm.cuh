@@ -86,6 +86,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
 
   const uint32_t total = p.tiles * p.batch, k_blocks = (p.k + BK - 1) / BK;
   auto tile_coords = [&](uint32_t t, uint32_t& z, uint32_t& tm, uint32_t& tn) {
@@ -204,7 +206,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       // 32 columns from c on of this lane's row
       auto finish = [&](float (&v)[32], uint32_t c) {
         if (c >= p.n || row0 >= p.m) return;
-        if (SYM && c > row0 + 31) return;                      // wholly above the diagonal: the mirrored tile's
+        if (SYM && c > row0) return;                           // above the diagonal: another warp's mirrored block
         const uint64_t at = (uint64_t)row * p.ld + c;
         const bool mine = row < p.m;
         if constexpr (POLY) {
@@ -241,8 +243,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           if constexpr (PARTS == 2) split2(v[2 * j], v[2 * j + 1], w[0][j], w[PARTS - 1][j]);
           else w[0][j] = pack2_t<false>(v[2 * j], v[2 * j + 1]);
         }
-        const bool below = !SYM || c + 31 < row0;              // no entry of the warp's block on or above the diagonal
-        if (below && mine) {
+        if (mine) {
 #pragma unroll
           for (int s = 0; s < PARTS; ++s)
 #pragma unroll
@@ -251,8 +252,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
                 *reinterpret_cast<uint4*>(out + s * p.part + at + q * 8) = make_uint4(w[s][4 * q], w[s][4 * q + 1], w[s][4 * q + 2], w[s][4 * q + 3]);
         }
         if constexpr (SYM) {
-          if (below && row0 + 32 <= p.m) {
-            // mirrored: two neighbouring lanes trade halves, so that each stores two rows' entries of one column side by side
+          // Mirrored, unless the warp's 32 x 32 block lies on the diagonal (there the whole block has been computed and stored): two
+          // neighbouring lanes trade halves, so that each stores two rows' entries of one column side by side.
+          if (c < row0) {
             const bool odd = lane & 1;
 #pragma unroll
             for (int s = 0; s < PARTS; ++s)
@@ -260,18 +262,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
               for (int j = 0; j < 16; ++j) {
                 const uint32_t other = __shfl_xor_sync(0xffffffffu, w[s][j], 1);
                 const uint32_t pair = odd ? __byte_perm(other, w[s][j], 0x7632) : __byte_perm(w[s][j], other, 0x5410);
-                *reinterpret_cast<uint32_t*>(out + s * p.part + (uint64_t)(c + 2 * j + (odd ? 1 : 0)) * p.ld + (row & ~1u)) = pair;
-              }
-          } else if (mine) {
-#pragma unroll
-            for (int s = 0; s < PARTS; ++s)
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const uint32_t col = c + j;
-                if (col > row) continue;
-                const uint16_t h = (uint16_t)(w[s][j / 2] >> (16 * (j & 1)));
-                if (!below) out[s * p.part + (uint64_t)row * p.ld + col] = h;
-                if (col < row) out[s * p.part + (uint64_t)col * p.ld + row] = h;
+                if ((row | 1u) < p.ld)
+                  *reinterpret_cast<uint32_t*>(out + s * p.part + (uint64_t)(c + 2 * j + (odd ? 1 : 0)) * p.ld + (row & ~1u)) = pair;
               }
           }
         }
@@ -337,6 +329,21 @@ inline bool encode(void* fn, CUtensorMap* map, const Operand& o, int parts, uint
   return encode_map(fn, map, false, o.ptr, o.cols, o.rows, o.ld, (uint64_t)parts, parts > 1 ? o.part() : 0, batch, batch > 1 ? o.part() * parts : 0, box_rows);
 }
 
+// Tiles are 128 x 256, or 128 x 128 where those fill the SMs' last round better.  A narrow tile costs more per entry, because both
+// operands' reads from shared memory then run at its rate: 0.83 of a wide tile's time with one part (12.8 against 15.5 us at k = 2048),
+// 0.60 with two (26.2 against 45.9 us: there the tensor core multiplies three times what it reads).
+template <bool SYM> uint32_t tile_count(uint32_t m, uint32_t n, uint32_t bn) {
+  const uint32_t tiles_m = (m + BM - 1) / BM;
+  if (!SYM) return tiles_m * ((n + bn - 1) / bn);
+  uint32_t t = 0;
+  for (uint32_t tm = 0; tm < tiles_m; ++tm) t += tm / (bn / BM) + 1;
+  return t;
+}
+template <int PARTS, bool SYM> int tile_width(uint32_t m, uint32_t n, uint32_t batch, int sm_count) {
+  auto rounds = [&](uint32_t bn) { return (tile_count<SYM>(m, n, bn) * (uint64_t)batch + sm_count - 1) / sm_count; };
+  return (PARTS == 1 ? 83 : 60) * rounds(128) < 100 * rounds(256) ? 128 : 256;
+}
+
 template <int PARTS, int BN, bool SYM, bool POLY, bool B_MN>
 cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mb, GemmArgs p, const LaunchCtx& lc) {
   using SM = Smem<PARTS, BN>;
@@ -346,16 +353,10 @@ cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mb, GemmArgs p, con
   if (e != cudaSuccess) return e;
   p.tiles_m = (p.m + BM - 1) / BM;
   p.tiles_n = (p.n + BN - 1) / BN;
-  if (SYM) {
-    p.tiles = 0;
-    for (uint32_t tm = 0; tm < p.tiles_m; ++tm) p.tiles += tm / (BN / BM) + 1;
-  } else {
-    p.tiles = p.tiles_m * p.tiles_n;
-  }
+  p.tiles = tile_count<SYM>(p.m, p.n, BN);
   p.status = lc.status_word;
   const unsigned grid = (unsigned)std::min<uint64_t>((uint64_t)p.tiles * p.batch, (uint64_t)lc.sm_count);
-  kern<<<grid, THREADS, SM::TOTAL, lc.stream>>>(ma, mb, p);
-  return cudaGetLastError();
+  return launch_pdl(kern, dim3(grid), THREADS, SM::TOTAL, lc.stream, ma, mb, p);
 }
 
 }  // namespace muon
