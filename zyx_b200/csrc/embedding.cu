@@ -7,10 +7,11 @@
 // Gradient, three launches and no floating-point atomic:
 //   index    The vocabulary is cut into ranges, one CTA each.  Every CTA scans all token numbers (from L2; 64 KB at 16384 tokens),
 //            counts those below its range - which is where its part of the sorted order begins, so no CTA waits for another - and
-//            counting-sorts those inside it.  Rows that no token names are written as zeros here.
-//   sum      The sorted order is cut into chunks of equal length, whatever the token frequencies: a group of threads adds a chunk's
-//            rows in f32 registers, run by run.  A run inside one chunk is stored; a run that crosses a border leaves f32 partials.
-//   combine  Adds the partials of each crossing run, in chunk order.
+//            counting-sorts those inside it.
+//   sum      The sorted order is cut into chunks of equal length, whatever the token frequencies.  A group of threads adds the rows
+//            of the runs that begin in its chunk in f32 registers; a run of more than two chunks is shared by the chunks it
+//            crosses, each leaving f32 partials.  The same launch writes the rows of zeros.
+//   combine  Adds the partials of each shared run, in chunk order.
 // The order of every sum depends on ids alone.
 #include <algorithm>
 
@@ -23,9 +24,12 @@ namespace {
 
 constexpr int EMB_THREADS = 256;
 constexpr int EMB_TOKENS = 4;          // rows in flight per thread
-constexpr int IDX_THREADS = 512, IDX_WARPS = IDX_THREADS / 32;
-constexpr int IDX_MAX_ROWS = 1024;     // rows of a vocabulary range (histograms: 16 warps x 1024 x 4 B of shared memory)
-constexpr int CMB_WARPS = 16;
+constexpr int IDX_THREADS = 1024, IDX_WARPS = IDX_THREADS / 32;
+constexpr int IDX_MAX_ROWS = 1024;     // rows of a vocabulary range, one per thread (histograms: 32 warps x 1024 x 4 B of shared memory)
+constexpr int IDX_BATCH = 4;           // loads of four token numbers in flight per lane
+constexpr int CMB_WARPS = 8, CMB_COLS = 128;
+constexpr uint32_t CHUNK = 32;         // places of the sorted order per group; runs of more than two chunks are shared
+constexpr int FILL_ROWS = 64;          // table rows that a CTA of the sum launch looks through for absent ones
 
 template <typename ID> __device__ __forceinline__ int64_t id_at(const ID* ids, uint64_t i) { return (int64_t)ids[i]; }
 
@@ -65,7 +69,9 @@ embedding_kernel(const ID* __restrict__ ids, const typename Elem<T>::store_t* __
 }
 
 // ---- the sorted order ---------------------------------------------------------------------------------------------------------
+// token: its number below 2^24, FIRST on the first of a run (a table row's tokens), SHARED on all of a run longer than two chunks
 struct SortedToken { uint32_t row, token; };
+constexpr uint32_t FIRST = 1u << 31, SHARED = 1u << 30, TOKEN = (1u << 24) - 1;
 
 // four token numbers from position i on, -1 behind the last; i is a multiple of 4
 template <typename ID> __device__ __forceinline__ void load4(const ID* ids, uint32_t i, uint32_t n, int64_t (&v)[4]) {
@@ -83,102 +89,89 @@ template <typename ID> __device__ __forceinline__ void load4(const ID* ids, uint
   }
 }
 
-template <typename T, typename ID, int VEC>
+template <typename ID>
 __global__ void __launch_bounds__(IDX_THREADS)
-embedding_index_kernel(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, uint32_t range, SortedToken* __restrict__ sorted,
-                       uint32_t* __restrict__ starts, typename Elem<T>::store_t* __restrict__ dtable, uint64_t ld, uint32_t packs, int zero_rows) {
-  extern __shared__ uint32_t hist[];              // [warp][row of the range]
-  __shared__ uint32_t total[IDX_MAX_ROWS], warp_sum[IDX_WARPS], below_sum[IDX_WARPS];
+embedding_index_kernel(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, uint32_t range, uint32_t long_run, SortedToken* __restrict__ sorted, uint32_t* __restrict__ starts) {
+  extern __shared__ uint32_t hist[];              // [warp][row of the range]: counts, then the next free place
+  __shared__ uint32_t first[IDX_MAX_ROWS], shared_run[IDX_MAX_ROWS / 32], warp_sum[IDX_WARPS], below_sum[IDX_WARPS];
+  pdl_trigger();
   const uint32_t lo = blockIdx.x * range, rows = min(range, vocab - lo);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* mine = hist + warp * range;
   for (uint32_t i = threadIdx.x; i < IDX_WARPS * range; i += IDX_THREADS) hist[i] = 0;
   __syncthreads();
   // each warp owns one slice of the tokens, in both passes
+  constexpr uint32_t STEP = 128 * IDX_BATCH;
   const uint32_t slice = ((n + IDX_WARPS - 1) / IDX_WARPS + 127) / 128 * 128;
   const uint32_t begin = min(n, warp * slice), end = min(n, begin + slice);
   uint32_t below = 0;
-#pragma unroll 4
-  for (uint32_t i = begin + lane * 4; i < end; i += 128) {
-    int64_t v[4];
-    load4(ids, i, end, v);
+  for (uint32_t i0 = begin; i0 < end; i0 += STEP) {
+    int64_t v[IDX_BATCH][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint64_t r = (uint64_t)v[j] - lo;             // a negative number is far above any range
-      if (r < rows) atomicAdd(&mine[r], 1u);
-      else below += v[j] >= 0 && v[j] < (int64_t)lo;
-    }
+    for (int q = 0; q < IDX_BATCH; ++q) load4(ids, i0 + q * 128 + lane * 4, end, v[q]);
+#pragma unroll
+    for (int q = 0; q < IDX_BATCH; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t r = (uint64_t)v[q][j] - lo;             // a negative number is far above any range
+        if (r < rows) atomicAdd(&mine[r], 1u);
+        else below += v[q][j] >= 0 && v[q][j] < (int64_t)lo;
+      }
   }
   below = warp_reduce(below, OpSum());
   if (lane == 0) below_sum[warp] = below;
   __syncthreads();
-  uint32_t base = 0;
-#pragma unroll
-  for (int w = 0; w < IDX_WARPS; ++w) base += below_sum[w];
-  // exclusive scan over (row, warp): two consecutive rows per thread
-  uint32_t t[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const uint32_t r = threadIdx.x * 2 + k;
-    t[k] = 0;
-    if (r < rows)
-      for (int w = 0; w < IDX_WARPS; ++w) t[k] += hist[w * range + r];
-    if (r < rows) total[r] = t[k];
+  // exclusive scan over (row, warp), a row per thread
+  uint32_t total = 0, at = 0;
+  if (threadIdx.x < rows) {
+#pragma unroll 8
+    for (int w = 0; w < IDX_WARPS; ++w) total += hist[w * range + threadIdx.x];
   }
-  uint32_t s = t[0] + t[1];
+  uint32_t s = total;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t up = __shfl_up_sync(0xffffffffu, s, o);
     if (lane >= o) s += up;
   }
   if (lane == 31) warp_sum[warp] = s;
+  const uint32_t longs = __ballot_sync(0xffffffffu, total > long_run);
+  if (lane == 0) shared_run[warp] = longs;
   __syncthreads();
-  uint32_t at = base + s - (t[0] + t[1]);
-  for (int w = 0; w < warp; ++w) at += warp_sum[w];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const uint32_t r = threadIdx.x * 2 + k;
-    if (r < rows) {
-      starts[lo + r] = at;
-      uint32_t run = at;
-      for (int w = 0; w < IDX_WARPS; ++w) { const uint32_t c = hist[w * range + r]; hist[w * range + r] = run; run += c; }
-      at = run;
-      if (lo + r == vocab - 1) starts[vocab] = at;
-    }
+  at = warp_reduce(below_sum[lane] + (lane < warp ? warp_sum[lane] : 0u), OpSum()) + s - total;
+  if (threadIdx.x < rows) {
+    starts[lo + threadIdx.x] = at;
+    first[threadIdx.x] = at;
+    uint32_t run = at;
+#pragma unroll 8
+    for (int w = 0; w < IDX_WARPS; ++w) { const uint32_t c = hist[w * range + threadIdx.x]; hist[w * range + threadIdx.x] = run; run += c; }
+    if (lo + threadIdx.x == vocab - 1) starts[vocab] = run;
   }
   __syncthreads();
   // second pass: equal rows of a warp's 32 lanes take consecutive places
-#pragma unroll 4
-  for (uint32_t i0 = begin; i0 < end; i0 += 128) {
-    int64_t v[4];
-    const uint32_t i = i0 + lane * 4;
-    if (i < end) load4(ids, i, end, v);
-    else { v[0] = v[1] = v[2] = v[3] = -1; }
+  for (uint32_t i0 = begin; i0 < end; i0 += STEP) {
+    int64_t v[IDX_BATCH][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint64_t r = (uint64_t)v[j] - lo;             // a negative number is far above any range
-      const bool in = r < rows;
-      const uint32_t active = __ballot_sync(0xffffffffu, in);
-      if (active == 0) continue;
-      if (in) {
-        const uint32_t same = __match_any_sync(active, (uint32_t)r);
-        const uint32_t rank = __popc(same & ((1u << lane) - 1u));
-        const uint32_t place = mine[r];
-        sorted[place + rank] = SortedToken{lo + (uint32_t)r, i + j};
-        __syncwarp(active);
-        if (rank == 0) mine[r] = place + __popc(same);
+    for (int q = 0; q < IDX_BATCH; ++q) load4(ids, i0 + q * 128 + lane * 4, end, v[q]);
+#pragma unroll
+    for (int q = 0; q < IDX_BATCH; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t r = (uint64_t)v[q][j] - lo;
+        const bool in = r < rows;
+        const uint32_t active = __ballot_sync(0xffffffffu, in);
+        if (active == 0) continue;
+        if (in) {
+          const uint32_t same = __match_any_sync(active, (uint32_t)r), rank = __popc(same & ((1u << lane) - 1u));
+          const uint32_t place = mine[r];
+          uint32_t token = i0 + q * 128 + lane * 4 + j;
+          if (place + rank == first[r]) token |= FIRST;
+          if (shared_run[r >> 5] >> (r & 31) & 1u) token |= SHARED;
+          sorted[place + rank] = SortedToken{lo + (uint32_t)r, token};
+          __syncwarp(active);
+          if (rank == 0) mine[r] = place + __popc(same);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-    }
-  }
-  if (zero_rows) {
-    RawVec<T, VEC> z;
-    z.zero();
-    for (uint32_t r = warp; r < rows; r += IDX_WARPS) {
-      if (total[r] != 0) continue;
-      auto* row = dtable + (uint64_t)(lo + r) * ld;
-      for (uint32_t k = lane; k < packs; k += 32) z.store_stream(row + (uint64_t)k * VEC);
-    }
   }
 }
 
@@ -186,8 +179,8 @@ embedding_index_kernel(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, u
 struct EmbGradParams {
   const SortedToken* sorted;
   const uint32_t* starts;      // [vocab + 1]
-  float* partial;              // [chunk][2][dim]: 0 the run that came in from the chunk before, 1 the one that begins here and goes on
-  uint32_t vocab, dim, packs, chunk;
+  float* partial;              // [chunk][2][dim]: 0 the shared run that came in from the chunk before, 1 the one that begins here
+  uint32_t vocab, dim, packs, chunk, chunks, sum_ctas;
   uint64_t ld_table, ld_out;
   float scale;
   int accumulate, rn;
@@ -211,107 +204,121 @@ __device__ __forceinline__ void emb_store_row(typename Elem<T>::store_t* dst, fl
 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(EMB_THREADS)
-embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typename Elem<T>::store_t* dtable, EmbGradParams p, int log_tpt) {
+embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typename Elem<T>::store_t* dtable, const EmbGradParams p, int log_tpt) {
   constexpr int U = 8;
-  const uint32_t tpt = 1u << log_tpt, groups = EMB_THREADS >> log_tpt;
-  const uint32_t c = blockIdx.x * groups + (threadIdx.x >> log_tpt);
+  const uint32_t tpt = 1u << log_tpt, groups = EMB_THREADS >> log_tpt, group = threadIdx.x >> log_tpt;
   const uint32_t pack = blockIdx.y * tpt + (threadIdx.x & (tpt - 1));
+  const uint64_t col = (uint64_t)pack * VEC;
+  pdl_trigger();
+  pdl_wait();
+  if (pack >= p.packs) return;
+  if (blockIdx.x >= p.sum_ctas) {         // rows that no token names
+    const uint32_t r0 = (blockIdx.x - p.sum_ctas) * FILL_ROWS;
+    RawVec<T, VEC> z;
+    z.zero();
+#pragma unroll 4
+    for (uint32_t r = r0 + group; r < min(p.vocab, r0 + FILL_ROWS); r += groups)
+      if (p.starts[r] == p.starts[r + 1]) z.store_stream(dtable + (uint64_t)r * p.ld_table + col);
+    return;
+  }
+  const uint32_t c = blockIdx.x * groups + group;
   const uint32_t n = p.starts[p.vocab];
   const uint64_t begin64 = (uint64_t)c * p.chunk;
-  if (begin64 >= n || pack >= p.packs) return;
+  if (begin64 >= n) return;
   const uint32_t begin = (uint32_t)begin64, end = (uint32_t)min((uint64_t)n, begin64 + p.chunk);
-  const uint64_t col = (uint64_t)pack * VEC;
+  // runs that begin here are taken whole, unless they are shared; one that came in is taken only if it is shared
+  const SortedToken head = p.sorted[begin], tail = p.sorted[end - 1];
+  const uint32_t lo = head.token & (FIRST | SHARED) ? begin : p.starts[head.row + 1];
+  const uint32_t hi = tail.token & SHARED ? end : p.starts[tail.row + 1];
+  if (lo >= hi) return;
   float acc[VEC];
-  uint32_t row = 0xffffffffu;
-  auto flush = [&](uint32_t stop) {       // the run of `row` ends at `stop` (its end, or the chunk's)
-    float* part = p.partial + (uint64_t)c * 2 * p.dim + col;
-    const bool came_in = p.starts[row] < begin, goes_on = stop == end && p.starts[row + 1] > end;
-    if (came_in) {
+  uint32_t row = 0, slot = (head.token & FIRST) || lo != begin ? 1 : 0;
+  bool shared = false;
+  auto flush = [&] {
+    if (shared) {
+      float* part = p.partial + ((uint64_t)c * 2 + slot) * p.dim + col;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) part[k] = acc[k];
-    } else if (goes_on) {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) part[p.dim + k] = acc[k];
     } else {
       emb_store_row<T, VEC>(dtable + (uint64_t)row * p.ld_table + col, acc, p);
     }
+    slot = 1;
   };
-  for (uint32_t i = begin; i < end; i += U) {
-    SortedToken s[U];
-    RawVec<T, VEC> r[U];
+  SortedToken s[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) s[u] = i + u < end ? p.sorted[i + u] : SortedToken{0xffffffffu, 0};
+  for (int u = 0; u < U; ++u) s[u] = p.sorted[min(lo + u, hi - 1)];
+  for (uint32_t i = lo; i < hi; i += U) {
+    RawVec<T, VEC> r[U];
+    SortedToken next[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i + u < end) r[u].load_stream(dout + (uint64_t)s[u].token * p.ld_out + col);
+      if (i + u < hi) r[u].load_stream(dout + (uint64_t)(s[u].token & TOKEN) * p.ld_out + col);
+#pragma unroll
+    for (int u = 0; u < U; ++u) next[u] = p.sorted[min(i + U + u, hi - 1)];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (i + u >= end) break;
-      float v[VEC];
-      r[u].decode(v);
-      if (s[u].row != row) {
-        if (row != 0xffffffffu) flush(i + u);
-        row = s[u].row;
+      if (i + u < hi) {
+        float v[VEC];
+        r[u].decode(v);
+        const bool starts_run = (s[u].token & FIRST) || i + u == lo;
+        if (starts_run) {
+          if (i + u != lo) flush();
+          row = s[u].row;
+          shared = s[u].token & SHARED;
+        }
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] = v[k];
-      } else {
+        for (int k = 0; k < VEC; ++k) acc[k] = starts_run ? v[k] : acc[k] + v[k];
+      }
+    }
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+    for (int u = 0; u < U; ++u) s[u] = next[u];
+  }
+  flush();
+}
+
+// CTA: eight chunks x 128 columns.  Each warp looks whether a shared run begins in one of them; each run found is added by all warps,
+// which take consecutive shares of its partials.
+template <typename T>
+__global__ void __launch_bounds__(CMB_WARPS * 32)
+embedding_combine_kernel(typename Elem<T>::store_t* dtable, const EmbGradParams p) {
+  __shared__ uint32_t found[CMB_WARPS][3];           // row, first chunk, last chunk
+  __shared__ float part[CMB_WARPS][CMB_COLS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  const uint32_t n = p.starts[p.vocab], c = blockIdx.x * CMB_WARPS + warp;
+  const uint64_t begin = (uint64_t)c * p.chunk, end = begin + p.chunk;
+  if (lane == 0) {
+    found[warp][2] = 0;
+    if (end < n) {
+      const SortedToken s = p.sorted[end - 1];
+      if (s.token & SHARED) {
+        const uint32_t r0 = p.starts[s.row], r1 = p.starts[s.row + 1];
+        if (r0 >= begin) { found[warp][0] = s.row; found[warp][1] = c; found[warp][2] = (r1 - 1) / p.chunk; }
       }
     }
   }
-  flush(end);
-}
-
-// One warp per 32 columns and share of the partials; the CTA's warps split each crossing run's list.
-template <typename T>
-__global__ void __launch_bounds__(CMB_WARPS * 32)
-embedding_combine_kernel(typename Elem<T>::store_t* dtable, EmbGradParams p, uint32_t chunks) {
-  __shared__ uint32_t list[CMB_WARPS * 32];
-  __shared__ uint32_t found;
-  __shared__ float part[CMB_WARPS][32];
-  const uint32_t n = p.starts[p.vocab];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t col = blockIdx.x * 32 + lane;
-  // the chunks this CTA looks at: y, y + Y, ...; those whose last run begins in them and goes on are listed, in order
-  for (uint32_t t0 = blockIdx.y; t0 < chunks; t0 += gridDim.y * (CMB_WARPS * 32)) {
-    const uint64_t c = t0 + (uint64_t)threadIdx.x * gridDim.y, begin = c * p.chunk, end = begin + p.chunk;
-    bool crosses = false;
-    if (c < chunks && end < n) {
-      const uint32_t row = p.sorted[end - 1].row;
-      crosses = p.starts[row] >= begin && p.starts[row + 1] > end;
-    }
-    const uint32_t ballot = __ballot_sync(0xffffffffu, crosses);
-    __shared__ uint32_t warp_count[CMB_WARPS];
-    if (lane == 0) warp_count[warp] = __popc(ballot);
-    __syncthreads();
-    uint32_t at = __popc(ballot & ((1u << lane) - 1u));
-    for (int w = 0; w < warp; ++w) at += warp_count[w];
-    if (crosses) list[at] = (uint32_t)c;
-    if (threadIdx.x == CMB_WARPS * 32 - 1) found = at + (crosses ? 1 : 0);
-    __syncthreads();
-    const uint32_t m = found;
-    for (uint32_t q = 0; q < m; ++q) {
-      const uint32_t c0 = list[q];
-      const uint32_t row = p.sorted[(uint64_t)c0 * p.chunk + p.chunk - 1].row;
-      const uint32_t last = (p.starts[row + 1] - 1) / p.chunk, count = last - c0;       // partials behind the first chunk's
-      const uint32_t per = (count + CMB_WARPS - 1) / CMB_WARPS;
+  __syncthreads();
+  for (int q = 0; q < CMB_WARPS; ++q) {
+    if (found[q][2] == 0) continue;                  // a shared run ends behind its first chunk
+    const uint32_t row = found[q][0], c0 = found[q][1], count = found[q][2] - c0 + 1, per = (count + CMB_WARPS - 1) / CMB_WARPS;
+    const uint32_t k0 = min(count, warp * per), k1 = min(count, k0 + per);
+#pragma unroll
+    for (int h = 0; h < CMB_COLS / 32; ++h) {
+      const uint32_t col = blockIdx.y * CMB_COLS + h * 32 + lane;
       float sum = 0.0f;
       if (col < p.dim) {
-        if (warp == 0) sum = p.partial[((uint64_t)c0 * 2 + 1) * p.dim + col];
-        const uint32_t k0 = min(count, warp * per), k1 = min(count, k0 + per);
 #pragma unroll 8
-        for (uint32_t k = k0; k < k1; ++k) sum += p.partial[(uint64_t)(c0 + 1 + k) * 2 * p.dim + col];
+        for (uint32_t k = k0; k < k1; ++k) sum += p.partial[((uint64_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * p.dim + col];
       }
-      part[warp][lane] = sum;
-      __syncthreads();
-      if (warp == 0 && col < p.dim) {
-        float acc[1] = {0.0f};
+      part[warp][h * 32 + lane] = sum;
+    }
+    __syncthreads();
+    const uint32_t col = blockIdx.y * CMB_COLS + threadIdx.x;
+    if (threadIdx.x < CMB_COLS && col < p.dim) {
+      float acc[1] = {0.0f};
 #pragma unroll
-        for (int w = 0; w < CMB_WARPS; ++w) acc[0] += part[w][lane];
-        emb_store_row<T, 1>(dtable + (uint64_t)row * p.ld_table + col, acc, p);
-      }
-      __syncthreads();
+      for (int w = 0; w < CMB_WARPS; ++w) acc[0] += part[w][threadIdx.x];
+      emb_store_row<T, 1>(dtable + (uint64_t)row * p.ld_table + col, acc, p);
     }
     __syncthreads();
   }
@@ -357,23 +364,21 @@ cudaError_t run_embedding_bwd(const zyxb_embedding_desc& d, uint64_t ldt, uint64
   p.sorted = (const SortedToken*)scratch; p.starts = (const uint32_t*)(scratch + pl.starts_off); p.partial = (float*)(scratch + pl.partial_off);
   p.vocab = (uint32_t)d.vocab; p.dim = (uint32_t)d.dim; p.packs = (uint32_t)(d.dim / VEC); p.chunk = pl.chunk;
   p.ld_table = ldt; p.ld_out = ldo; p.scale = scale; p.accumulate = d.accumulate ? 1 : 0; p.rn = lc.round_nearest ? 1 : 0;
-  const int smem = (int)(IDX_WARPS * pl.range * 4);
+  p.chunks = pl.chunks;
   static uint64_t configured = 0;
-  cudaError_t e = ensure_dynamic_smem(embedding_index_kernel<T, ID, VEC>, IDX_WARPS * IDX_MAX_ROWS * 4, &configured);
+  cudaError_t e = ensure_dynamic_smem(embedding_index_kernel<ID>, IDX_WARPS * IDX_MAX_ROWS * 4, &configured);
   if (e != cudaSuccess) return e;
-  embedding_index_kernel<T, ID, VEC><<<pl.ranges, IDX_THREADS, smem, lc.stream>>>((const ID*)args[0], (uint32_t)d.tokens, (uint32_t)d.vocab, pl.range,
-                                                                                (SortedToken*)scratch, (uint32_t*)(scratch + pl.starts_off), (S*)args[2],
-                                                                                ldt, p.packs, p.accumulate ? 0 : 1);
+  embedding_index_kernel<ID><<<pl.ranges, IDX_THREADS, IDX_WARPS * pl.range * 4, lc.stream>>>((const ID*)args[0], (uint32_t)d.tokens, (uint32_t)d.vocab, pl.range, 2 * pl.chunk,
+                                                                                            (SortedToken*)scratch, (uint32_t*)(scratch + pl.starts_off));
   const int log_tpt = log2_ceil(p.packs, 8);
   const uint32_t groups = EMB_THREADS >> log_tpt;
-  const dim3 grid((pl.chunks + groups - 1) / groups, (unsigned)((p.packs + (1u << log_tpt) - 1) >> log_tpt));
-  embedding_sum_kernel<T, VEC><<<grid, EMB_THREADS, 0, lc.stream>>>((const S*)args[1], (S*)args[2], p, log_tpt);
-  if (pl.chunks > 1) {
-    const unsigned slabs = (unsigned)((d.dim + 31) / 32);
-    const unsigned ys = std::max(1u, std::min(pl.chunks, 592u / slabs));
-    embedding_combine_kernel<T><<<dim3(slabs, ys), CMB_WARPS * 32, 0, lc.stream>>>((S*)args[2], p, pl.chunks);
-  }
-  return cudaSuccess;
+  p.sum_ctas = (pl.chunks + groups - 1) / groups;
+  const unsigned fill = p.accumulate ? 0 : (p.vocab + FILL_ROWS - 1) / FILL_ROWS;
+  const dim3 grid(p.sum_ctas + fill, (unsigned)((p.packs + (1u << log_tpt) - 1) >> log_tpt));
+  e = launch_pdl(embedding_sum_kernel<T, VEC>, grid, EMB_THREADS, 0, lc.stream, (const S*)args[1], (S*)args[2], p, log_tpt);
+  if (e != cudaSuccess || d.tokens <= 2 * pl.chunk) return e;
+  return launch_pdl(embedding_combine_kernel<T>, dim3((pl.chunks + CMB_WARPS - 1) / CMB_WARPS, (unsigned)((d.dim + CMB_COLS - 1) / CMB_COLS)), CMB_WARPS * 32, 0,
+                    lc.stream, (S*)args[2], p);
 }
 
 }  // namespace
@@ -436,7 +441,7 @@ int launch_embedding_bwd(const zyxb_embedding_desc& d, void* const* args, const 
   pl.ranges = (uint32_t)((d.vocab + pl.range - 1) / pl.range);
   pl.starts_off = (d.tokens * sizeof(SortedToken) + 255) / 256 * 256;
   pl.partial_off = pl.starts_off + ((d.vocab + 1) * 4 + 255) / 256 * 256;
-  pl.chunk = 32;
+  pl.chunk = CHUNK;
   auto chunks = [&] { return (d.tokens + pl.chunk - 1) / pl.chunk; };
   while (chunks() > 1 && pl.partial_off + chunks() * 2 * d.dim * 4 > lc.scratch_bytes) pl.chunk *= 2;     // partials have to fit the scratch
   pl.chunks = (uint32_t)chunks();
@@ -448,7 +453,7 @@ int launch_embedding_bwd(const zyxb_embedding_desc& d, void* const* args, const 
   ZYXB_EMB_DISPATCH(ZYXB_EMB_BWD)
 #undef ZYXB_EMB_BWD
   if (e != cudaSuccess) { err = std::string("embedding gradient: ") + cudaGetErrorString(e); return ZYXB_ERR_KERNEL_LAUNCH; }
-  return check_launch(lc, err, "embedding gradient", pl.chunks > 1 ? 3 : 2);
+  return check_launch(lc, err, "embedding gradient", d.tokens > 2 * pl.chunk ? 3 : 2);
 }
 
 }  // namespace zyxb

@@ -114,7 +114,37 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 
 constexpr float E4M3_MAX = 448.0f, AMAX_FLOOR = 1e-30f;
 
-template <typename T, int PACKS, bool ALIGNED, bool QUANT>
+// a vector of y as 8-bit floats; scale_of(column)
+template <typename T, bool ALIGNED, class F>
+__device__ __forceinline__ void put_e4m3(const RowView<T, ALIGNED>& view, const float (&y)[RowView<T, ALIGNED>::VEC], const RmsParams& p, uint64_t row, int pack, F scale_of) {
+  constexpr int VEC = RowView<T, ALIGNED>::VEC;
+  uint8_t* out = reinterpret_cast<uint8_t*>(p.y) + row * p.cols;
+  const int c0 = view.col(pack);
+  float q[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) q[k] = y[k] / scale_of(c0 + k);
+  uint32_t w[VEC / 4];
+#pragma unroll
+  for (int k = 0; k < VEC / 4; ++k) w[k] = e4m3x2(q[4 * k], q[4 * k + 1]) | (e4m3x2(q[4 * k + 2], q[4 * k + 3]) << 16);
+  if (ALIGNED) {
+    if constexpr (VEC == 8) __stcs(reinterpret_cast<uint2*>(out + c0), make_uint2(w[0], w[1]));
+    else __stcs(reinterpret_cast<uint32_t*>(out + c0), w[0]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      if (view.inside(c0 + k)) out[c0 + k] = (uint8_t)(w[k / 4] >> (8 * (k % 4)));
+  }
+}
+
+// How the largest |y| of a column group is found: LANES where a group is a power of two of whole vectors, which lie in neighbouring
+// lanes of one warp (shuffles; 1 scale per 128 columns of bf16 is 16 lanes); SHARED for every other group (integer maxima in shared
+// memory, one per warp where a row is one group).
+enum { QUANT_NONE = 0, QUANT_LANES = 1, QUANT_SHARED = 2 };
+
+// the bits of |y| order like the values, and a NaN above all of them: it becomes its group's scale
+__device__ __forceinline__ uint32_t amax_bits_of(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+template <typename T, int PACKS, bool ALIGNED, int QUANT>
 __global__ void __launch_bounds__(1024) rmsnorm_kernel(RmsParams p) {
   using View = RowView<T, ALIGNED>;
   constexpr int VEC = View::VEC;
@@ -152,7 +182,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_kernel(RmsParams p) {
       for (int k = 0; k < VEC; ++k) sum[0] += h[i][k] * h[i][k];
     }
   }
-  if constexpr (QUANT) {
+  if constexpr (QUANT == QUANT_SHARED) {
     for (uint32_t g = threadIdx.x; g < (blockDim.x >> p.log_tpr) * p.n_groups; g += blockDim.x) amax_bits[g] = __float_as_uint(AMAX_FLOOR);
     if (p.log_tpr <= 5) __syncthreads();             // wider rows pass a barrier in row_sum
   }
@@ -171,52 +201,63 @@ __global__ void __launch_bounds__(1024) rmsnorm_kernel(RmsParams p) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) h[i][k] *= rstd;
     }
-    if constexpr (!QUANT) view.store(h[i], p.y, pack, p.rn != 0);
+    if constexpr (QUANT == QUANT_NONE) view.store(h[i], p.y, pack, p.rn != 0);
   }
-  if constexpr (QUANT) {
-    // The bits of |y| order like the values, and a NaN above all of them: it becomes its group's scale.
-    uint32_t* mine = amax_bits + in_cta * p.n_groups;
+  if constexpr (QUANT == QUANT_LANES) {
+    const int width = (int)p.group / VEC;              // lanes per column group
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int pack = t + i * tpr;
-      if (!live || !view.has(pack)) continue;
-      const int c0 = max(0, view.col(pack)), c1 = min((int)p.cols, view.col(pack) + VEC) - 1;
-      const uint32_t g0 = (uint32_t)c0 / p.group, g1 = (uint32_t)c1 / p.group;
-      uint32_t m0 = 0, m1 = 0;                       // a vector meets at most two groups
+      const bool in = live && view.has(pack);
+      uint32_t m = __float_as_uint(AMAX_FLOOR);
+      if (in) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const int c = view.col(pack) + k;
-        if (!view.inside(c)) continue;
-        const uint32_t b = __float_as_uint(h[i][k]) & 0x7fffffffu;
-        if ((uint32_t)c < (g0 + 1) * p.group) m0 = max(m0, b); else m1 = max(m1, b);
+        for (int k = 0; k < VEC; ++k) m = max(m, amax_bits_of(h[i][k]));
       }
-      atomicMax(&mine[g0], m0);
-      if (g1 != g0) atomicMax(&mine[g1], m1);
+      for (int o = width >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if (!in) continue;
+      const float scale = __uint_as_float(m) / E4M3_MAX;
+      put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int) { return scale; });
+      if (pack % width == 0) p.scales[row * p.n_groups + pack / width] = scale;
+    }
+  }
+  if constexpr (QUANT == QUANT_SHARED) {
+    uint32_t* mine = amax_bits + in_cta * p.n_groups;
+    if (p.n_groups == 1) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < PACKS; ++i)
+        if (live && view.has(t + i * tpr)) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) m = max(m, view.inside(view.col(t + i * tpr) + k) ? amax_bits_of(h[i][k]) : 0u);
+        }
+      for (int o = min(32, tpr) >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if ((t & 31) == 0) atomicMax(&mine[0], m);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PACKS; ++i) {
+        const int pack = t + i * tpr;
+        if (!live || !view.has(pack)) continue;
+        const int c0 = max(0, view.col(pack)), c1 = min((int)p.cols, view.col(pack) + VEC) - 1;
+        const uint32_t g0 = (uint32_t)c0 / p.group, g1 = (uint32_t)c1 / p.group;
+        uint32_t m0 = 0, m1 = 0;                       // a vector meets at most two groups
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const int c = view.col(pack) + k;
+          if (!view.inside(c)) continue;
+          const uint32_t b = amax_bits_of(h[i][k]);
+          if ((uint32_t)c < (g0 + 1) * p.group) m0 = max(m0, b); else m1 = max(m1, b);
+        }
+        atomicMax(&mine[g0], m0);
+        if (g1 != g0) atomicMax(&mine[g1], m1);
+      }
     }
     __syncthreads();
-    uint8_t* y = reinterpret_cast<uint8_t*>(p.y) + row * p.cols;
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int pack = t + i * tpr;
       if (!live || !view.has(pack)) continue;
-      const int c0 = view.col(pack);
-      float q[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const int c = min(max(c0 + k, 0), (int)p.cols - 1);
-        q[k] = h[i][k] / (__uint_as_float(mine[(uint32_t)c / p.group]) / E4M3_MAX);
-      }
-      uint32_t w[VEC / 4];
-#pragma unroll
-      for (int k = 0; k < VEC / 4; ++k) w[k] = e4m3x2(q[4 * k], q[4 * k + 1]) | (e4m3x2(q[4 * k + 2], q[4 * k + 3]) << 16);
-      if (ALIGNED) {
-        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(y + c0) = make_uint2(w[0], w[1]);
-        else *reinterpret_cast<uint32_t*>(y + c0) = w[0];
-      } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k)
-          if (view.inside(c0 + k)) y[c0 + k] = (uint8_t)(w[k / 4] >> (8 * (k % 4)));
-      }
+      put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int c) { return __uint_as_float(mine[p.n_groups == 1 ? 0 : (uint32_t)min(max(c, 0), (int)p.cols - 1) / p.group]) / E4M3_MAX; });
     }
     if (live)
       for (uint32_t g = t; g < p.n_groups; g += tpr) p.scales[row * p.n_groups + g] = __uint_as_float(mine[g]) / E4M3_MAX;
@@ -229,6 +270,7 @@ template <typename T, int PACKS, bool ALIGNED>
 __global__ void __launch_bounds__(1024) rmsnorm_bwd_kernel(RmsParams p) {
   using View = RowView<T, ALIGNED>;
   constexpr int VEC = View::VEC;
+  constexpr bool PREFETCH = PACKS * VEC <= 8;        // what 64 registers hold twice
   __shared__ float red[2][32][2];
   extern __shared__ float dw_shared[];               // [group of the CTA][cols]
   const int tpr = 1 << p.log_tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & (tpr - 1), groups = blockDim.x >> p.log_tpr;
@@ -241,29 +283,35 @@ __global__ void __launch_bounds__(1024) rmsnorm_bwd_kernel(RmsParams p) {
   if (!ALIGNED && p.weight_on)
     for (uint32_t c = t; c < p.cols; c += tpr) dw_mine[c] = 0.0f;
   const uint64_t step = (uint64_t)gridDim.x * groups;
-  int parity = 0;
-  for (uint64_t row0 = (uint64_t)blockIdx.x * groups; row0 < p.rows; row0 += step, parity ^= 1) {
-    const uint64_t row = row0 + in_cta;
-    const bool live = row < p.rows;
-    const View view(live ? row : 0, p.ld, p.cols);
-    RawVec<T, VEC> rh[PACKS], rg[PACKS], rd[PACKS];
+  struct Row { RawVec<T, VEC> h[PACKS], g[PACKS], d[PACKS]; };
+  auto fetch = [&](Row& r, uint64_t row) {
+    const View view(row, p.ld, p.cols);
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int pack = t + i * tpr;
-      rh[i].zero(); rg[i].zero(); rd[i].zero();
-      if (live && view.has(pack)) {
-        view.load(rh[i], p.h, pack);
-        view.load(rg[i], p.dy, pack);
-        if (p.dh_on) view.load(rd[i], p.dh, pack);
+      r.h[i].zero(); r.g[i].zero(); r.d[i].zero();
+      if (row < p.rows && view.has(pack)) {
+        view.load(r.h[i], p.h, pack);
+        view.load(r.g[i], p.dy, pack);
+        if (p.dh_on) view.load(r.d[i], p.dh, pack);
       }
     }
+  };
+  int parity = 0;
+  Row now, next;
+  fetch(now, (uint64_t)blockIdx.x * groups + in_cta);
+  for (uint64_t row0 = (uint64_t)blockIdx.x * groups; row0 < p.rows; row0 += step, parity ^= 1) {
+    const uint64_t row = row0 + in_cta;
+    const bool live = row < p.rows;
+    const View view(row, p.ld, p.cols);
+    if (PREFETCH) fetch(next, row + step);          // in flight during this row's sums
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int pack = t + i * tpr;
       float h[VEC], g[VEC];
-      rh[i].decode(h);
-      rg[i].decode(g);
+      now.h[i].decode(h);
+      now.g[i].decode(g);
       if (p.weight_on && live && view.has(pack)) {
         float w[VEC];
         view.weight(w, p.weight, pack);
@@ -282,8 +330,8 @@ __global__ void __launch_bounds__(1024) rmsnorm_bwd_kernel(RmsParams p) {
       const int pack = t + i * tpr;
       if (!live || !view.has(pack)) continue;
       float h[VEC], g[VEC], o[VEC];
-      rh[i].decode(h);
-      rg[i].decode(g);
+      now.h[i].decode(h);
+      now.g[i].decode(g);
       if (p.weight_on) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
@@ -300,13 +348,16 @@ __global__ void __launch_bounds__(1024) rmsnorm_bwd_kernel(RmsParams p) {
       for (int k = 0; k < VEC; ++k) o[k] = rstd * (g[k] - h[k] * pull);
       if (p.dh_on) {
         float d[VEC];
-        rd[i].decode(d);
+        now.d[i].decode(d);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o[k] += d[k];
       }
       view.store(o, p.y, pack, p.rn != 0);
     }
+    if (PREFETCH) now = next;
+    else if (row0 + step < p.rows) fetch(now, row + step);
   }
+  pdl_trigger();
   if (!p.weight_on) return;
   // the CTA's groups are added in order, then one row of partials per CTA
   if constexpr (ALIGNED) {
@@ -327,25 +378,23 @@ __global__ void __launch_bounds__(1024) rmsnorm_bwd_kernel(RmsParams p) {
   }
 }
 
-// dweight[c] = sum over the CTAs' partials, in order: 32 columns per CTA, 8 warps share the list
+// dweight[c] = sum over the CTAs' partials, in order: 32 columns per CTA, 32 warps share the list
 template <typename T>
-__global__ void __launch_bounds__(256) rmsnorm_dweight_kernel(const float* __restrict__ partial, uint32_t n, uint32_t cols, typename Elem<T>::store_t* dweight, int rn) {
-  __shared__ float part[8][32];
+__global__ void __launch_bounds__(1024) rmsnorm_dweight_kernel(const float* partial, uint32_t n, uint32_t cols, typename Elem<T>::store_t* dweight, int rn) {
+  __shared__ float part[32][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t c = blockIdx.x * 32 + lane;
+  pdl_wait();
   float sum = 0.0f;
   if (c < cols) {
-#pragma unroll 16
-    for (uint32_t i = warp; i < n; i += 8) sum += partial[(uint64_t)i * cols + c];
+#pragma unroll 8
+    for (uint32_t i = warp; i < n; i += 32) sum += partial[(uint64_t)i * cols + c];
   }
   part[warp][lane] = sum;
   __syncthreads();
-  if (warp == 0 && c < cols) {
-    float v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) v += part[w][lane];
-    dweight[c] = round_store<T>(v, rn != 0);
-  }
+  const float v = warp_reduce(part[lane][warp], OpSum());        // warp w: column w
+  const uint32_t cw = blockIdx.x * 32 + warp;
+  if (lane == 0 && cw < cols) dweight[cw] = round_store<T>(v, rn != 0);
 }
 
 int log2_up(uint64_t v) {
@@ -375,8 +424,19 @@ template <typename T, int PACKS, bool ALIGNED>
 cudaError_t run_rms(const RmsParams& p, const RmsShape& s, bool quant, const LaunchCtx& lc) {
   const uint64_t per_cta = (uint64_t)(s.threads >> s.log_tpr);
   const unsigned grid = (unsigned)((p.rows + per_cta - 1) / per_cta);
-  if (quant) rmsnorm_kernel<T, PACKS, ALIGNED, true><<<grid, s.threads, per_cta * p.n_groups * 4, lc.stream>>>(p);
-  else rmsnorm_kernel<T, PACKS, ALIGNED, false><<<grid, s.threads, 0, lc.stream>>>(p);
+  constexpr uint32_t VEC = 16 / sizeof(typename Elem<T>::store_t);
+  const uint32_t width = p.group / VEC;
+  if (!quant) {
+    rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_NONE><<<grid, s.threads, 0, lc.stream>>>(p);
+    return cudaSuccess;
+  }
+  if constexpr (ALIGNED) {
+    if (p.group % VEC == 0 && (width & (width - 1)) == 0 && width <= 32 && (int)width <= 1 << s.log_tpr) {
+      rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_LANES><<<grid, s.threads, 0, lc.stream>>>(p);
+      return cudaSuccess;
+    }
+  }
+  rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_SHARED><<<grid, s.threads, per_cta * p.n_groups * 4, lc.stream>>>(p);
   return cudaSuccess;
 }
 
@@ -425,7 +485,7 @@ cudaError_t rms_backward(const RmsParams& p, const LaunchCtx& lc) {
   ZYXB_RMS_PACKS(ZYXB_RMS_BWD)
 #undef ZYXB_RMS_BWD
   if (e == cudaSuccess && p.weight_on)
-    rmsnorm_dweight_kernel<T><<<(p.cols + 31) / 32, 256, 0, lc.stream>>>(q.partial, grid, p.cols, (S*)q.dweight, q.rn);
+    e = launch_pdl(rmsnorm_dweight_kernel<T>, dim3((p.cols + 31) / 32), 1024, 0, lc.stream, (const float*)q.partial, grid, p.cols, (S*)q.dweight, q.rn);
   return e;
 }
 
