@@ -73,19 +73,21 @@ embedding_kernel(const ID* __restrict__ ids, const typename Elem<T>::store_t* __
 struct SortedToken { uint32_t row, token; };
 constexpr uint32_t FIRST = 1u << 31, SHARED = 1u << 30, TOKEN = (1u << 24) - 1;
 
-// four token numbers from position i on, -1 behind the last; i is a multiple of 4
-template <typename ID> __device__ __forceinline__ void load4(const ID* ids, uint32_t i, uint32_t n, int64_t (&v)[4]) {
+// four token numbers from position i on; -1 behind the last and for those that 32 bits do not hold; i is a multiple of 4
+template <typename ID> __device__ __forceinline__ void load4(const ID* ids, uint32_t i, uint32_t n, int (&v)[4]) {
   if (i + 4 <= n) {
     if constexpr (sizeof(ID) == 4) {
       const int4 q = *reinterpret_cast<const int4*>(ids + i);
       v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
     } else {
       const longlong2 a = *reinterpret_cast<const longlong2*>(ids + i), b = *reinterpret_cast<const longlong2*>(ids + i + 2);
-      v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+      const long long w[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = (uint64_t)w[j] <= 0x7fffffffull ? (int)w[j] : -1;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = i + j < n ? (int64_t)ids[i + j] : -1;
+    for (int j = 0; j < 4; ++j) v[j] = i + j < n && (sizeof(ID) == 4 || (uint64_t)ids[i + j] <= 0x7fffffffull) ? (int)ids[i + j] : -1;
   }
 }
 
@@ -106,16 +108,16 @@ embedding_index_kernel(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, u
   const uint32_t begin = min(n, warp * slice), end = min(n, begin + slice);
   uint32_t below = 0;
   for (uint32_t i0 = begin; i0 < end; i0 += STEP) {
-    int64_t v[IDX_BATCH][4];
+    int v[IDX_BATCH][4];
 #pragma unroll
     for (int q = 0; q < IDX_BATCH; ++q) load4(ids, i0 + q * 128 + lane * 4, end, v[q]);
 #pragma unroll
     for (int q = 0; q < IDX_BATCH; ++q)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint64_t r = (uint64_t)v[q][j] - lo;             // a negative number is far above any range
+        const uint32_t r = (uint32_t)v[q][j] - lo;             // a negative number is far above any range
         if (r < rows) atomicAdd(&mine[r], 1u);
-        else below += v[q][j] >= 0 && v[q][j] < (int64_t)lo;
+        else below += (uint32_t)v[q][j] < lo;
       }
   }
   below = warp_reduce(below, OpSum());
@@ -149,24 +151,24 @@ embedding_index_kernel(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, u
   __syncthreads();
   // second pass: equal rows of a warp's 32 lanes take consecutive places
   for (uint32_t i0 = begin; i0 < end; i0 += STEP) {
-    int64_t v[IDX_BATCH][4];
+    int v[IDX_BATCH][4];
 #pragma unroll
     for (int q = 0; q < IDX_BATCH; ++q) load4(ids, i0 + q * 128 + lane * 4, end, v[q]);
 #pragma unroll
     for (int q = 0; q < IDX_BATCH; ++q)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint64_t r = (uint64_t)v[q][j] - lo;
+        const uint32_t r = (uint32_t)v[q][j] - lo;
         const bool in = r < rows;
         const uint32_t active = __ballot_sync(0xffffffffu, in);
         if (active == 0) continue;
         if (in) {
-          const uint32_t same = __match_any_sync(active, (uint32_t)r), rank = __popc(same & ((1u << lane) - 1u));
+          const uint32_t same = __match_any_sync(active, r), rank = __popc(same & ((1u << lane) - 1u));
           const uint32_t place = mine[r];
           uint32_t token = i0 + q * 128 + lane * 4 + j;
           if (place + rank == first[r]) token |= FIRST;
           if (shared_run[r >> 5] >> (r & 31) & 1u) token |= SHARED;
-          sorted[place + rank] = SortedToken{lo + (uint32_t)r, token};
+          sorted[place + rank] = SortedToken{lo + r, token};
           __syncwarp(active);
           if (rank == 0) mine[r] = place + __popc(same);
         }
@@ -186,26 +188,26 @@ struct EmbGradParams {
   int accumulate, rn;
 };
 
+// scale * acc (+ what the row held) to the table
 template <typename T, int VEC>
-__device__ __forceinline__ void emb_store_row(typename Elem<T>::store_t* dst, float (&acc)[VEC], const EmbGradParams& p) {
-  RawVec<T, VEC> r;
+__device__ __forceinline__ void emb_store_row(typename Elem<T>::store_t* dst, float (&acc)[VEC], const RawVec<T, VEC>& held, const EmbGradParams& p) {
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] *= p.scale;
   if (p.accumulate) {
     float old[VEC];
-    r.load(dst);
-    r.decode(old);
+    held.decode(old);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] += old[k];
   }
+  RawVec<T, VEC> r;
   round_encode<T, VEC>(r, acc, p.rn != 0);
   r.store_stream(dst);
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(EMB_THREADS)
+__global__ void __launch_bounds__(EMB_THREADS, 4)
 embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typename Elem<T>::store_t* dtable, const EmbGradParams p, int log_tpt) {
-  constexpr int U = 8;
+  constexpr int U = 4;                    // rows in flight per thread; four CTAs per SM
   const uint32_t tpt = 1u << log_tpt, groups = EMB_THREADS >> log_tpt, group = threadIdx.x >> log_tpt;
   const uint32_t pack = blockIdx.y * tpt + (threadIdx.x & (tpt - 1));
   const uint64_t col = (uint64_t)pack * VEC;
@@ -234,13 +236,14 @@ embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typenam
   float acc[VEC];
   uint32_t row = 0, slot = (head.token & FIRST) || lo != begin ? 1 : 0;
   bool shared = false;
+  RawVec<T, VEC> held;                    // accumulate: the row as it was, loaded when its run begins
   auto flush = [&] {
     if (shared) {
       float* part = p.partial + ((uint64_t)c * 2 + slot) * p.dim + col;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) part[k] = acc[k];
     } else {
-      emb_store_row<T, VEC>(dtable + (uint64_t)row * p.ld_table + col, acc, p);
+      emb_store_row<T, VEC>(dtable + (uint64_t)row * p.ld_table + col, acc, held, p);
     }
     slot = 1;
   };
@@ -265,6 +268,7 @@ embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typenam
           if (i + u != lo) flush();
           row = s[u].row;
           shared = s[u].token & SHARED;
+          if (p.accumulate && !shared) held.load(dtable + (uint64_t)row * p.ld_table + col);
         }
 #pragma unroll
         for (int k = 0; k < VEC; ++k) acc[k] = starts_run ? v[k] : acc[k] + v[k];
@@ -302,23 +306,28 @@ embedding_combine_kernel(typename Elem<T>::store_t* dtable, const EmbGradParams 
     if (found[q][2] == 0) continue;                  // a shared run ends behind its first chunk
     const uint32_t row = found[q][0], c0 = found[q][1], count = found[q][2] - c0 + 1, per = (count + CMB_WARPS - 1) / CMB_WARPS;
     const uint32_t k0 = min(count, warp * per), k1 = min(count, k0 + per);
+    const uint32_t col0 = blockIdx.y * CMB_COLS + lane;
+    float sum[CMB_COLS / 32] = {};
+#pragma unroll 4
+    for (uint32_t k = k0; k < k1; ++k) {
+      const float* from = p.partial + ((uint64_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * p.dim + col0;
 #pragma unroll
-    for (int h = 0; h < CMB_COLS / 32; ++h) {
-      const uint32_t col = blockIdx.y * CMB_COLS + h * 32 + lane;
-      float sum = 0.0f;
-      if (col < p.dim) {
-#pragma unroll 8
-        for (uint32_t k = k0; k < k1; ++k) sum += p.partial[((uint64_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * p.dim + col];
-      }
-      part[warp][h * 32 + lane] = sum;
+      for (int h = 0; h < CMB_COLS / 32; ++h)
+        if (col0 + h * 32 < p.dim) sum[h] += from[h * 32];
     }
+#pragma unroll
+    for (int h = 0; h < CMB_COLS / 32; ++h) part[warp][h * 32 + lane] = sum[h];
     __syncthreads();
     const uint32_t col = blockIdx.y * CMB_COLS + threadIdx.x;
     if (threadIdx.x < CMB_COLS && col < p.dim) {
       float acc[1] = {0.0f};
 #pragma unroll
       for (int w = 0; w < CMB_WARPS; ++w) acc[0] += part[w][threadIdx.x];
-      emb_store_row<T, 1>(dtable + (uint64_t)row * p.ld_table + col, acc, p);
+      auto* dst = dtable + (uint64_t)row * p.ld_table + col;
+      RawVec<T, 1> held;
+      held.zero();
+      if (p.accumulate) held.load(dst);
+      emb_store_row<T, 1>(dst, acc, held, p);
     }
     __syncthreads();
   }

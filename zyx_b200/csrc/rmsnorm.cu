@@ -24,17 +24,24 @@ struct RmsParams {
   float *scales, *partial;
   uint64_t rows, ld;
   uint32_t cols, group, n_groups;
-  float eps;
+  float eps, inv_cols;
   int log_tpr, rn, residual_on, weight_on, dh_on;
 };
 
-// sum over the group's threads of up to two values; `parity` alternates between calls, so one barrier per call is enough
+// Sum over a row's threads of up to two values.  `parity` alternates between calls, so one barrier per call is enough.
 template <int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], int log_tpr, float (*buf)[32][N], int parity) {
-  const int width = min(32, 1 << log_tpr);
-  for (int o = width >> 1; o > 0; o >>= 1) {
+  if (log_tpr >= 5) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+  } else {
+    for (int o = (1 << log_tpr) >> 1; o > 0; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
   }
   if (log_tpr > 5) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wpr = 1 << (log_tpr - 5);
@@ -44,14 +51,16 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int log_tpr, float (*buf)
     }
     __syncthreads();
     const int first = warp & ~(wpr - 1);
+    float s[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = lane < wpr ? buf[parity][first + lane][i] : 0.0f;
-    for (int o = wpr >> 1; o > 0; o >>= 1) {
+    for (int i = 0; i < N; ++i) s[i] = 0.0f;
+#pragma unroll 4
+    for (int w = 0; w < wpr; ++w) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      for (int i = 0; i < N; ++i) s[i] += buf[parity][first + w][i];
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, v[i], 0);
+    for (int i = 0; i < N; ++i) v[i] = s[i];
   }
 }
 
@@ -80,29 +89,33 @@ struct RowView {
     for (int k = 0; k < VEC; ++k) v[k] = inside(col(pack) + k) ? Elem<T>::load(p[k]) : 0.0f;
     round_encode<T, VEC>(r, v, true);          // exact: the values are of the storage type
   }
-  __device__ __forceinline__ void store(const float (&v)[VEC], void* base, int pack, bool rn) const {
+  __device__ __forceinline__ void store(const typename Nums<VEC>::V (&n)[Nums<VEC>::N], void* base, int pack, bool rn) const {
     S* p = reinterpret_cast<S*>(base) + start + (uint64_t)pack * VEC;
     if (whole(pack)) {
       RawVec<T, VEC> r;
-      round_encode<T, VEC>(r, v, rn);
+      Nums<VEC>::encode(r, n, rn);
       r.store_stream(p);
       return;
     }
+    float v[VEC];
+    Nums<VEC>::floats(v, n);
 #pragma unroll
     for (int k = 0; k < VEC; ++k)
       if (inside(col(pack) + k)) p[k] = round_store<T>(v[k], rn);
   }
   // the weight's entries under a vector (the weight itself starts on a boundary, the row need not)
-  __device__ __forceinline__ void weight(float (&v)[VEC], const void* w, int pack) const {
+  __device__ __forceinline__ void weight(typename Nums<VEC>::V (&n)[Nums<VEC>::N], const void* w, int pack) const {
     const S* p = reinterpret_cast<const S*>(w);
+    RawVec<T, VEC> r;
     if constexpr (ALIGNED) {
-      RawVec<T, VEC> r;
       r.load(p + pack * VEC);
-      r.decode(v);
     } else {
+      float v[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) v[k] = inside(col(pack) + k) ? Elem<T>::load(p[col(pack) + k]) : 0.0f;
+      round_encode<T, VEC>(r, v, true);
     }
+    Nums<VEC>::decode(n, r);
   }
 };
 
@@ -114,7 +127,7 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 
 constexpr float E4M3_MAX = 448.0f, AMAX_FLOOR = 1e-30f;
 
-// a vector of y as 8-bit floats; scale_of(column)
+// a vector of y as 8-bit floats; scale_of(column): the reciprocal of its scale
 template <typename T, bool ALIGNED, class F>
 __device__ __forceinline__ void put_e4m3(const RowView<T, ALIGNED>& view, const float (&y)[RowView<T, ALIGNED>::VEC], const RmsParams& p, uint64_t row, int pack, F scale_of) {
   constexpr int VEC = RowView<T, ALIGNED>::VEC;
@@ -122,7 +135,7 @@ __device__ __forceinline__ void put_e4m3(const RowView<T, ALIGNED>& view, const 
   const int c0 = view.col(pack);
   float q[VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) q[k] = y[k] / scale_of(c0 + k);
+  for (int k = 0; k < VEC; ++k) q[k] = y[k] * scale_of(c0 + k);
   uint32_t w[VEC / 4];
 #pragma unroll
   for (int k = 0; k < VEC / 4; ++k) w[k] = e4m3x2(q[4 * k], q[4 * k + 1]) | (e4m3x2(q[4 * k + 2], q[4 * k + 3]) << 16);
@@ -144,18 +157,18 @@ enum { QUANT_NONE = 0, QUANT_LANES = 1, QUANT_SHARED = 2 };
 // the bits of |y| order like the values, and a NaN above all of them: it becomes its group's scale
 __device__ __forceinline__ uint32_t amax_bits_of(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-template <typename T, int PACKS, bool ALIGNED, int QUANT>
-__global__ void __launch_bounds__(1024) rmsnorm_kernel(RmsParams p) {
+template <typename T, int PACKS, bool ALIGNED, int QUANT, int THREADS>
+__global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsParams p) {
   using View = RowView<T, ALIGNED>;
   constexpr int VEC = View::VEC;
-  __shared__ float red[2][32][1];
-  extern __shared__ uint32_t amax_bits[];            // QUANT: largest |y| of each column group, per row of the CTA, as its bits
+  using Num = Nums<VEC>;
+  __shared__ float red[1][32][1];
+  extern __shared__ uint32_t amax_bits[];            // QUANT_SHARED: largest |y| of each column group, per row of the CTA, as its bits
   const int tpr = 1 << p.log_tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & (tpr - 1);
   const uint64_t row = (uint64_t)blockIdx.x * (blockDim.x >> p.log_tpr) + in_cta;
   const bool live = row < p.rows;
   const View view(live ? row : 0, p.ld, p.cols);
-  float h[PACKS][VEC];
-  float sum[1] = {0.0f};
+  typename Num::V v[PACKS][Num::N], sq = Num::splat(0.0f);
   {
     RawVec<T, VEC> rx[PACKS], rr[PACKS];
 #pragma unroll
@@ -170,38 +183,41 @@ __global__ void __launch_bounds__(1024) rmsnorm_kernel(RmsParams p) {
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int pack = t + i * tpr;
-      rx[i].decode(h[i]);
+      Num::decode(v[i], rx[i]);
       if (p.residual_on) {
-        float r[VEC];
-        rr[i].decode(r);
+        typename Num::V r[Num::N];
+        Num::decode(r, rr[i]);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) h[i][k] += r[k];
-        if (live && view.has(pack)) view.store(h[i], p.h, pack, p.rn != 0);
+        for (int k = 0; k < Num::N; ++k) v[i][k] = Num::add(v[i][k], r[k]);
+        if (live && view.has(pack)) view.store(v[i], p.h, pack, p.rn != 0);
       }
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) sum[0] += h[i][k] * h[i][k];
+      for (int k = 0; k < Num::N; ++k) sq = Num::fma(v[i][k], v[i][k], sq);
     }
   }
   if constexpr (QUANT == QUANT_SHARED) {
     for (uint32_t g = threadIdx.x; g < (blockDim.x >> p.log_tpr) * p.n_groups; g += blockDim.x) amax_bits[g] = __float_as_uint(AMAX_FLOOR);
     if (p.log_tpr <= 5) __syncthreads();             // wider rows pass a barrier in row_sum
   }
+  float sum[1] = {Num::sum(sq)};
   row_sum(sum, p.log_tpr, red, 0);
-  const float rstd = 1.0f / sqrtf(sum[0] / (float)p.cols + p.eps);
+  const float rstd = rsqrtf(sum[0] * p.inv_cols + p.eps);
+  float h[PACKS][VEC];
 #pragma unroll
   for (int i = 0; i < PACKS; ++i) {
     const int pack = t + i * tpr;
-    if (!live || !view.has(pack)) continue;
-    if (p.weight_on) {
-      float w[VEC];
+    const bool in = live && view.has(pack);
+    if (in && p.weight_on) {
+      typename Num::V w[Num::N];
       view.weight(w, p.weight, pack);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * rstd * w[k];
+      for (int k = 0; k < Num::N; ++k) v[i][k] = Num::mul(Num::mul(v[i][k], Num::splat(rstd)), w[k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) h[i][k] *= rstd;
+      for (int k = 0; k < Num::N; ++k) v[i][k] = Num::mul(v[i][k], Num::splat(rstd));
     }
-    if constexpr (QUANT == QUANT_NONE) view.store(h[i], p.y, pack, p.rn != 0);
+    if constexpr (QUANT == QUANT_NONE) { if (in) view.store(v[i], p.y, pack, p.rn != 0); }
+    else Num::floats(h[i], v[i]);
   }
   if constexpr (QUANT == QUANT_LANES) {
     const int width = (int)p.group / VEC;              // lanes per column group
@@ -216,8 +232,8 @@ __global__ void __launch_bounds__(1024) rmsnorm_kernel(RmsParams p) {
       }
       for (int o = width >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (!in) continue;
-      const float scale = __uint_as_float(m) / E4M3_MAX;
-      put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int) { return scale; });
+      const float scale = __uint_as_float(m) / E4M3_MAX, inv = 1.0f / scale;
+      put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int) { return inv; });
       if (pack % width == 0) p.scales[row * p.n_groups + pack / width] = scale;
     }
   }
@@ -257,119 +273,104 @@ __global__ void __launch_bounds__(1024) rmsnorm_kernel(RmsParams p) {
     for (int i = 0; i < PACKS; ++i) {
       const int pack = t + i * tpr;
       if (!live || !view.has(pack)) continue;
-      put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int c) { return __uint_as_float(mine[p.n_groups == 1 ? 0 : (uint32_t)min(max(c, 0), (int)p.cols - 1) / p.group]) / E4M3_MAX; });
+      put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int c) { return 1.0f / (__uint_as_float(mine[p.n_groups == 1 ? 0 : (uint32_t)min(max(c, 0), (int)p.cols - 1) / p.group]) / E4M3_MAX); });
     }
     if (live)
       for (uint32_t g = t; g < p.n_groups; g += tpr) p.scales[row * p.n_groups + g] = __uint_as_float(mine[g]) / E4M3_MAX;
   }
 }
 
-// Rows are dealt to the groups of a persistent grid, so that a thread keeps the weight gradient of its columns in registers (or,
-// where rows start at odd places and a column wanders between threads, in shared memory) until its last row.
-template <typename T, int PACKS, bool ALIGNED>
-__global__ void __launch_bounds__(1024) rmsnorm_bwd_kernel(RmsParams p) {
-  using View = RowView<T, ALIGNED>;
-  constexpr int VEC = View::VEC;
-  constexpr bool PREFETCH = PACKS * VEC <= 8;        // what 64 registers hold twice
+// Rows are dealt to the groups of a persistent grid, so that a thread keeps its columns' weights and their gradient in registers
+// from the first of its rows to the last.  Where rows do not start on vector boundaries a vector is one element (a column has to
+// stay with its thread); a warp's loads are then still one line each.
+template <typename T, int VEC, int PACKS, int THREADS>
+__global__ void __launch_bounds__(THREADS) rmsnorm_bwd_kernel(const RmsParams p) {
+  using S = typename Elem<T>::store_t;
+  using Num = Nums<VEC>;
+  using V = typename Num::V;
+  constexpr int N = Num::N;
   __shared__ float red[2][32][2];
   extern __shared__ float dw_shared[];               // [group of the CTA][cols]
   const int tpr = 1 << p.log_tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & (tpr - 1), groups = blockDim.x >> p.log_tpr;
-  float* dw_mine = dw_shared + (size_t)in_cta * p.cols;
-  float dw[PACKS][VEC];
+  auto col = [&](int i) { return (uint32_t)(t + i * tpr) * VEC; };
+  V w[PACKS][N], dw[PACKS][N];
 #pragma unroll
-  for (int i = 0; i < PACKS; ++i)
+  for (int i = 0; i < PACKS; ++i) {
+    RawVec<T, VEC> r;
+    if (p.weight_on && col(i) < p.cols) r.load((const S*)p.weight + col(i)); else r.zero();
+    Num::decode(w[i], r);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) dw[i][k] = 0.0f;
-  if (!ALIGNED && p.weight_on)
-    for (uint32_t c = t; c < p.cols; c += tpr) dw_mine[c] = 0.0f;
+    for (int k = 0; k < N; ++k) {
+      if (!p.weight_on) w[i][k] = Num::splat(1.0f);
+      dw[i][k] = Num::splat(0.0f);
+    }
+  }
   const uint64_t step = (uint64_t)gridDim.x * groups;
   struct Row { RawVec<T, VEC> h[PACKS], g[PACKS], d[PACKS]; };
   auto fetch = [&](Row& r, uint64_t row) {
-    const View view(row, p.ld, p.cols);
+    const uint64_t at = row * p.ld;
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-      const int pack = t + i * tpr;
       r.h[i].zero(); r.g[i].zero(); r.d[i].zero();
-      if (row < p.rows && view.has(pack)) {
-        view.load(r.h[i], p.h, pack);
-        view.load(r.g[i], p.dy, pack);
-        if (p.dh_on) view.load(r.d[i], p.dh, pack);
+      if (row < p.rows && col(i) < p.cols) {
+        r.h[i].load_stream((const S*)p.h + at + col(i));
+        r.g[i].load_stream((const S*)p.dy + at + col(i));
+        if (p.dh_on) r.d[i].load_stream((const S*)p.dh + at + col(i));
       }
     }
   };
   int parity = 0;
-  Row now, next;
+  Row now;
   fetch(now, (uint64_t)blockIdx.x * groups + in_cta);
   for (uint64_t row0 = (uint64_t)blockIdx.x * groups; row0 < p.rows; row0 += step, parity ^= 1) {
     const uint64_t row = row0 + in_cta;
-    const bool live = row < p.rows;
-    const View view(row, p.ld, p.cols);
-    if (PREFETCH) fetch(next, row + step);          // in flight during this row's sums
-    float s[2] = {0.0f, 0.0f};
+    V h[PACKS][N], g[PACKS][N], d[PACKS][N], hh = Num::splat(0.0f), gh = Num::splat(0.0f);
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-      const int pack = t + i * tpr;
-      float h[VEC], g[VEC];
-      now.h[i].decode(h);
-      now.g[i].decode(g);
-      if (p.weight_on && live && view.has(pack)) {
-        float w[VEC];
-        view.weight(w, p.weight, pack);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) g[k] *= w[k];
-      }
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) { s[0] += h[k] * h[k]; s[1] += g[k] * h[k]; }
+      Num::decode(h[i], now.h[i]);
+      Num::decode(g[i], now.g[i]);
+      Num::decode(d[i], now.d[i]);
     }
+    fetch(now, row + step);                          // in flight during this row's sums
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        hh = Num::fma(h[i][k], h[i][k], hh);
+        gh = Num::fma(Num::mul(g[i][k], w[i][k]), h[i][k], gh);
+      }
+    float s[2] = {Num::sum(hh), Num::sum(gh)};
     row_sum(s, p.log_tpr, red, parity);
-    const float rstd = 1.0f / sqrtf(s[0] / (float)p.cols + p.eps);
-    const float pull = rstd * rstd * (s[1] / (float)p.cols);          // dx = rstd * (dy w - h * pull)
-    if (!ALIGNED) __syncwarp();
+    if (row >= p.rows) continue;                     // this group's last round; the others' barriers are behind it
+    const float rstd = rsqrtf(s[0] * p.inv_cols + p.eps);
+    // dx = rstd * (dy w) - h * (rstd^3 * mean(dy w h)) + dh;  dw += dy * h * rstd
+    const V up = Num::splat(rstd), down = Num::splat(-(rstd * rstd * rstd) * (s[1] * p.inv_cols));
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-      const int pack = t + i * tpr;
-      if (!live || !view.has(pack)) continue;
-      float h[VEC], g[VEC], o[VEC];
-      now.h[i].decode(h);
-      now.g[i].decode(g);
-      if (p.weight_on) {
+      if (col(i) >= p.cols) continue;
+      V o[N];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const float d = g[k] * (h[k] * rstd);
-          if constexpr (ALIGNED) dw[i][k] += d;
-          else if (view.inside(view.col(pack) + k)) dw_mine[view.col(pack) + k] += d;
-        }
-        float w[VEC];
-        view.weight(w, p.weight, pack);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) g[k] *= w[k];
+      for (int k = 0; k < N; ++k) {
+        const V gu = Num::mul(g[i][k], up);
+        dw[i][k] = Num::fma(gu, h[i][k], dw[i][k]);
+        o[k] = Num::add(Num::fma(gu, w[i][k], Num::mul(h[i][k], down)), d[i][k]);
       }
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) o[k] = rstd * (g[k] - h[k] * pull);
-      if (p.dh_on) {
-        float d[VEC];
-        now.d[i].decode(d);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) o[k] += d[k];
-      }
-      view.store(o, p.y, pack, p.rn != 0);
+      RawVec<T, VEC> r;
+      Num::encode(r, o, p.rn != 0);
+      r.store_stream((S*)p.y + row * p.ld + col(i));
     }
-    if (PREFETCH) now = next;
-    else if (row0 + step < p.rows) fetch(now, row + step);
   }
   pdl_trigger();
   if (!p.weight_on) return;
   // the CTA's groups are added in order, then one row of partials per CTA
-  if constexpr (ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < PACKS; ++i) {
-      const int pack = t + i * tpr;
-      if ((uint32_t)pack * VEC < p.cols) {
+  for (int i = 0; i < PACKS; ++i)
+    if (col(i) < p.cols) {
+      float f[VEC];
+      Num::floats(f, dw[i]);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) dw_mine[pack * VEC + k] = dw[i][k];
-      }
+      for (int k = 0; k < VEC; ++k) dw_shared[(size_t)in_cta * p.cols + col(i) + k] = f[k];
     }
-  }
   __syncthreads();
   for (uint32_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
     float sum = 0.0f;
@@ -405,14 +406,13 @@ int log2_up(uint64_t v) {
 
 struct RmsShape { bool aligned; int log_tpr, packs, threads; };
 
-// vectors that cover a row, one per thread up to `most` threads; a row's group is at least 8 threads wide
-template <typename T>
-RmsShape rms_shape(const RmsParams& p, int most_log) {
-  constexpr int VEC = 16 / (int)sizeof(typename Elem<T>::store_t);
+// Threads per row and vectors per thread.  A thread's fixed work (addresses, the row's sum) is worth about a vector's, so rows are
+// held by few threads with four vectors each (two for f32: as many bytes in registers) - unless there are too few rows to fill the
+// SMs that way, where a row is spread as wide as it goes.
+RmsShape rms_shape(uint64_t rows, uint64_t vectors, int packs_wanted, int sm_count) {
   RmsShape s{};
-  s.aligned = p.cols % VEC == 0 && p.ld % VEC == 0;
-  const uint64_t vectors = s.aligned ? p.cols / VEC : (p.cols + 2 * VEC - 2) / VEC;
-  s.log_tpr = std::min(most_log, std::max(3, log2_up(vectors)));
+  int packs = rows * vectors < (uint64_t)sm_count * 2048 ? 1 : packs_wanted;
+  s.log_tpr = std::min(10, std::max(3, log2_up((vectors + packs - 1) / packs)));
   const int need = (int)((vectors + (1u << s.log_tpr) - 1) >> s.log_tpr);
   s.packs = 1;
   while (s.packs < need) s.packs *= 2;
@@ -420,70 +420,92 @@ RmsShape rms_shape(const RmsParams& p, int most_log) {
   return s;
 }
 
-template <typename T, int PACKS, bool ALIGNED>
+template <typename T, int PACKS, bool ALIGNED, int THREADS>
 cudaError_t run_rms(const RmsParams& p, const RmsShape& s, bool quant, const LaunchCtx& lc) {
   const uint64_t per_cta = (uint64_t)(s.threads >> s.log_tpr);
   const unsigned grid = (unsigned)((p.rows + per_cta - 1) / per_cta);
   constexpr uint32_t VEC = 16 / sizeof(typename Elem<T>::store_t);
   const uint32_t width = p.group / VEC;
   if (!quant) {
-    rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_NONE><<<grid, s.threads, 0, lc.stream>>>(p);
+    rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_NONE, THREADS><<<grid, s.threads, 0, lc.stream>>>(p);
     return cudaSuccess;
   }
   if constexpr (ALIGNED) {
     if (p.group % VEC == 0 && (width & (width - 1)) == 0 && width <= 32 && (int)width <= 1 << s.log_tpr) {
-      rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_LANES><<<grid, s.threads, 0, lc.stream>>>(p);
+      rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_LANES, THREADS><<<grid, s.threads, 0, lc.stream>>>(p);
       return cudaSuccess;
     }
   }
-  rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_SHARED><<<grid, s.threads, per_cta * p.n_groups * 4, lc.stream>>>(p);
+  rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_SHARED, THREADS><<<grid, s.threads, per_cta * p.n_groups * 4, lc.stream>>>(p);
   return cudaSuccess;
 }
 
-template <typename T, int PACKS, bool ALIGNED>
-cudaError_t run_rms_bwd(RmsParams& p, const RmsShape& s, unsigned* grid_out, const LaunchCtx& lc) {
-  const int groups = s.threads >> s.log_tpr;
-  const size_t smem = p.weight_on ? (size_t)groups * p.cols * 4 : 0;
-  static uint64_t configured = 0;
-  cudaError_t e = ensure_dynamic_smem(rmsnorm_bwd_kernel<T, PACKS, ALIGNED>, 80 << 10, &configured);
-  if (e != cudaSuccess) return e;
-  const uint64_t work = (p.rows + groups - 1) / groups;
-  *grid_out = (unsigned)std::min<uint64_t>(work, (uint64_t)lc.sm_count * std::max(1, 2048 / s.threads / 2));
-  rmsnorm_bwd_kernel<T, PACKS, ALIGNED><<<*grid_out, s.threads, smem, lc.stream>>>(p);
-  return cudaSuccess;
+template <typename T, bool ALIGNED>
+cudaError_t run_rms_packs(const RmsParams& p, const RmsShape& s, bool quant, const LaunchCtx& lc) {
+  if (s.threads == 256) {
+    if (s.packs == 1) return run_rms<T, 1, ALIGNED, 256>(p, s, quant, lc);
+    if (s.packs == 2) return run_rms<T, 2, ALIGNED, 256>(p, s, quant, lc);
+    return run_rms<T, 4, ALIGNED, 256>(p, s, quant, lc);
+  }
+  if (s.packs == 1) return run_rms<T, 1, ALIGNED, 1024>(p, s, quant, lc);
+  if (s.packs == 2) return run_rms<T, 2, ALIGNED, 1024>(p, s, quant, lc);
+  if constexpr (sizeof(T) == 4 && !ALIGNED) { if (s.packs == 8) return run_rms<T, 8, ALIGNED, 1024>(p, s, quant, lc); }     // 4097 vectors
+  return run_rms<T, 4, ALIGNED, 1024>(p, s, quant, lc);
 }
-
-// 16384 columns are 1024 threads x 2 vectors of 16-bit elements or x 4 of f32; rows off the boundary can need one vector more
-#define ZYXB_RMS_PACKS(CALL)                                                                       \
-  constexpr bool wide = sizeof(T) == 4;                                                            \
-  if (s.packs == 1) e = s.aligned ? CALL(1, true) : CALL(1, false);                                \
-  else if (s.packs == 2) e = s.aligned ? CALL(2, true) : CALL(2, false);                           \
-  else if (s.packs == 4 && !s.aligned) e = CALL(4, false);                                         \
-  else if constexpr (wide) { if (s.packs == 4) e = CALL(4, true); else e = CALL(8, false); }
 
 template <typename T>
 cudaError_t rms_forward(const RmsParams& p, bool quant, const LaunchCtx& lc) {
+  constexpr uint32_t VEC = 16 / sizeof(typename Elem<T>::store_t);
   RmsParams q = p;
-  const RmsShape s = rms_shape<T>(p, 10);
+  const bool aligned = p.cols % VEC == 0 && p.ld % VEC == 0;
+  const RmsShape s = rms_shape(p.rows, aligned ? p.cols / VEC : (p.cols + 2 * VEC - 2) / VEC, 4, lc.sm_count);
   q.log_tpr = s.log_tpr;
-  cudaError_t e = cudaSuccess;
-#define ZYXB_RMS_FWD(P, A) (run_rms<T, P, A>(q, s, quant, lc))
-  ZYXB_RMS_PACKS(ZYXB_RMS_FWD)
-#undef ZYXB_RMS_FWD
-  return e;
+  return aligned ? run_rms_packs<T, true>(q, s, quant, lc) : run_rms_packs<T, false>(q, s, quant, lc);
+}
+
+template <typename T, int VEC, int PACKS, int THREADS>
+cudaError_t run_rms_bwd(const RmsParams& p, const RmsShape& s, unsigned* grid_out, const LaunchCtx& lc) {
+  const int groups = s.threads >> s.log_tpr;
+  const size_t smem = p.weight_on ? (size_t)groups * p.cols * 4 : 0;
+  auto kern = rmsnorm_bwd_kernel<T, VEC, PACKS, THREADS>;
+  static uint64_t configured = 0;
+  cudaError_t e = ensure_dynamic_smem(kern, 80 << 10, &configured);
+  if (e != cudaSuccess) return e;
+  int per_sm = 1;
+  if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads, smem)) != cudaSuccess) return e;
+  const uint64_t work = (p.rows + groups - 1) / groups;
+  *grid_out = (unsigned)std::min<uint64_t>(work, (uint64_t)lc.sm_count * std::max(1, per_sm));
+  kern<<<*grid_out, s.threads, smem, lc.stream>>>(p);
+  return cudaSuccess;
+}
+
+template <typename T, int VEC>
+cudaError_t run_rms_bwd_packs(const RmsParams& p, const RmsShape& s, unsigned* grid, const LaunchCtx& lc) {
+  if (s.threads == 256) {
+    if (s.packs == 1) return run_rms_bwd<T, VEC, 1, 256>(p, s, grid, lc);
+    if (s.packs == 2) return run_rms_bwd<T, VEC, 2, 256>(p, s, grid, lc);
+    if constexpr (VEC == 1) return s.packs == 4 ? run_rms_bwd<T, VEC, 4, 256>(p, s, grid, lc) : run_rms_bwd<T, VEC, 8, 256>(p, s, grid, lc);
+    else return run_rms_bwd<T, VEC, 4, 256>(p, s, grid, lc);
+  }
+  if constexpr (VEC > 1) { if (s.threads == 512 && s.packs <= 2) return run_rms_bwd<T, VEC, 2, 512>(p, s, grid, lc); }
+  if (s.packs <= 2) return run_rms_bwd<T, VEC, 2, 1024>(p, s, grid, lc);
+  if constexpr (VEC == 1) {
+    if (s.packs == 8) return run_rms_bwd<T, VEC, 8, 1024>(p, s, grid, lc);
+    if (s.packs == 16) return run_rms_bwd<T, VEC, 16, 1024>(p, s, grid, lc);
+  }
+  return run_rms_bwd<T, VEC, 4, 1024>(p, s, grid, lc);
 }
 
 template <typename T>
 cudaError_t rms_backward(const RmsParams& p, const LaunchCtx& lc) {
   using S = typename Elem<T>::store_t;
+  constexpr uint32_t VEC = 16 / sizeof(S);
   RmsParams q = p;
-  const RmsShape s = rms_shape<T>(p, 10);
+  const bool aligned = p.cols % VEC == 0 && p.ld % VEC == 0;
+  const RmsShape s = rms_shape(p.rows, aligned ? p.cols / VEC : p.cols, aligned ? 2 : 8, lc.sm_count);
   q.log_tpr = s.log_tpr;
   unsigned grid = 0;
-  cudaError_t e = cudaSuccess;
-#define ZYXB_RMS_BWD(P, A) (run_rms_bwd<T, P, A>(q, s, &grid, lc))
-  ZYXB_RMS_PACKS(ZYXB_RMS_BWD)
-#undef ZYXB_RMS_BWD
+  cudaError_t e = aligned ? run_rms_bwd_packs<T, (int)VEC>(q, s, &grid, lc) : run_rms_bwd_packs<T, 1>(q, s, &grid, lc);
   if (e == cudaSuccess && p.weight_on)
     e = launch_pdl(rmsnorm_dweight_kernel<T>, dim3((p.cols + 31) / 32), 1024, 0, lc.stream, (const float*)q.partial, grid, p.cols, (S*)q.dweight, q.rn);
   return e;
@@ -515,7 +537,7 @@ int launch_rmsnorm(const zyxb_rmsnorm_desc& d, void* const* args, const uint64_t
   ZYXB_CHECK_ARG(n_args == want, "rmsnorm: expected args x [,residual] [,weight] -> [h,] y [,scales]");
   const uint64_t es = dtype_size(d.dtype);
   RmsParams p{};
-  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.eps = d.eps; p.rn = lc.round_nearest ? 1 : 0;
+  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.eps = d.eps; p.inv_cols = 1.0f / (float)d.cols; p.rn = lc.round_nearest ? 1 : 0;
   p.residual_on = d.has_residual ? 1 : 0; p.weight_on = d.has_weight ? 1 : 0;
   p.group = d.group ? std::min<uint32_t>(d.group, p.cols) : p.cols;
   p.n_groups = (p.cols + p.group - 1) / p.group;
@@ -549,7 +571,7 @@ int launch_rmsnorm_bwd(const zyxb_rmsnorm_desc& d, void* const* args, const uint
   ZYXB_CHECK_ARG(n_args == want, "rmsnorm backward: expected args h, dy [,weight] [,dh] -> dx [,dweight]");
   const uint64_t es = dtype_size(d.dtype);
   RmsParams p{};
-  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.eps = d.eps; p.rn = lc.round_nearest ? 1 : 0;
+  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.eps = d.eps; p.inv_cols = 1.0f / (float)d.cols; p.rn = lc.round_nearest ? 1 : 0;
   p.weight_on = d.has_weight ? 1 : 0; p.dh_on = d.has_dh ? 1 : 0;
   int i = 0;
   ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm backward: h too small"); p.h = args[i++];
