@@ -22,7 +22,9 @@ class BackendError(RuntimeError):
 
 
 def _evs(events):
-    events = [e for e in (events or []) if e is not None and e.id != 0]
+    if not events:
+        return None, 0
+    events = [e for e in events if e is not None and e.id != 0]
     if not events:
         return None, 0
     arr = (L.Event * len(events))(*events)

@@ -28,7 +28,7 @@ constexpr int IDX_THREADS = 1024, IDX_WARPS = IDX_THREADS / 32;
 constexpr int IDX_MAX_ROWS = 1024;     // rows of a vocabulary range, one per thread (histograms: 32 warps x 1024 x 4 B of shared memory)
 constexpr int IDX_BATCH = 4;           // loads of four token numbers in flight per lane
 constexpr int CMB_WARPS = 8, CMB_COLS = 128;
-constexpr uint32_t CHUNK = 32;         // places of the sorted order per group; runs of more than two chunks are shared
+constexpr uint32_t CHUNK = 32, CHUNK_LEAST = 8;      // places of the sorted order per group; runs of more than two chunks are shared
 constexpr int FILL_ROWS = 64;          // table rows that a CTA of the sum launch looks through for absent ones
 
 template <typename ID> __device__ __forceinline__ int64_t id_at(const ID* ids, uint64_t i) { return (int64_t)ids[i]; }
@@ -39,6 +39,8 @@ embedding_kernel(const ID* __restrict__ ids, const typename Elem<T>::store_t* __
                  uint32_t tokens, uint64_t vocab, uint32_t packs, int log_tpt, uint64_t ld_table, uint64_t ld_out, float scale, int rn) {
   const uint32_t tpt = 1u << log_tpt, group = threadIdx.x >> log_tpt, groups = EMB_THREADS >> log_tpt;
   const uint32_t pack = blockIdx.y * tpt + (threadIdx.x & (tpt - 1));
+  pdl_trigger();
+  pdl_wait();
   if (pack >= packs) return;
   const uint64_t first = (uint64_t)blockIdx.x * groups * EMB_TOKENS + group;
   int64_t id[EMB_TOKENS];
@@ -101,6 +103,7 @@ embedding_index_kernel(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, u
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* mine = hist + warp * range;
   for (uint32_t i = threadIdx.x; i < IDX_WARPS * range; i += IDX_THREADS) hist[i] = 0;
+  pdl_wait();
   __syncthreads();
   // each warp owns one slice of the tokens, in both passes
   constexpr uint32_t STEP = 128 * IDX_BATCH;
@@ -207,7 +210,7 @@ __device__ __forceinline__ void emb_store_row(typename Elem<T>::store_t* dst, fl
 template <typename T, int VEC>
 __global__ void __launch_bounds__(EMB_THREADS, 4)
 embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typename Elem<T>::store_t* dtable, const EmbGradParams p, int log_tpt) {
-  constexpr int U = 4;                    // rows in flight per thread; four CTAs per SM
+  constexpr int U = VEC >= 4 ? 4 : 8;     // rows in flight per thread; four CTAs per SM
   const uint32_t tpt = 1u << log_tpt, groups = EMB_THREADS >> log_tpt, group = threadIdx.x >> log_tpt;
   const uint32_t pack = blockIdx.y * tpt + (threadIdx.x & (tpt - 1));
   const uint64_t col = (uint64_t)pack * VEC;
@@ -353,14 +356,14 @@ bool matrix_fits(uint64_t rows, uint64_t ld, uint64_t dim, uint64_t es, uint64_t
 }
 
 template <typename T, typename ID, int VEC>
-void run_embedding(const zyxb_embedding_desc& d, uint64_t ldt, uint64_t ldo, float scale, void* const* args, const LaunchCtx& lc) {
+cudaError_t run_embedding(const zyxb_embedding_desc& d, uint64_t ldt, uint64_t ldo, float scale, void* const* args, const LaunchCtx& lc) {
   using S = typename Elem<T>::store_t;
   const uint32_t packs = (uint32_t)(d.dim / VEC);
   const int log_tpt = log2_ceil(packs, 8);
   const uint64_t per_cta = (uint64_t)(EMB_THREADS >> log_tpt) * EMB_TOKENS;
   const dim3 grid((unsigned)((d.tokens + per_cta - 1) / per_cta), (unsigned)((packs + (1u << log_tpt) - 1) >> log_tpt));
-  embedding_kernel<T, ID, VEC><<<grid, EMB_THREADS, 0, lc.stream>>>((const ID*)args[0], (const S*)args[1], (S*)args[2], (uint32_t)d.tokens,
-                                                                   d.vocab, packs, log_tpt, ldt, ldo, scale, lc.round_nearest ? 1 : 0);
+  return launch_pdl(embedding_kernel<T, ID, VEC>, grid, EMB_THREADS, 0, lc.stream, (const ID*)args[0], (const S*)args[1], (S*)args[2], (uint32_t)d.tokens,
+                    d.vocab, packs, log_tpt, ldt, ldo, scale, lc.round_nearest ? 1 : 0);
 }
 
 struct EmbPlan { uint32_t range, ranges, chunk, chunks; uint64_t starts_off, partial_off; };
@@ -377,8 +380,9 @@ cudaError_t run_embedding_bwd(const zyxb_embedding_desc& d, uint64_t ldt, uint64
   static uint64_t configured = 0;
   cudaError_t e = ensure_dynamic_smem(embedding_index_kernel<ID>, IDX_WARPS * IDX_MAX_ROWS * 4, &configured);
   if (e != cudaSuccess) return e;
-  embedding_index_kernel<ID><<<pl.ranges, IDX_THREADS, IDX_WARPS * pl.range * 4, lc.stream>>>((const ID*)args[0], (uint32_t)d.tokens, (uint32_t)d.vocab, pl.range, 2 * pl.chunk,
-                                                                                            (SortedToken*)scratch, (uint32_t*)(scratch + pl.starts_off));
+  e = launch_pdl(embedding_index_kernel<ID>, dim3(pl.ranges), IDX_THREADS, IDX_WARPS * pl.range * 4, lc.stream, (const ID*)args[0], (uint32_t)d.tokens,
+                 (uint32_t)d.vocab, pl.range, 2 * pl.chunk, (SortedToken*)scratch, (uint32_t*)(scratch + pl.starts_off));
+  if (e != cudaSuccess) return e;
   const int log_tpt = log2_ceil(p.packs, 8);
   const uint32_t groups = EMB_THREADS >> log_tpt;
   p.sum_ctas = (pl.chunks + groups - 1) / groups;
@@ -431,9 +435,11 @@ int launch_embedding(const zyxb_embedding_desc& d, void* const* args, const uint
   ZYXB_CHECK_ARG(args[2] != args[1] && args[2] != args[0], "embedding: out must be a buffer of its own");
   const float scale = d.scale == 0.0f ? 1.0f : d.scale;
   const uint32_t vec = emb_vec(d, ldt, ldo);
-#define ZYXB_EMB_FWD(T, ID, V) run_embedding<T, ID, V>(d, ldt, ldo, scale, args, lc)
+  cudaError_t e = cudaSuccess;
+#define ZYXB_EMB_FWD(T, ID, V) e = run_embedding<T, ID, V>(d, ldt, ldo, scale, args, lc)
   ZYXB_EMB_DISPATCH(ZYXB_EMB_FWD)
 #undef ZYXB_EMB_FWD
+  if (e != cudaSuccess) { err = std::string("embedding: ") + cudaGetErrorString(e); return ZYXB_ERR_KERNEL_LAUNCH; }
   return check_launch(lc, err, "embedding");
 }
 
@@ -450,13 +456,17 @@ int launch_embedding_bwd(const zyxb_embedding_desc& d, void* const* args, const 
   pl.ranges = (uint32_t)((d.vocab + pl.range - 1) / pl.range);
   pl.starts_off = (d.tokens * sizeof(SortedToken) + 255) / 256 * 256;
   pl.partial_off = pl.starts_off + ((d.vocab + 1) * 4 + 255) / 256 * 256;
+  // few tokens: shorter chunks, so that every SM has three CTAs' worth of them (4099 tokens of 777 f32: 24 -> 22 us; at 16384 of 2048
+  // bf16, which 32 places fill, chunks of 8 cost more partials than they save: 61 -> 68 us)
+  const uint32_t vec = emb_vec(d, ldt, ldo);
+  const uint64_t threads_wide = (d.dim / vec + 31) / 32 * 32;
   pl.chunk = CHUNK;
   auto chunks = [&] { return (d.tokens + pl.chunk - 1) / pl.chunk; };
+  while (pl.chunk > CHUNK_LEAST && chunks() * threads_wide < (uint64_t)lc.sm_count * 3 * EMB_THREADS) pl.chunk /= 2;
   while (chunks() > 1 && pl.partial_off + chunks() * 2 * d.dim * 4 > lc.scratch_bytes) pl.chunk *= 2;     // partials have to fit the scratch
   pl.chunks = (uint32_t)chunks();
   ZYXB_CHECK_ARG(pl.partial_off + (uint64_t)pl.chunks * 2 * d.dim * 4 <= lc.scratch_bytes, "embedding gradient: too large for the scratch memory");
   const float scale = d.scale == 0.0f ? 1.0f : d.scale;
-  const uint32_t vec = emb_vec(d, ldt, ldo);
   cudaError_t e = cudaSuccess;
 #define ZYXB_EMB_BWD(T, ID, V) e = run_embedding_bwd<T, ID, V>(d, ldt, ldo, scale, pl, args, lc)
   ZYXB_EMB_DISPATCH(ZYXB_EMB_BWD)

@@ -37,6 +37,7 @@ __global__ void __launch_bounds__(MUON_THREADS) muon_momentum_kernel(const __gri
   constexpr int VEC = 16 / (int)sizeof(S);
   __shared__ double part[MUON_THREADS / 32];
   pdl_trigger();
+  pdl_wait();
   const MuonMatrix& m = k.m[blockIdx.y];
   const uint64_t n = (uint64_t)k.lo * k.hi, vectors = n / VEC;
   const S* g = (const S*)m.g;
@@ -215,6 +216,7 @@ __global__ void __launch_bounds__(MUON_THREADS) muon_step_kernel(const __grid_co
   const uint16_t* in = x.ptr + blockIdx.z * x.part() * PARTS;
   const float step = (m.tall ? step_tall : step_flat) * muon::UNSCALE;
   S* p = (S*)m.p;
+  pdl_trigger();
   pdl_wait();
   auto get = [&](float (&v)[8], uint32_t y, uint32_t q) {
 #pragma unroll
@@ -347,8 +349,8 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
 
   const unsigned sums = (unsigned)std::min<uint64_t>(MUON_PARTIALS, ((uint64_t)lo * hi + MUON_THREADS * 16 - 1) / (MUON_THREADS * 16));
   const dim3 tiles((hi + TILE - 1) / TILE, (lo + TILE - 1) / TILE, batch);
-  muon_momentum_kernel<T><<<dim3(sums, batch), MUON_THREADS, 0, lc.stream>>>(k, partial);
-  cudaError_t e = launch_pdl(muon_normalize_kernel<T, PARTS>, tiles, MUON_THREADS, 0, lc.stream, k, partial, (int)sums, d.eps == 0.0f ? 1e-7f : d.eps, x[0]);
+  cudaError_t e = launch_pdl(muon_momentum_kernel<T>, dim3(sums, batch), MUON_THREADS, 0, lc.stream, k, partial);
+  if (e == cudaSuccess) e = launch_pdl(muon_normalize_kernel<T, PARTS>, tiles, MUON_THREADS, 0, lc.stream, k, partial, (int)sums, d.eps == 0.0f ? 1e-7f : d.eps, x[0]);
 
   const int bn_sym = muon::tile_width<PARTS, true>(lo, lo, batch, lc.sm_count), bn_apply = muon::tile_width<PARTS, false>(lo, hi, batch, lc.sm_count);
   CUtensorMap x_rows[2], x_cols[2], x_k[2], gram_rows, gram_cols, poly_rows;

@@ -154,7 +154,14 @@ __device__ __forceinline__ void put_e4m3(const RowView<T, ALIGNED>& view, const 
 // memory, one per warp where a row is one group).
 enum { QUANT_NONE = 0, QUANT_LANES = 1, QUANT_SHARED = 2 };
 
-// the bits of |y| order like the values, and a NaN above all of them: it becomes its group's scale
+// largest of m and |v|; a NaN stays, and becomes its group's scale
+__device__ __forceinline__ float max_abs(float m, float a, float b) {
+  float r;
+  asm("{\n\t.reg .f32 x, y;\n\tabs.f32 x, %1;\n\tabs.f32 y, %2;\n\tmax.NaN.f32 %0, x, y, %3;\n\t}" : "=f"(r) : "f"(a), "f"(b), "f"(m));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+// the bits of |y| order like the values, and a NaN's above all of them
 __device__ __forceinline__ uint32_t amax_bits_of(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 template <typename T, int PACKS, bool ALIGNED, int QUANT, int THREADS>
@@ -168,6 +175,8 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsParams p) {
   const uint64_t row = (uint64_t)blockIdx.x * (blockDim.x >> p.log_tpr) + in_cta;
   const bool live = row < p.rows;
   const View view(live ? row : 0, p.ld, p.cols);
+  pdl_trigger();
+  pdl_wait();
   typename Num::V v[PACKS][Num::N], sq = Num::splat(0.0f);
   {
     RawVec<T, VEC> rx[PACKS], rr[PACKS];
@@ -225,14 +234,14 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsParams p) {
     for (int i = 0; i < PACKS; ++i) {
       const int pack = t + i * tpr;
       const bool in = live && view.has(pack);
-      uint32_t m = __float_as_uint(AMAX_FLOOR);
+      float m = AMAX_FLOOR;
       if (in) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) m = max(m, amax_bits_of(h[i][k]));
+        for (int k = 0; k < VEC; k += 2) m = max_abs(m, h[i][k], h[i][k + 1]);
       }
-      for (int o = width >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int o = width >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (!in) continue;
-      const float scale = __uint_as_float(m) / E4M3_MAX, inv = 1.0f / scale;
+      const float scale = m / E4M3_MAX, inv = 1.0f / scale;
       put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int) { return inv; });
       if (pack % width == 0) p.scales[row * p.n_groups + pack / width] = scale;
     }
@@ -294,6 +303,8 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_bwd_kernel(const RmsParams p)
   const int tpr = 1 << p.log_tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & (tpr - 1), groups = blockDim.x >> p.log_tpr;
   auto col = [&](int i) { return (uint32_t)(t + i * tpr) * VEC; };
   V w[PACKS][N], dw[PACKS][N];
+  pdl_trigger();
+  pdl_wait();
 #pragma unroll
   for (int i = 0; i < PACKS; ++i) {
     RawVec<T, VEC> r;
@@ -360,7 +371,6 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_bwd_kernel(const RmsParams p)
       r.store_stream((S*)p.y + row * p.ld + col(i));
     }
   }
-  pdl_trigger();
   if (!p.weight_on) return;
   // the CTA's groups are added in order, then one row of partials per CTA
 #pragma unroll
@@ -427,17 +437,14 @@ cudaError_t run_rms(const RmsParams& p, const RmsShape& s, bool quant, const Lau
   constexpr uint32_t VEC = 16 / sizeof(typename Elem<T>::store_t);
   const uint32_t width = p.group / VEC;
   if (!quant) {
-    rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_NONE, THREADS><<<grid, s.threads, 0, lc.stream>>>(p);
-    return cudaSuccess;
+    return launch_pdl(rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_NONE, THREADS>, dim3(grid), s.threads, 0, lc.stream, p);
   }
   if constexpr (ALIGNED) {
     if (p.group % VEC == 0 && (width & (width - 1)) == 0 && width <= 32 && (int)width <= 1 << s.log_tpr) {
-      rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_LANES, THREADS><<<grid, s.threads, 0, lc.stream>>>(p);
-      return cudaSuccess;
+      return launch_pdl(rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_LANES, THREADS>, dim3(grid), s.threads, 0, lc.stream, p);
     }
   }
-  rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_SHARED, THREADS><<<grid, s.threads, per_cta * p.n_groups * 4, lc.stream>>>(p);
-  return cudaSuccess;
+  return launch_pdl(rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_SHARED, THREADS>, dim3(grid), s.threads, per_cta * p.n_groups * 4, lc.stream, p);
 }
 
 template <typename T, bool ALIGNED>
@@ -475,25 +482,27 @@ cudaError_t run_rms_bwd(const RmsParams& p, const RmsShape& s, unsigned* grid_ou
   if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads, smem)) != cudaSuccess) return e;
   const uint64_t work = (p.rows + groups - 1) / groups;
   *grid_out = (unsigned)std::min<uint64_t>(work, (uint64_t)lc.sm_count * std::max(1, per_sm));
-  kern<<<*grid_out, s.threads, smem, lc.stream>>>(p);
-  return cudaSuccess;
+  return launch_pdl(kern, dim3(*grid_out), s.threads, smem, lc.stream, p);
 }
 
+// The adjoint's groups: a column's weight, its gradient, this row's h, dy, dh and the next row's all stay in registers, so a thread
+// takes two vectors (up to twelve single elements where rows are off the boundaries; 512 threads of 128 registers hold 6144 columns
+// that way) and the group grows to 1024 threads.
 template <typename T, int VEC>
 cudaError_t run_rms_bwd_packs(const RmsParams& p, const RmsShape& s, unsigned* grid, const LaunchCtx& lc) {
-  if (s.threads == 256) {
-    if (s.packs == 1) return run_rms_bwd<T, VEC, 1, 256>(p, s, grid, lc);
-    if (s.packs == 2) return run_rms_bwd<T, VEC, 2, 256>(p, s, grid, lc);
-    if constexpr (VEC == 1) return s.packs == 4 ? run_rms_bwd<T, VEC, 4, 256>(p, s, grid, lc) : run_rms_bwd<T, VEC, 8, 256>(p, s, grid, lc);
-    else return run_rms_bwd<T, VEC, 4, 256>(p, s, grid, lc);
-  }
-  if constexpr (VEC > 1) { if (s.threads == 512 && s.packs <= 2) return run_rms_bwd<T, VEC, 2, 512>(p, s, grid, lc); }
-  if (s.packs <= 2) return run_rms_bwd<T, VEC, 2, 1024>(p, s, grid, lc);
   if constexpr (VEC == 1) {
-    if (s.packs == 8) return run_rms_bwd<T, VEC, 8, 1024>(p, s, grid, lc);
-    if (s.packs == 16) return run_rms_bwd<T, VEC, 16, 1024>(p, s, grid, lc);
+    if (s.threads == 256) {
+      if (s.packs == 1) return run_rms_bwd<T, 1, 1, 256>(p, s, grid, lc);
+      return s.packs <= 4 ? run_rms_bwd<T, 1, 4, 256>(p, s, grid, lc) : run_rms_bwd<T, 1, 8, 256>(p, s, grid, lc);
+    }
+    if (s.threads == 512) return s.packs <= 4 ? run_rms_bwd<T, 1, 4, 512>(p, s, grid, lc) : run_rms_bwd<T, 1, 12, 512>(p, s, grid, lc);
+    return s.packs <= 8 ? run_rms_bwd<T, 1, 8, 1024>(p, s, grid, lc) : run_rms_bwd<T, 1, 16, 1024>(p, s, grid, lc);
+  } else {
+    if (s.threads == 256) return s.packs == 1 ? run_rms_bwd<T, VEC, 1, 256>(p, s, grid, lc) : run_rms_bwd<T, VEC, 2, 256>(p, s, grid, lc);
+    if (s.threads == 512) return run_rms_bwd<T, VEC, 2, 512>(p, s, grid, lc);
+    if constexpr (sizeof(T) == 4) { if (s.packs > 2) return run_rms_bwd<T, VEC, 4, 1024>(p, s, grid, lc); }
+    return run_rms_bwd<T, VEC, 2, 1024>(p, s, grid, lc);
   }
-  return run_rms_bwd<T, VEC, 4, 1024>(p, s, grid, lc);
 }
 
 template <typename T>
@@ -502,7 +511,10 @@ cudaError_t rms_backward(const RmsParams& p, const LaunchCtx& lc) {
   constexpr uint32_t VEC = 16 / sizeof(S);
   RmsParams q = p;
   const bool aligned = p.cols % VEC == 0 && p.ld % VEC == 0;
-  const RmsShape s = rms_shape(p.rows, aligned ? p.cols / VEC : p.cols, aligned ? 2 : 8, lc.sm_count);
+  const uint32_t vectors = aligned ? p.cols / VEC : p.cols;
+  RmsShape s = rms_shape(p.rows, vectors, aligned ? 2 : 8, lc.sm_count);
+  if (!aligned && s.log_tpr == 10 && vectors <= 512 * 12) { s.log_tpr = 9; s.threads = 512; }
+  s.packs = (int)((vectors + (1u << s.log_tpr) - 1) >> s.log_tpr);
   q.log_tpr = s.log_tpr;
   unsigned grid = 0;
   cudaError_t e = aligned ? run_rms_bwd_packs<T, (int)VEC>(q, s, &grid, lc) : run_rms_bwd_packs<T, 1>(q, s, &grid, lc);
