@@ -634,7 +634,7 @@ int32_t zyxb_program_create(zyxb_ctx* ctx, int32_t dev, const zyxb_kernel_desc* 
   if (desc->kind == ZYXB_KIND_MUON) {
     NOT_WHILE_CAPTURING("zyxb_program_create of a Muon program", ZYXB_ERR_KERNEL_COMPILATION);
     workspace_bytes = round_up(muon_workspace_bytes(desc->u.muon, desc->u.muon.rows, desc->u.muon.cols), 512);
-    cudaError_t e = device_malloc(D, workspace_bytes, &workspace);
+    cudaError_t e = workspace_bytes ? device_malloc(D, workspace_bytes, &workspace) : cudaSuccess;
     if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "program_create: workspace", e); }
   }
   uint32_t id;

@@ -1,0 +1,408 @@
+// The whole update of a matrix with at most 128 rows (or columns) in one launch: momentum, norm, every Newton-Schulz step and the
+// weight's step, by one thread-block cluster per matrix.
+//
+// X [128, hi] is cut along hi over the cluster's CTAs and stays in their shared memory as f16 parts from the first step to the last.
+// Per step and CTA:
+//   gram   the partial Gram matrix of its columns (tcgen05, both operands the same tiles), added over the cluster through
+//          distributed shared memory: each CTA adds 128 / C of the rows, in CTA order, and hands them to all
+//   poly   B = a I + b A + c A^2, by every CTA for itself; B takes A's place
+//   apply  X <- B X, its own columns
+// A tile of 64 columns holds 128 rows of 128 bytes, 16-byte units swizzled by row: as an operand of the Gram product it is K-major (the
+// contraction runs along the 128 bytes), as the right operand of B X it is MN-major (the contraction runs down the rows).  The same
+// bytes serve both, so nothing is transposed.
+// What a step costs is latency: three dependent groups of products of a few hundred clocks, and four cluster barriers.
+#pragma once
+#include "muon_gemm.cuh"
+#include "rounding.cuh"
+
+namespace zyxb {
+namespace muon {
+
+constexpr int SMALL_ROWS = 128, SMALL_THREADS = 256, SMALL_CTAS = 8;
+enum { ERR_SMALL = 0x100000u };
+
+template <int PARTS> struct Small {
+  static constexpr int COLS = 512 / PARTS;                       // of X per CTA, at most: 128 KB
+  static constexpr int TILE_BYTES = SMALL_ROWS * 128;            // 64 columns of one part
+  static constexpr int X = 0;                                    // [tile][part]
+  static constexpr int A = SMALL_ROWS * COLS * 2 * PARTS;        // [part][tile of 64 columns]
+  static constexpr int STAGE = A + PARTS * 2 * TILE_BYTES;       // f32 [128][64], for the exchange
+  static constexpr int TAIL = STAGE + SMALL_ROWS * 64 * 4;
+  static constexpr int TOTAL = TAIL + 256 + 1024;
+};
+
+struct SmallMatrix { void* p; const void* g; void* buf; uint32_t tall; };
+constexpr int SMALL_TABLE = 32;
+struct SmallArgs {
+  SmallMatrix m[SMALL_TABLE];
+  uint32_t lo, hi, cols;            // cols of X per CTA, a multiple of 64
+  float momentum, grad_scale, eps, a, b, c, decay, step_flat, step_tall;
+  int steps, nesterov, rn;
+  uint32_t* status;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ double ld_cluster_f64(uint32_t addr) { double v; asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory"); return v; }
+__device__ __forceinline__ void st_cluster2(uint32_t addr, uint32_t x, uint32_t y) { asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory"); }
+__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+
+// byte of element (row, column below 64) inside a tile
+__device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t col) { return row * 128 + ((((col >> 3) ^ row) & 7) << 4) + ((col & 7) << 1); }
+
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_constant__ SmallArgs p) {
+  using SM = Small<PARTS>;
+  using S = typename Elem<T>::store_t;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  const uint32_t bar = base + SM::TAIL;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::TAIL + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  double* sums = reinterpret_cast<double*>(smem + SM::TAIL + 16);      // [0] this CTA's, [1..8] the warps'
+  const uint32_t rank = cluster_rank(), ctas = cluster_size(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
+  // all of X and A, so that rows and columns the matrix does not have are zeros
+  for (uint32_t i = threadIdx.x; i < SM::STAGE / 16; i += SMALL_THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  const SmallMatrix& m = p.m[blockIdx.x / ctas];
+  const uint32_t j0 = rank * p.cols, nj = p.hi > j0 ? min(p.cols, p.hi - j0) : 0;        // this CTA's columns of X
+  const S* g = (const S*)m.g;
+  S* b = (S*)m.buf;
+  // Eight neighbours in memory per item.  Lying: eight columns of a row of X; standing (the stored matrix is X transposed): eight rows of
+  // a column of X, neighbouring lanes on neighbouring columns.
+  const uint32_t eights = m.tall ? (p.lo + 7) / 8 : (nj + 7) / 8, items = m.tall ? eights * nj : eights * p.lo;
+  const uint32_t row_len = m.tall ? p.lo : p.hi;
+  const bool vector = row_len % 8 == 0;
+  auto place = [&](uint32_t item, uint32_t& r, uint32_t& c) {       // of the stored matrix
+    if (m.tall) { r = j0 + item % nj; c = item / nj * 8; }
+    else { r = item / eights; c = j0 + item % eights * 8; }
+  };
+  // entries behind the row, or behind this CTA's columns, are not this item's
+  auto count = [&](uint32_t c) { return m.tall ? min(8u, p.lo - c) : min(8u, j0 + nj - c); };
+  auto load = [&](float (&v)[8], const S* from, uint64_t at, uint32_t n) {
+    if (vector && n == 8) {
+      constexpr int VEC = 16 / (int)sizeof(S);
+#pragma unroll
+      for (int h = 0; h < 8 / VEC; ++h) {
+        RawVec<T, VEC> r;
+        r.load(from + at + h * VEC);
+        float f[VEC];
+        r.decode(f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[h * VEC + j] = f[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < (int)n ? Elem<T>::load(from[at + j]) : 0.0f;
+    }
+  };
+  auto save = [&](const float (&v)[8], S* to, uint64_t at, uint32_t n, bool rn) {
+    if (vector && n == 8) {
+      constexpr int VEC = 16 / (int)sizeof(S);
+#pragma unroll
+      for (int h = 0; h < 8 / VEC; ++h) {
+        RawVec<T, VEC> r;
+        float o[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = v[h * VEC + j];
+        round_encode<T, VEC>(r, o, rn);
+        r.store(to + at + h * VEC);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < (int)n) to[at + j] = round_store<T>(v[j], rn);
+    }
+  };
+
+  // momentum, and the sum of squares of the direction (64 bits: see muon.cu)
+  double sum = 0.0;
+  for (uint32_t i = threadIdx.x; i < items; i += SMALL_THREADS) {
+    uint32_t r, c;
+    place(i, r, c);
+    const uint64_t at = (uint64_t)r * row_len + c;
+    const uint32_t n = count(c);
+    float u[8], f[8];
+    load(u, g, at, n);
+    if (b) load(f, b, at, n);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      u[j] *= p.grad_scale;
+      if (b) {
+        f[j] = Elem<T>::load(round_store<T>(p.momentum * f[j] + u[j], p.rn != 0));
+        u[j] = p.nesterov ? u[j] + p.momentum * f[j] : f[j];
+      }
+      sum += (double)u[j] * (double)u[j];
+    }
+    if (b) save(f, b, at, n, true);          // exact: rounded above
+  }
+  sum = warp_reduce(sum, OpSum());
+  if (lane == 0) sums[1 + warp] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int w = 0; w < SMALL_THREADS / 32; ++w) s += sums[1 + w];
+    sums[0] = s;
+  }
+  cluster_sync();
+  double total = 0.0;
+  for (uint32_t q = 0; q < ctas; ++q) total += ld_cluster_f64(map_to(smem_u32(sums), q));
+  const float inv = SCALE / ((float)sqrt(total) + p.eps);
+  for (uint32_t i = threadIdx.x; i < items; i += SMALL_THREADS) {
+    uint32_t r, c;
+    place(i, r, c);
+    const uint64_t at = (uint64_t)r * row_len + c;
+    const uint32_t n = count(c);
+    float u[8], f[8];
+    load(u, g, at, n);
+    if (b) load(f, b, at, n);                // what this thread stored
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      u[j] *= p.grad_scale;
+      if (b) u[j] = p.nesterov ? u[j] + p.momentum * f[j] : f[j];
+      u[j] *= inv;
+    }
+    uint32_t w[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split2(u[2 * j], u[2 * j + 1], w[0][j], w[1][j]);
+    if (!m.tall) {
+      const uint32_t col = c - j0;
+#pragma unroll
+      for (int s = 0; s < PARTS; ++s)
+        *reinterpret_cast<uint4*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(r, col & 63)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+    } else {
+      const uint32_t col = r - j0;
+#pragma unroll
+      for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint16_t*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(c + j, col & 63)) = (uint16_t)(w[s][j / 2] >> (16 * (j & 1)));
+    }
+  }
+  fence_proxy_async_all();
+  tc_fence_before();
+  __syncthreads();
+
+  constexpr uint32_t gram_idesc = make_idesc(false, false, false, 128, 128);
+  const uint32_t tiles = p.cols / 64, x_base = base + SM::X, a_base = base + SM::A, stage = base + SM::STAGE;
+  const uint32_t quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane, lane_addr = (quarter * 32u) << 16;
+  uint32_t phase = 0;
+  // one product with its parts; the small ones first
+  auto multiply = [&](uint32_t d, uint32_t a, uint32_t a_part, uint32_t bb, uint32_t b_part, uint32_t lbo, uint32_t idesc, bool more) {
+    auto ad = [&](int q) { return make_smem_desc(a + q * a_part, 16, 1024); };
+    auto bd = [&](int q) { return make_smem_desc(bb + q * b_part, lbo, 1024); };
+    if constexpr (PARTS == 2) {
+      umma_f16(d, ad(1), bd(0), idesc, more ? 1u : 0u);
+      umma_f16(d, ad(0), bd(1), idesc, 1u);
+      umma_f16(d, ad(0), bd(0), idesc, 1u);
+    } else {
+      umma_f16(d, ad(0), bd(0), idesc, more ? 1u : 0u);
+    }
+  };
+  auto wait = [&] {
+    mbar_wait(bar, phase, abort_flag, p.status, ERR_SMALL);      // given up: the status word tells, every barrier below is still reached
+    phase ^= 1;
+    tc_fence_after();
+  };
+  // this thread's row of A, 32 columns from c on
+  auto a_at = [&](int s, uint32_t c) { return smem + SM::A + (s * 2 + (c >> 6)) * SM::TILE_BYTES + tile_at(row, c & 63); };
+
+  for (int it = 0; it < p.steps; ++it) {
+    // ---- gram: two parts: an accumulator per 128 of k (24 additions), as in muon_gemm.cuh
+    if (threadIdx.x == 0) {
+      tc_fence_after();
+      for (uint32_t t = 0; t < tiles; ++t)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint32_t at = x_base + t * PARTS * SM::TILE_BYTES + kk * 32, d = tmem + (PARTS == 2 ? (t >> 1) * 128 : 0);
+          multiply(d, at, SM::TILE_BYTES, at, SM::TILE_BYTES, 16, gram_idesc, (PARTS == 2 ? (t & 1) : t) != 0 || kk != 0);
+        }
+      umma_commit(bar);
+    }
+    wait();
+#pragma unroll 1
+    for (uint32_t pass = 0; pass < 2; ++pass) {
+      float v[32];
+      {
+        uint32_t r[32];
+        tmem_ld32(tmem + lane_addr + pass * 64 + half * 32, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        if (PARTS == 2 && tiles > 2) {
+          tmem_ld32(tmem + lane_addr + 128 + pass * 64 + half * 32, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
+        }
+      }
+#pragma unroll
+      for (uint32_t q = 0; q < 8; ++q)
+        *reinterpret_cast<float4*>(smem + SM::STAGE + row * 256 + (((half * 8 + q) ^ (row & 15)) << 4)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      cluster_sync();
+      // rows rank, rank + C, ...: 16 units of four columns each
+      for (uint32_t i = threadIdx.x; i < SMALL_ROWS / ctas * 16; i += SMALL_THREADS) {
+        const uint32_t rr = i / 16 * ctas + rank, q = i % 16, at = stage + rr * 256 + ((q ^ (rr & 15)) << 4);
+        float4 f[SMALL_CTAS];
+#pragma unroll
+        for (uint32_t k = 0; k < SMALL_CTAS; ++k)
+          if (k < ctas) f[k] = ld_cluster4(map_to(at, k));
+        float4 s = f[0];
+#pragma unroll
+        for (uint32_t k = 1; k < SMALL_CTAS; ++k)
+          if (k < ctas) { s.x += f[k].x; s.y += f[k].y; s.z += f[k].z; s.w += f[k].w; }
+        uint32_t w[2][2];
+        split2(s.x * UNSCALE, s.y * UNSCALE, w[0][0], w[1][0]);
+        split2(s.z * UNSCALE, s.w * UNSCALE, w[0][1], w[1][1]);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          const uint32_t to = a_base + (part * 2 + pass) * SM::TILE_BYTES + tile_at(rr, q * 4);
+          for (uint32_t k = 0; k < ctas; ++k) st_cluster2(map_to(to, k), w[part][0], w[part][1]);
+        }
+      }
+      fence_proxy_async_all();
+      tc_fence_before();
+      cluster_sync();
+    }
+    // ---- poly
+    if (threadIdx.x == 0) {
+      fence_proxy_async_all();
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const uint32_t at = a_base + (kk >> 2) * SM::TILE_BYTES + (kk & 3) * 32;
+        multiply(tmem, at, 2 * SM::TILE_BYTES, at, 2 * SM::TILE_BYTES, 16, gram_idesc, kk != 0);
+      }
+      umma_commit(bar);
+    }
+    wait();
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t c0 = half * 64 + h * 32;
+      uint32_t r[32];
+      tmem_ld32(tmem + lane_addr + c0, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q) {
+        uint4* at[PARTS];
+        float a8[8];
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) {
+          at[s] = reinterpret_cast<uint4*>(a_at(s, c0 + q * 8));
+          const uint4 w = *at[s];
+          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&ws[j]));
+            a8[2 * j] = s ? a8[2 * j] + f.x : f.x;
+            a8[2 * j + 1] = s ? a8[2 * j + 1] + f.y : f.y;
+          }
+        }
+        uint32_t w[2][4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float v = p.c * (__uint_as_float(r[q * 8 + j]) * UNSCALE) + p.b * a8[j];
+          if (c0 + q * 8 + j == row) v += p.a * SCALE;
+          a8[j] = v;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split2(a8[2 * j], a8[2 * j + 1], w[0][j], w[1][j]);
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) *at[s] = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+      }
+    }
+    fence_proxy_async_all();
+    tc_fence_before();
+    __syncthreads();
+    // ---- apply: 256 columns per product at most
+    const uint32_t d0 = PARTS == 2 ? 256 : 0;
+    if (threadIdx.x == 0) {
+      tc_fence_after();
+      for (uint32_t c0 = 0; c0 < p.cols; c0 += 256) {
+        const uint32_t idesc = make_idesc(false, false, true, 128, (int)min(256u, p.cols - c0));
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          multiply(tmem + d0 + c0, a_base + (kk >> 2) * SM::TILE_BYTES + (kk & 3) * 32, 2 * SM::TILE_BYTES, x_base + (c0 >> 6) * PARTS * SM::TILE_BYTES + kk * 2048,
+                   SM::TILE_BYTES, PARTS * SM::TILE_BYTES, idesc, kk != 0);
+      }
+      umma_commit(bar);
+    }
+    wait();
+#pragma unroll 1
+    for (uint32_t c0 = half * 32; c0 < p.cols; c0 += 64) {
+      uint32_t r[32];
+      tmem_ld32(tmem + lane_addr + d0 + c0, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q) {
+        uint32_t w[2][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split2(__uint_as_float(r[q * 8 + 2 * j]) * UNSCALE, __uint_as_float(r[q * 8 + 2 * j + 1]) * UNSCALE, w[0][j], w[1][j]);
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s)
+          *reinterpret_cast<uint4*>(smem + SM::X + ((c0 >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(row, (c0 & 63) + q * 8)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+      }
+    }
+    fence_proxy_async_all();
+    tc_fence_before();
+    __syncthreads();
+  }
+
+  // ---- the weight's step
+  S* pw = (S*)m.p;
+  const float step = (m.tall ? p.step_tall : p.step_flat) * UNSCALE;
+  for (uint32_t i = threadIdx.x; i < items; i += SMALL_THREADS) {
+    uint32_t r, c;
+    place(i, r, c);
+    const uint64_t at = (uint64_t)r * row_len + c;
+    const uint32_t n = count(c);
+    float f[8], x[8];
+    load(f, pw, at, n);
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t xr = m.tall ? c + j : r, col = m.tall ? r - j0 : c - j0 + j;
+        const float v = f16_to_f32(*reinterpret_cast<const uint16_t*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(xr, col & 63)));
+        x[j] = s ? x[j] + v : v;
+      }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = f[j] * p.decay - step * x[j];
+    save(f, pw, at, n, p.rn != 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace muon
+}  // namespace zyxb
