@@ -10,7 +10,8 @@
 // A tile of 64 columns holds 128 rows of 128 bytes, 16-byte units swizzled by row: as an operand of the Gram product it is K-major (the
 // contraction runs along the 128 bytes), as the right operand of B X it is MN-major (the contraction runs down the rows).  The same
 // bytes serve both, so nothing is transposed.
-// What a step costs is latency: three dependent groups of products of a few hundred clocks, and four cluster barriers.
+// What a step costs is latency: three dependent groups of products of some 1500 clocks each, and two cluster barriers around the
+// exchange (which moves the triangle: distributed shared memory carried some 14 bytes a clock per SM).
 #pragma once
 #include "muon_gemm.cuh"
 #include "rounding.cuh"
@@ -26,8 +27,8 @@ template <int PARTS> struct Small {
   static constexpr int TILE_BYTES = SMALL_ROWS * 128;            // 64 columns of one part
   static constexpr int X = 0;                                    // [tile][part]
   static constexpr int A = SMALL_ROWS * COLS * 2 * PARTS;        // [part][tile of 64 columns]
-  static constexpr int STAGE = A + PARTS * 2 * TILE_BYTES;       // f32 [128][64], for the exchange
-  static constexpr int TAIL = STAGE + SMALL_ROWS * 64 * 4;
+  static constexpr int STAGE = A + PARTS * 2 * TILE_BYTES;       // f32, the lower triangle of [128][128], for the exchange
+  static constexpr int TAIL = STAGE + 4 * (32 * 33 / 2) * 16;
   static constexpr int TOTAL = TAIL + 256 + 1024;
 };
 
@@ -59,6 +60,20 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
 __device__ __forceinline__ double ld_cluster_f64(uint32_t addr) { double v; asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory"); return v; }
 __device__ __forceinline__ void st_cluster2(uint32_t addr, uint32_t x, uint32_t y) { asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory"); }
 __device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+
+// the exchanged lower triangle: units of four columns
+constexpr uint32_t STAGE_UNITS = 4 * 32 * 33 / 2;
+__device__ __forceinline__ uint32_t unit_at(uint32_t row, uint32_t unit) {
+  const uint32_t q = row / 4;
+  return (2 * q * (q + 1) + (row % 4) * (q + 1) + unit) * 16;
+}
+// four 8 x 8 matrices of 16-bit entries; each lane names one row of one of them
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void stmatrix4_trans(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 
 // byte of element (row, column below 64) inside a tile
 __device__ __forceinline__ uint32_t tile_at(uint32_t row, uint32_t col) { return row * 128 + ((((col >> 3) ^ row) & 7) << 4) + ((col & 7) << 1); }
@@ -141,26 +156,43 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     }
   };
 
+  // U items at a time, so that their loads are in flight together: f(first, loaded) for each
+  constexpr uint32_t U = 4;
+  struct Item { uint64_t at; uint32_t r, c, n; };
+  auto item_at = [&](uint32_t i) {
+    Item t{0, 0, 0, 0};
+    if (i < items) {
+      place(i, t.r, t.c);
+      t.at = (uint64_t)t.r * row_len + t.c;
+      t.n = count(t.c);
+    }
+    return t;
+  };
+
   // momentum, and the sum of squares of the direction (64 bits: see muon.cu)
   double sum = 0.0;
-  for (uint32_t i = threadIdx.x; i < items; i += SMALL_THREADS) {
-    uint32_t r, c;
-    place(i, r, c);
-    const uint64_t at = (uint64_t)r * row_len + c;
-    const uint32_t n = count(c);
-    float u[8], f[8];
-    load(u, g, at, n);
-    if (b) load(f, b, at, n);
+  for (uint32_t i0 = threadIdx.x; i0 < items; i0 += U * SMALL_THREADS) {
+    Item t[U];
+    float u[U][8], f[U][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      u[j] *= p.grad_scale;
-      if (b) {
-        f[j] = Elem<T>::load(round_store<T>(p.momentum * f[j] + u[j], p.rn != 0));
-        u[j] = p.nesterov ? u[j] + p.momentum * f[j] : f[j];
-      }
-      sum += (double)u[j] * (double)u[j];
+    for (uint32_t e = 0; e < U; ++e) {
+      t[e] = item_at(i0 + e * SMALL_THREADS);
+      load(u[e], g, t[e].at, t[e].n);
+      if (b) load(f[e], b, t[e].at, t[e].n);
     }
-    if (b) save(f, b, at, n, true);          // exact: rounded above
+#pragma unroll
+    for (uint32_t e = 0; e < U; ++e) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        u[e][j] *= p.grad_scale;
+        if (b) {
+          f[e][j] = Elem<T>::load(round_store<T>(p.momentum * f[e][j] + u[e][j], p.rn != 0));
+          u[e][j] = p.nesterov ? u[e][j] + p.momentum * f[e][j] : f[e][j];
+        }
+        sum += (double)u[e][j] * (double)u[e][j];
+      }
+      if (b) save(f[e], b, t[e].at, t[e].n, true);          // exact: rounded above
+    }
   }
   sum = warp_reduce(sum, OpSum());
   if (lane == 0) sums[1 + warp] = sum;
@@ -174,35 +206,40 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
   double total = 0.0;
   for (uint32_t q = 0; q < ctas; ++q) total += ld_cluster_f64(map_to(smem_u32(sums), q));
   const float inv = SCALE / ((float)sqrt(total) + p.eps);
-  for (uint32_t i = threadIdx.x; i < items; i += SMALL_THREADS) {
-    uint32_t r, c;
-    place(i, r, c);
-    const uint64_t at = (uint64_t)r * row_len + c;
-    const uint32_t n = count(c);
-    float u[8], f[8];
-    load(u, g, at, n);
-    if (b) load(f, b, at, n);                // what this thread stored
+  for (uint32_t i0 = threadIdx.x; i0 < items; i0 += U * SMALL_THREADS) {
+    Item t[U];
+    float u[U][8], f[U][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      u[j] *= p.grad_scale;
-      if (b) u[j] = p.nesterov ? u[j] + p.momentum * f[j] : f[j];
-      u[j] *= inv;
+    for (uint32_t e = 0; e < U; ++e) {
+      t[e] = item_at(i0 + e * SMALL_THREADS);
+      load(u[e], g, t[e].at, t[e].n);
+      if (b) load(f[e], b, t[e].at, t[e].n);                // what this thread stored
     }
-    uint32_t w[2][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) split2(u[2 * j], u[2 * j + 1], w[0][j], w[1][j]);
-    if (!m.tall) {
-      const uint32_t col = c - j0;
+    for (uint32_t e = 0; e < U; ++e) {
+      if (t[e].n == 0) continue;
 #pragma unroll
-      for (int s = 0; s < PARTS; ++s)
-        *reinterpret_cast<uint4*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(r, col & 63)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
-    } else {
-      const uint32_t col = r - j0;
+      for (int j = 0; j < 8; ++j) {
+        u[e][j] *= p.grad_scale;
+        if (b) u[e][j] = p.nesterov ? u[e][j] + p.momentum * f[e][j] : f[e][j];
+        u[e][j] *= inv;
+      }
+      uint32_t w[2][4];
 #pragma unroll
-      for (int s = 0; s < PARTS; ++s)
+      for (int j = 0; j < 4; ++j) split2(u[e][2 * j], u[e][2 * j + 1], w[0][j], w[1][j]);
+      if (!m.tall) {
+        const uint32_t col = t[e].c - j0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          *reinterpret_cast<uint16_t*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(c + j, col & 63)) = (uint16_t)(w[s][j / 2] >> (16 * (j & 1)));
+        for (int s = 0; s < PARTS; ++s)
+          *reinterpret_cast<uint4*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(t[e].r, col & 63)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+      } else {
+        const uint32_t col = t[e].r - j0;
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint16_t*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(t[e].c + j, col & 63)) = (uint16_t)(w[s][j / 2] >> (16 * (j & 1)));
+      }
     }
   }
   fence_proxy_async_all();
@@ -230,8 +267,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     phase ^= 1;
     tc_fence_after();
   };
-  // this thread's row of A, 32 columns from c on
-  auto a_at = [&](int s, uint32_t c) { return smem + SM::A + (s * 2 + (c >> 6)) * SM::TILE_BYTES + tile_at(row, c & 63); };
+  auto a_byte = [&](uint32_t s, uint32_t r, uint32_t c) { return (s * 2 + (c >> 6)) * SM::TILE_BYTES + tile_at(r, c & 63); };     // of A
 
   for (int it = 0; it < p.steps; ++it) {
     // ---- gram: two parts: an accumulator per 128 of k (24 additions), as in muon_gemm.cuh
@@ -246,50 +282,74 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
       umma_commit(bar);
     }
     wait();
-#pragma unroll 1
-    for (uint32_t pass = 0; pass < 2; ++pass) {
+    // The lower triangle, in units of four columns: row r has r / 4 + 1 of them, behind 2 q (q + 1) + (r % 4)(q + 1) others (q = r / 4).
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint32_t c0 = half * 64 + h * 32;
+      if (c0 > quarter * 32) continue;                 // above the diagonal for the whole warp
       float v[32];
-      {
-        uint32_t r[32];
-        tmem_ld32(tmem + lane_addr + pass * 64 + half * 32, r);
+      uint32_t r[32];
+      tmem_ld32(tmem + lane_addr + c0, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+      if (PARTS == 2 && tiles > 2) {
+        tmem_ld32(tmem + lane_addr + 128 + c0, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-        if (PARTS == 2 && tiles > 2) {
-          tmem_ld32(tmem + lane_addr + 128 + pass * 64 + half * 32, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
-        }
+        for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r[j]);
       }
 #pragma unroll
       for (uint32_t q = 0; q < 8; ++q)
-        *reinterpret_cast<float4*>(smem + SM::STAGE + row * 256 + (((half * 8 + q) ^ (row & 15)) << 4)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-      cluster_sync();
-      // rows rank, rank + C, ...: 16 units of four columns each
-      for (uint32_t i = threadIdx.x; i < SMALL_ROWS / ctas * 16; i += SMALL_THREADS) {
-        const uint32_t rr = i / 16 * ctas + rank, q = i % 16, at = stage + rr * 256 + ((q ^ (rr & 15)) << 4);
-        float4 f[SMALL_CTAS];
-#pragma unroll
-        for (uint32_t k = 0; k < SMALL_CTAS; ++k)
-          if (k < ctas) f[k] = ld_cluster4(map_to(at, k));
-        float4 s = f[0];
-#pragma unroll
-        for (uint32_t k = 1; k < SMALL_CTAS; ++k)
-          if (k < ctas) { s.x += f[k].x; s.y += f[k].y; s.z += f[k].z; s.w += f[k].w; }
-        uint32_t w[2][2];
-        split2(s.x * UNSCALE, s.y * UNSCALE, w[0][0], w[1][0]);
-        split2(s.z * UNSCALE, s.w * UNSCALE, w[0][1], w[1][1]);
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-          const uint32_t to = a_base + (part * 2 + pass) * SM::TILE_BYTES + tile_at(rr, q * 4);
-          for (uint32_t k = 0; k < ctas; ++k) st_cluster2(map_to(to, k), w[part][0], w[part][1]);
-        }
-      }
-      fence_proxy_async_all();
-      tc_fence_before();
-      cluster_sync();
+        if (c0 / 4 + q <= row / 4) *reinterpret_cast<float4*>(smem + SM::STAGE + unit_at(row, c0 / 4 + q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
     }
+    cluster_sync();
+    // the C-th part of the units each
+    const uint32_t share = (STAGE_UNITS + ctas - 1) / ctas;
+    for (uint32_t i = rank * share + threadIdx.x; i < min(STAGE_UNITS, (rank + 1) * share); i += SMALL_THREADS) {
+      float4 f[SMALL_CTAS];
+#pragma unroll
+      for (uint32_t k = 0; k < SMALL_CTAS; ++k)
+        if (k < ctas) f[k] = ld_cluster4(map_to(stage + i * 16, k));
+      uint32_t q4 = (uint32_t)((sqrtf(1.0f + 2.0f * (float)i) - 1.0f) * 0.5f);       // 2 q (q + 1) <= i
+      while (2 * (q4 + 1) * (q4 + 2) <= i) ++q4;
+      while (2 * q4 * (q4 + 1) > i) --q4;
+      const uint32_t in = i - 2 * q4 * (q4 + 1), rr = q4 * 4 + in / (q4 + 1), q = in % (q4 + 1);
+      float4 s = f[0];
+#pragma unroll
+      for (uint32_t k = 1; k < SMALL_CTAS; ++k)
+        if (k < ctas) { s.x += f[k].x; s.y += f[k].y; s.z += f[k].z; s.w += f[k].w; }
+      uint32_t w[2][2];
+      split2(s.x * UNSCALE, s.y * UNSCALE, w[0][0], w[1][0]);
+      split2(s.z * UNSCALE, s.w * UNSCALE, w[0][1], w[1][1]);
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
+        const uint32_t to = a_base + a_byte(part, rr, q * 4);
+        for (uint32_t k = 0; k < ctas; ++k) st_cluster2(map_to(to, k), w[part][0], w[part][1]);
+      }
+    }
+    cluster_sync();
+    // the upper triangle: the 120 blocks of 8 x 8 below the diagonal, four per instruction, loaded and stored transposed ...
+    for (uint32_t op = warp; op < 30 * PARTS; op += SMALL_THREADS / 32) {
+      const uint32_t part = op / 30, t = op % 30 * 4 + (lane >> 3);
+      uint32_t bi = (uint32_t)((1.0f + sqrtf(1.0f + 8.0f * (float)t)) * 0.5f);        // bi (bi - 1) / 2 <= t
+      while (bi * (bi + 1) / 2 <= t) ++bi;
+      while (bi * (bi - 1) / 2 > t) --bi;
+      const uint32_t bj = t - bi * (bi - 1) / 2, in = lane & 7;
+      uint32_t r[4];
+      ldmatrix4(r, a_base + a_byte(part, bi * 8 + in, bj * 8));
+      stmatrix4_trans(a_base + a_byte(part, bj * 8 + in, bi * 8), r);
+    }
+    // ... and the blocks on it, a row per thread
+    if (threadIdx.x < 128 * PARTS) {
+      const uint32_t part = threadIdx.x >> 7, r = threadIdx.x & 127, d = r & ~7u;
+#pragma unroll
+      for (uint32_t c = 0; c < 7; ++c)
+        if (d + c < r) *reinterpret_cast<uint16_t*>(smem + SM::A + a_byte(part, d + c, r)) = *reinterpret_cast<const uint16_t*>(smem + SM::A + a_byte(part, r, d + c));
+    }
+    fence_proxy_async_all();
+    tc_fence_before();
+    __syncthreads();
     // ---- poly
     if (threadIdx.x == 0) {
       fence_proxy_async_all();
@@ -314,7 +374,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
         float a8[8];
 #pragma unroll
         for (int s = 0; s < PARTS; ++s) {
-          at[s] = reinterpret_cast<uint4*>(a_at(s, c0 + q * 8));
+          at[s] = reinterpret_cast<uint4*>(smem + SM::A + a_byte(s, row, c0 + q * 8));
           const uint4 w = *at[s];
           const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -377,24 +437,38 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
   // ---- the weight's step
   S* pw = (S*)m.p;
   const float step = (m.tall ? p.step_tall : p.step_flat) * UNSCALE;
-  for (uint32_t i = threadIdx.x; i < items; i += SMALL_THREADS) {
-    uint32_t r, c;
-    place(i, r, c);
-    const uint64_t at = (uint64_t)r * row_len + c;
-    const uint32_t n = count(c);
-    float f[8], x[8];
-    load(f, pw, at, n);
+  for (uint32_t i0 = threadIdx.x; i0 < items; i0 += U * SMALL_THREADS) {
+    Item t[U];
+    float f[U][8];
 #pragma unroll
-    for (int s = 0; s < PARTS; ++s)
+    for (uint32_t e = 0; e < U; ++e) {
+      t[e] = item_at(i0 + e * SMALL_THREADS);
+      load(f[e], pw, t[e].at, t[e].n);
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t xr = m.tall ? c + j : r, col = m.tall ? r - j0 : c - j0 + j;
-        const float v = f16_to_f32(*reinterpret_cast<const uint16_t*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(xr, col & 63)));
-        x[j] = s ? x[j] + v : v;
+    for (uint32_t e = 0; e < U; ++e) {
+      if (t[e].n == 0) continue;
+      float x[8];
+#pragma unroll
+      for (int s = 0; s < PARTS; ++s) {
+        float v[8];
+        const uint32_t col = m.tall ? t[e].r - j0 : t[e].c - j0;
+        const uint8_t* tile = smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES;
+        if (m.tall) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = f16_to_f32(*reinterpret_cast<const uint16_t*>(tile + tile_at(t[e].c + j, col & 63)));
+        } else {
+          RawVec<f16_t, 8> r;
+          r.load(reinterpret_cast<const uint16_t*>(tile + tile_at(t[e].r, col & 63)));
+          r.decode(v);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = s ? x[j] + v[j] : v[j];
       }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = f[j] * p.decay - step * x[j];
-    save(f, pw, at, n, p.rn != 0);
+      for (int j = 0; j < 8; ++j) f[e][j] = f[e][j] * p.decay - step * x[j];
+      save(f[e], pw, t[e].at, t[e].n, p.rn != 0);
+    }
   }
   tc_fence_before();
   __syncthreads();
