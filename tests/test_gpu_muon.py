@@ -72,7 +72,7 @@ def check(sess, dtype, shapes, rng, lr=0.02, weight_decay=0.01, momentum=0.95, n
 
 # up to 128 rows or columns: one launch, while X fits eight CTAs (2048 columns of f32, 4096 of 16-bit); the rest by products
 SHAPES = [(1, 1), (1, 9), (7, 1), (5, 3), (16, 16), (33, 70), (128, 784), (10, 128), (128, 2048), (1999, 100), (2049, 128), (77, 4096), (4097, 33), (130, 129),
-          (300, 77), (513, 260), (256, 1030), (640, 640)]
+          (300, 77), (513, 260), (256, 1030), (640, 640), (129, 4100), (2500, 200), (384, 1537)]
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES, ids=R.NAMES.get)

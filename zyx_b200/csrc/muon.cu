@@ -309,7 +309,9 @@ uint64_t up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
 struct MuonPlan { uint64_t lo, hi; std::vector<int> members; };
 
 uint64_t muon_bytes(uint64_t lo, uint64_t hi, uint64_t batch, int parts) {
-  return up(batch * MUON_PARTIALS * sizeof(double), 256) + 2 * up(batch * parts * lo * up(hi, 8) * 2, 256) + 2 * up(batch * parts * lo * up(lo, 8) * 2, 256);
+  const uint32_t splits = parts == 2 ? muon::split_count<2>((uint32_t)lo, (uint32_t)hi, (uint32_t)batch) : muon::split_count<1>((uint32_t)lo, (uint32_t)hi, (uint32_t)batch);
+  const uint64_t split = splits > 1 ? muon::SPLIT_CTAS * 65536ull : 0;
+  return split + up(batch * MUON_PARTIALS * sizeof(double), 256) + 2 * up(batch * parts * lo * up(hi, 8) * 2, 256) + 2 * up(batch * parts * lo * up(lo, 8) * 2, 256);
 }
 
 // matrices that are updated together, in the order of their first members
@@ -327,7 +329,7 @@ std::vector<MuonPlan> muon_plan(const zyxb_muon_desc& d, const uint64_t* rows, c
 }
 
 // CTAs per matrix of the one-launch update, 0 where it does not take it: X has to fit the cluster's shared memory, 128 rows of 512 columns
-// (256 with two parts) per CTA.  At 128 x 784 f32 it takes SMALL_US us where the launch per product takes 174.
+// (256 with two parts) per CTA.  At 128 x 784 f32 it takes 67 us where a launch per product takes 174.
 template <int PARTS> uint32_t small_ctas(uint64_t lo, uint64_t hi) {
   if (lo > muon::SMALL_ROWS || hi > (uint64_t)muon::SMALL_CTAS * muon::Small<PARTS>::COLS) return 0;
   uint32_t c = 1;
@@ -387,13 +389,15 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
   };
   muon::Operand x[2], gram, poly;
   x[0] = operand(lo, hi); x[1] = operand(lo, hi); gram = operand(lo, lo); poly = operand(lo, lo);
+  const uint32_t splits = muon::split_count<PARTS>(lo, hi, batch);
+  float* split_sums = (float*)at;
 
   const unsigned sums = (unsigned)std::min<uint64_t>(MUON_PARTIALS, ((uint64_t)lo * hi + MUON_THREADS * 16 - 1) / (MUON_THREADS * 16));
   const dim3 tiles((hi + TILE - 1) / TILE, (lo + TILE - 1) / TILE, batch);
   cudaError_t e = launch_pdl(muon_momentum_kernel<T>, dim3(sums, batch), MUON_THREADS, 0, lc.stream, k, partial);
   if (e == cudaSuccess) e = launch_pdl(muon_normalize_kernel<T, PARTS>, tiles, MUON_THREADS, 0, lc.stream, k, partial, (int)sums, d.eps == 0.0f ? 1e-7f : d.eps, x[0]);
 
-  const int bn_sym = muon::tile_width<PARTS, true>(lo, lo, batch, lc.sm_count), bn_apply = muon::tile_width<PARTS, false>(lo, hi, batch, lc.sm_count);
+  const int bn_sym = splits > 1 ? 128 : muon::tile_width<PARTS, true>(lo, lo, batch, lc.sm_count), bn_apply = muon::tile_width<PARTS, false>(lo, hi, batch, lc.sm_count);
   CUtensorMap x_rows[2], x_cols[2], x_k[2], gram_rows, gram_cols, poly_rows;
   bool ok = true;
   for (int j = 0; j < 2; ++j)
@@ -412,7 +416,14 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
   const int steps = d.steps ? d.steps : 5;
   for (int i = 0; i < steps && e == cudaSuccess; ++i) {
     const int from = i & 1;
-    e = bn_sym == 128 ? muon::launch<PARTS, 128, true, false, false>(x_rows[from], x_cols[from], gemm_args(gram, hi), lc)
+    if (splits > 1) {
+      muon::GemmArgs s = gemm_args(gram, hi);
+      s.partial = split_sums; s.splits = splits;
+      e = muon::launch<PARTS, 128, true, false, false, true>(x_rows[from], x_cols[from], s, lc);
+      const unsigned blocks = (lo + 63) / 64;
+      if (e == cudaSuccess)
+        e = launch_pdl(muon::gram_finish_kernel<PARTS>, dim3(blocks, blocks, batch), 256, 0, lc.stream, (const float*)split_sums, splits, muon::tile_count<true>(lo, lo, 128), s);
+    } else e = bn_sym == 128 ? muon::launch<PARTS, 128, true, false, false>(x_rows[from], x_cols[from], gemm_args(gram, hi), lc)
                       : muon::launch<PARTS, 256, true, false, false>(x_rows[from], x_cols[from], gemm_args(gram, hi), lc);
     if (e != cudaSuccess) break;
     muon::GemmArgs g = gemm_args(poly, lo);
@@ -427,7 +438,7 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
   e = launch_pdl(muon_step_kernel<T, PARTS>, tiles, MUON_THREADS, 0, lc.stream, k, x[steps & 1], 1.0f - d.lr * d.weight_decay,
                  d.lr * muon_adjust(d.adjust, lo, hi), d.lr * muon_adjust(d.adjust, hi, lo));
   if (e != cudaSuccess) { err = std::string("muon: ") + cudaGetErrorString(e); return ZYXB_ERR_KERNEL_LAUNCH; }
-  return check_launch(lc, err, "muon", 3 + 3 * steps);
+  return check_launch(lc, err, "muon", 3 + (splits > 1 ? 4 : 3) * steps);
 }
 
 }  // namespace

@@ -10,6 +10,8 @@
 // The pipeline is the 16-bit matmul's: one persistent CTA per SM, warp 0 loads tiles by TMA, warp 1 issues tcgen05.mma, warps 2..9
 // read the accumulators from TMEM while the next tile is multiplied.  What differs:
 //   symmetry  only tiles that touch the lower triangle are computed, and stored twice: half of the work of gram and poly.
+//   split     a gram product with few tiles and a long contraction is cut along it: every CTA leaves its f32 sums, and a second
+//             launch adds them in order (129 x 4096 f32: 3 tiles, 64 k-blocks of 0.5 us each).
 //   rounding  the tensor core adds with truncation, which over 1536 additions costs 1.5e-4 of the result: below the 2^-11 of one
 //             part, far above the 2^-22 of two.  With two parts an accumulator takes 24 additions (128 of k), and the epilogue warps add
 //             the accumulators in f32 registers.
@@ -42,6 +44,8 @@ struct GemmArgs {
   uint32_t m, n, k, batch, tiles_m, tiles_n, tiles, ld;
   uint64_t part, stride;    // elements from hi to lo, from matrix to matrix, of out
   float a, b, c;            // poly; c is 1 otherwise
+  float* partial;           // split gram: [matrix][tile][split][128][BN]
+  uint32_t splits;          // 1: none
   uint32_t* status;
 };
 
@@ -59,7 +63,7 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = pack2_t<false>(x - hx, y - hy);
 }
 
-template <int PARTS, int BN, bool SYM, bool POLY, bool B_MN>
+template <int PARTS, int BN, bool SYM, bool POLY, bool B_MN, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, GemmArgs p) {
   using SM = Smem<PARTS, BN>;
@@ -89,8 +93,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   pdl_trigger();
   pdl_wait();
 
-  const uint32_t total = p.tiles * p.batch, k_blocks = (p.k + BK - 1) / BK;
+  const uint32_t splits = SPLIT ? p.splits : 1, total = p.tiles * p.batch * splits, all_blocks = (p.k + BK - 1) / BK;
+  // the k-blocks of one of the splits (the last of a tile's work items may have fewer, never none)
+  const uint32_t per_split = (all_blocks + splits - 1) / splits;
+  auto k_range = [&](uint32_t t, uint32_t& k0, uint32_t& k1) {
+    k0 = SPLIT ? t % splits * per_split : 0;
+    k1 = SPLIT ? min(all_blocks, k0 + per_split) : all_blocks;
+  };
   auto tile_coords = [&](uint32_t t, uint32_t& z, uint32_t& tm, uint32_t& tn) {
+    if (SPLIT) t /= splits;
     z = t / p.tiles;
     const uint32_t r = t - z * p.tiles;
     if constexpr (SYM) {
@@ -118,7 +129,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
         uint32_t z, tm, tn;
         tile_coords(t, z, tm, tn);
-        for (uint32_t kb = 0; kb < k_blocks; ++kb) {
+        uint32_t kb0, kb1;
+        k_range(t, kb0, kb1);
+        for (uint32_t kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status, ERR_PRODUCER)) { ok = false; break; }
           const uint32_t a_dst = base + stage * SM::STAGE, b_dst = a_dst + PARTS * SM::A_PART;
           mbar_expect_tx(full_bar(stage), SM::STAGE);
@@ -154,8 +167,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
       for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        for (uint32_t kb = 0; kb < k_blocks && ok; ++kb) {
-          const uint32_t in_chunk = PARTS == 2 ? kb % CHUNK_BLOCKS : kb;
+        uint32_t kb0, kb1;
+        k_range(t, kb0, kb1);
+        for (uint32_t kb = kb0; kb < kb1 && ok; ++kb) {
+          const uint32_t in_chunk = PARTS == 2 ? (kb - kb0) % CHUNK_BLOCKS : kb - kb0;
           if (in_chunk == 0) {
             if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1, abort_flag, p.status, ERR_MMA)) { ok = false; break; }
             tc_fence_after();
@@ -182,7 +197,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           }
           umma_commit(empty_bar(stage));
           if (++stage == SM::STAGES) { stage = 0; phase ^= 1; }
-          if (kb + 1 == k_blocks || (PARTS == 2 && in_chunk == CHUNK_BLOCKS - 1)) {
+          if (kb + 1 == kb1 || (PARTS == 2 && in_chunk == CHUNK_BLOCKS - 1)) {
             umma_commit(tfull_bar(acc));
             if (++acc == 2) { acc = 0; acc_phase ^= 1; }
           }
@@ -196,16 +211,24 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     constexpr int HALF = BN / 2, CH = HALF / 32;
     uint32_t acc = 0, acc_phase = 0;
     bool ok = true;
-    const uint32_t n_chunks = PARTS == 2 ? (k_blocks + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS : 1;
     for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
       uint32_t z, tm, tn;
       tile_coords(t, z, tm, tn);
+      uint32_t kb0, kb1;
+      k_range(t, kb0, kb1);
+      const uint32_t n_chunks = PARTS == 2 ? (kb1 - kb0 + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS : 1;
       uint16_t* out = p.out + z * p.stride;
       const uint16_t* gram = POLY ? p.gram + z * p.stride : nullptr;
       const uint32_t row0 = tm * BM + quarter * 32, row = row0 + lane;
       // 32 columns from c on of this lane's row
       auto finish = [&](float (&v)[32], uint32_t c) {
         if (c >= p.n || row0 >= p.m) return;
+        if constexpr (SPLIT) {
+          float4* to = reinterpret_cast<float4*>(p.partial + ((uint64_t)t * BM + quarter * 32 + lane) * BN + (c - tn * BN));
+#pragma unroll
+          for (int q = 0; q < 8; ++q) to[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          return;
+        }
         if (SYM && c > row0) return;                           // above the diagonal: another warp's mirrored block
         const uint64_t at = (uint64_t)row * p.ld + c;
         const bool mine = row < p.m;
@@ -324,6 +347,77 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   }
 }
 
+// ---- split gram ----------------------------------------------------------------------------------------------------------------
+// A = 2^-10 times the sum of the splits' tiles, as parts, with its mirror image: a 64 x 64 block of the lower triangle per CTA.
+template <int PARTS>
+__global__ void __launch_bounds__(256) gram_finish_kernel(const float* __restrict__ partial, uint32_t splits, uint32_t tiles, GemmArgs p) {
+  __shared__ float block[64][65];
+  const uint32_t bi = blockIdx.x, bj = blockIdx.y, z = blockIdx.z;
+  pdl_trigger();
+  pdl_wait();
+  if (bj > bi) return;
+  const uint32_t tm = bi / 2, tn = bj / 2, tile = tm * (tm + 1) / 2 + tn;
+  const float* from = partial + (((uint64_t)z * tiles + tile) * splits * BM + (bi & 1) * 64) * 128 + (bj & 1) * 64;
+  // past m there are rows no split has written; they are not read
+  const uint32_t rows = min(64u, p.m - bi * 64);
+  for (uint32_t i = threadIdx.x; i < rows * 16; i += 256) {
+    const uint32_t r = i / 16, c = i % 16 * 4;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (bj * 64 + (c & 32) < p.m) {
+#pragma unroll 8
+      for (uint32_t k = 0; k < splits; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(from + ((uint64_t)k * BM + r) * 128 + c);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      }
+    }
+    block[r][c] = s.x; block[r][c + 1] = s.y; block[r][c + 2] = s.z; block[r][c + 3] = s.w;
+  }
+  __syncthreads();
+  uint16_t* out = p.out + z * p.stride;
+  auto put = [&](uint32_t row, uint32_t col, const float (&v)[8]) {
+    uint32_t w[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split2(v[2 * j] * UNSCALE, v[2 * j + 1] * UNSCALE, w[0][j], w[1][j]);
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s)
+      *reinterpret_cast<uint4*>(out + s * p.part + (uint64_t)row * p.ld + col) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+  };
+  for (uint32_t i = threadIdx.x; i < 512; i += 256) {
+    const uint32_t r = i / 8, c = i % 8 * 8;
+    if (bi * 64 + r >= p.m || bj * 64 + c >= p.m) continue;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = block[r][c + j];
+    put(bi * 64 + r, bj * 64 + c, v);                      // columns behind m: spare
+  }
+  if (bi == bj) return;
+  for (uint32_t i = threadIdx.x; i < 512; i += 256) {
+    const uint32_t r = i % 64, c = i / 64 * 8;             // row r of the image: column r of the block
+    if (bj * 64 + r >= p.m || bi * 64 + c >= p.m) continue;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < rows ? block[c + j][r] : 0.0f;
+    put(bj * 64 + r, bi * 64 + c, v);
+  }
+}
+
+// CTAs that a split gram product may use: their partial sums are 64 KB each
+constexpr uint32_t SPLIT_CTAS = 144;
+// Splits of a gram product with 128 x 128 tiles: as many as give every CTA work, of four k-blocks at least.  The second launch costs
+// some 5 us a step, a k-block 0.5 us with two parts and 0.15 us with one, so 16 and 40 blocks have to be saved.  Measured, whole
+// updates: 129 x 4096 f32 344 -> 204 us, bf16 186 -> 144; 512 x 2048 f32 297 -> 249; below the rule 1024 x 1024 f32 299 -> 308,
+// bf16 165 -> 198, 512 x 2048 bf16 162 -> 165.
+template <int PARTS> uint32_t split_count(uint32_t m, uint32_t k, uint32_t batch) {
+  const uint32_t tiles_m = (m + BM - 1) / BM;
+  const uint64_t work = (uint64_t)tiles_m * (tiles_m + 1) / 2 * batch;
+  const uint32_t blocks = (k + BK - 1) / BK;
+  const uint32_t s = (uint32_t)std::min<uint64_t>(SPLIT_CTAS / std::max<uint64_t>(1, work), blocks / 4);
+  if (s < 2) return 1;
+  const uint32_t per = (blocks + s - 1) / s;
+  if (blocks - per < (PARTS == 2 ? 16 : 40)) return 1;
+  return (blocks + per - 1) / per;                          // no split without a block
+}
+
 // {contiguous, rows, parts, matrices} with a box of 64 x `box_rows`
 inline bool encode(void* fn, CUtensorMap* map, const Operand& o, int parts, uint32_t batch, uint32_t box_rows) {
   return encode_map(fn, map, false, o.ptr, o.cols, o.rows, o.ld, (uint64_t)parts, parts > 1 ? o.part() : 0, batch, batch > 1 ? o.part() * parts : 0, box_rows);
@@ -344,18 +438,18 @@ template <int PARTS, bool SYM> int tile_width(uint32_t m, uint32_t n, uint32_t b
   return (PARTS == 1 ? 83 : 60) * rounds(128) < 100 * rounds(256) ? 128 : 256;
 }
 
-template <int PARTS, int BN, bool SYM, bool POLY, bool B_MN>
+template <int PARTS, int BN, bool SYM, bool POLY, bool B_MN, bool SPLIT = false>
 cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mb, GemmArgs p, const LaunchCtx& lc) {
   using SM = Smem<PARTS, BN>;
   static uint64_t configured = 0;
-  auto kern = gemm_kernel<PARTS, BN, SYM, POLY, B_MN>;
+  auto kern = gemm_kernel<PARTS, BN, SYM, POLY, B_MN, SPLIT>;
   cudaError_t e = ensure_dynamic_smem(kern, SM::TOTAL, &configured);
   if (e != cudaSuccess) return e;
   p.tiles_m = (p.m + BM - 1) / BM;
   p.tiles_n = (p.n + BN - 1) / BN;
   p.tiles = tile_count<SYM>(p.m, p.n, BN);
   p.status = lc.status_word;
-  const unsigned grid = (unsigned)std::min<uint64_t>((uint64_t)p.tiles * p.batch, (uint64_t)lc.sm_count);
+  const unsigned grid = (unsigned)std::min<uint64_t>((uint64_t)p.tiles * p.batch * (SPLIT ? p.splits : 1), (uint64_t)lc.sm_count);
   return launch_pdl(kern, dim3(grid), THREADS, SM::TOTAL, lc.stream, ma, mb, p);
 }
 
