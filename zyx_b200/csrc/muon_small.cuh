@@ -109,17 +109,10 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
   const uint32_t j0 = rank * p.cols, nj = p.hi > j0 ? min(p.cols, p.hi - j0) : 0;        // this CTA's columns of X
   const S* g = (const S*)m.g;
   S* b = (S*)m.buf;
-  // Eight neighbours in memory per item.  Lying: eight columns of a row of X; standing (the stored matrix is X transposed): eight rows of
-  // a column of X, neighbouring lanes on neighbouring columns.
-  const uint32_t eights = m.tall ? (p.lo + 7) / 8 : (nj + 7) / 8, items = m.tall ? eights * nj : eights * p.lo;
-  const uint32_t row_len = m.tall ? p.lo : p.hi;
-  const bool vector = row_len % 8 == 0;
-  auto place = [&](uint32_t item, uint32_t& r, uint32_t& c) {       // of the stored matrix
-    if (m.tall) { r = j0 + item % nj; c = item / nj * 8; }
-    else { r = item / eights; c = j0 + item % eights * 8; }
-  };
-  // entries behind the row, or behind this CTA's columns, are not this item's
-  auto count = [&](uint32_t c) { return m.tall ? min(8u, p.lo - c) : min(8u, j0 + nj - c); };
+  // Eight neighbours in memory per item.  Lying: eight columns of a row of X.  Standing (the stored matrix is X transposed): this CTA's
+  // columns are whole stored rows, one stretch of memory that starts on a 128-byte boundary, whatever the rows' length.
+  const uint32_t eights = (nj + 7) / 8, stretch = nj * p.lo, items = m.tall ? (stretch + 7) / 8 : eights * p.lo;
+  const bool vector = m.tall || p.hi % 8 == 0;
   auto load = [&](float (&v)[8], const S* from, uint64_t at, uint32_t n) {
     if (vector && n == 8) {
       constexpr int VEC = 16 / (int)sizeof(S);
@@ -158,13 +151,20 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
 
   // U items at a time, so that their loads are in flight together: f(first, loaded) for each
   constexpr uint32_t U = 4;
+  // at: the first element; r, c: its place in X; n: how many of the eight are this item's
   struct Item { uint64_t at; uint32_t r, c, n; };
   auto item_at = [&](uint32_t i) {
     Item t{0, 0, 0, 0};
     if (i < items) {
-      place(i, t.r, t.c);
-      t.at = (uint64_t)t.r * row_len + t.c;
-      t.n = count(t.c);
+      if (m.tall) {
+        t.at = (uint64_t)j0 * p.lo + i * 8;
+        t.c = i * 8 / p.lo; t.r = i * 8 % p.lo;
+        t.n = min(8u, stretch - i * 8);
+      } else {
+        t.r = i / eights; t.c = i % eights * 8;
+        t.at = (uint64_t)t.r * p.hi + j0 + t.c;
+        t.n = min(8u, nj - t.c);
+      }
     }
     return t;
   };
@@ -228,17 +228,20 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
 #pragma unroll
       for (int j = 0; j < 4; ++j) split2(u[e][2 * j], u[e][2 * j + 1], w[0][j], w[1][j]);
       if (!m.tall) {
-        const uint32_t col = t[e].c - j0;
 #pragma unroll
         for (int s = 0; s < PARTS; ++s)
-          *reinterpret_cast<uint4*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(t[e].r, col & 63)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+          *reinterpret_cast<uint4*>(smem + SM::X + ((t[e].c >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(t[e].r, t[e].c & 63)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
       } else {
-        const uint32_t col = t[e].r - j0;
+        uint32_t r = t[e].r, c = t[e].c;
 #pragma unroll
-        for (int s = 0; s < PARTS; ++s)
+        for (int j = 0; j < 8; ++j) {
+          if (j < (int)t[e].n) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint16_t*>(smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(t[e].c + j, col & 63)) = (uint16_t)(w[s][j / 2] >> (16 * (j & 1)));
+            for (int s = 0; s < PARTS; ++s)
+              *reinterpret_cast<uint16_t*>(smem + SM::X + ((c >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(r, c & 63)) = (uint16_t)(w[s][j / 2] >> (16 * (j & 1)));
+          }
+          if (++r == p.lo) { r = 0; ++c; }
+        }
       }
     }
   }
@@ -448,22 +451,28 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
 #pragma unroll
     for (uint32_t e = 0; e < U; ++e) {
       if (t[e].n == 0) continue;
-      float x[8];
+      float x[8] = {};
+      if (m.tall) {
+        uint32_t r = t[e].r, c = t[e].c;
 #pragma unroll
-      for (int s = 0; s < PARTS; ++s) {
-        float v[8];
-        const uint32_t col = m.tall ? t[e].r - j0 : t[e].c - j0;
-        const uint8_t* tile = smem + SM::X + ((col >> 6) * PARTS + s) * SM::TILE_BYTES;
-        if (m.tall) {
+        for (int j = 0; j < 8; ++j) {
+          if (j < (int)t[e].n) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = f16_to_f32(*reinterpret_cast<const uint16_t*>(tile + tile_at(t[e].c + j, col & 63)));
-        } else {
-          RawVec<f16_t, 8> r;
-          r.load(reinterpret_cast<const uint16_t*>(tile + tile_at(t[e].r, col & 63)));
-          r.decode(v);
+            for (int s = 0; s < PARTS; ++s)
+              x[j] += f16_to_f32(*reinterpret_cast<const uint16_t*>(smem + SM::X + ((c >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(r, c & 63)));
+          }
+          if (++r == p.lo) { r = 0; ++c; }
         }
+      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = s ? x[j] + v[j] : v[j];
+        for (int s = 0; s < PARTS; ++s) {
+          RawVec<f16_t, 8> q;
+          q.load(reinterpret_cast<const uint16_t*>(smem + SM::X + ((t[e].c >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(t[e].r, t[e].c & 63)));
+          float v[8];
+          q.decode(v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] += v[j];
+        }
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[e][j] = f[e][j] * p.decay - step * x[j];

@@ -290,43 +290,41 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsParams p) {
 }
 
 // Rows are dealt to the groups of a persistent grid, so that a thread keeps its columns' weights and their gradient in registers
-// from the first of its rows to the last.  Where rows do not start on vector boundaries a vector is one element (a column has to
-// stay with its thread); a warp's loads are then still one line each.
-template <typename T, int VEC, int PACKS, int THREADS>
+// from the first of its rows to the last.  Where rows do not start on vector boundaries, the number of groups is a multiple of the
+// vector's length: all of a group's rows then start at the same place in a vector, and a column stays with its thread.
+template <typename T, int PACKS, bool ALIGNED, int THREADS>
 __global__ void __launch_bounds__(THREADS) rmsnorm_bwd_kernel(const RmsParams p) {
-  using S = typename Elem<T>::store_t;
+  using View = RowView<T, ALIGNED>;
+  constexpr int VEC = View::VEC;
   using Num = Nums<VEC>;
   using V = typename Num::V;
   constexpr int N = Num::N;
   __shared__ float red[2][32][2];
   extern __shared__ float dw_shared[];               // [group of the CTA][cols]
   const int tpr = 1 << p.log_tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & (tpr - 1), groups = blockDim.x >> p.log_tpr;
-  auto col = [&](int i) { return (uint32_t)(t + i * tpr) * VEC; };
+  const uint64_t step = (uint64_t)gridDim.x * groups;
+  const View first((uint64_t)blockIdx.x * groups + in_cta, p.ld, p.cols);        // stands for all rows where only the place in a vector counts
   V w[PACKS][N], dw[PACKS][N];
   pdl_trigger();
   pdl_wait();
 #pragma unroll
   for (int i = 0; i < PACKS; ++i) {
-    RawVec<T, VEC> r;
-    if (p.weight_on && col(i) < p.cols) r.load((const S*)p.weight + col(i)); else r.zero();
-    Num::decode(w[i], r);
+    const int pack = t + i * tpr;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if (!p.weight_on) w[i][k] = Num::splat(1.0f);
-      dw[i][k] = Num::splat(0.0f);
-    }
+    for (int k = 0; k < N; ++k) { w[i][k] = Num::splat(1.0f); dw[i][k] = Num::splat(0.0f); }
+    if (p.weight_on && first.has(pack)) first.weight(w[i], p.weight, pack);
   }
-  const uint64_t step = (uint64_t)gridDim.x * groups;
   struct Row { RawVec<T, VEC> h[PACKS], g[PACKS], d[PACKS]; };
   auto fetch = [&](Row& r, uint64_t row) {
-    const uint64_t at = row * p.ld;
+    const View view(row, p.ld, p.cols);
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
+      const int pack = t + i * tpr;
       r.h[i].zero(); r.g[i].zero(); r.d[i].zero();
-      if (row < p.rows && col(i) < p.cols) {
-        r.h[i].load_stream((const S*)p.h + at + col(i));
-        r.g[i].load_stream((const S*)p.dy + at + col(i));
-        if (p.dh_on) r.d[i].load_stream((const S*)p.dh + at + col(i));
+      if (row < p.rows && view.has(pack)) {
+        view.load(r.h[i], p.h, pack);
+        view.load(r.g[i], p.dy, pack);
+        if (p.dh_on) view.load(r.d[i], p.dh, pack);
       }
     }
   };
@@ -353,12 +351,14 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_bwd_kernel(const RmsParams p)
     float s[2] = {Num::sum(hh), Num::sum(gh)};
     row_sum(s, p.log_tpr, red, parity);
     if (row >= p.rows) continue;                     // this group's last round; the others' barriers are behind it
+    const View view(row, p.ld, p.cols);
     const float rstd = rsqrtf(s[0] * p.inv_cols + p.eps);
     // dx = rstd * (dy w) - h * (rstd^3 * mean(dy w h)) + dh;  dw += dy * h * rstd
     const V up = Num::splat(rstd), down = Num::splat(-(rstd * rstd * rstd) * (s[1] * p.inv_cols));
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-      if (col(i) >= p.cols) continue;
+      const int pack = t + i * tpr;
+      if (!view.has(pack)) continue;
       V o[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) {
@@ -366,21 +366,21 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_bwd_kernel(const RmsParams p)
         dw[i][k] = Num::fma(gu, h[i][k], dw[i][k]);
         o[k] = Num::add(Num::fma(gu, w[i][k], Num::mul(h[i][k], down)), d[i][k]);
       }
-      RawVec<T, VEC> r;
-      Num::encode(r, o, p.rn != 0);
-      r.store_stream((S*)p.y + row * p.ld + col(i));
+      view.store(o, p.y, pack, p.rn != 0);
     }
   }
   if (!p.weight_on) return;
   // the CTA's groups are added in order, then one row of partials per CTA
 #pragma unroll
-  for (int i = 0; i < PACKS; ++i)
-    if (col(i) < p.cols) {
-      float f[VEC];
-      Num::floats(f, dw[i]);
+  for (int i = 0; i < PACKS; ++i) {
+    const int pack = t + i * tpr;
+    if (!first.has(pack)) continue;
+    float f[VEC];
+    Num::floats(f, dw[i]);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) dw_shared[(size_t)in_cta * p.cols + col(i) + k] = f[k];
-    }
+    for (int k = 0; k < VEC; ++k)
+      if (first.inside(first.col(pack) + k)) dw_shared[(size_t)in_cta * p.cols + first.col(pack) + k] = f[k];
+  }
   __syncthreads();
   for (uint32_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
     float sum = 0.0f;
@@ -470,39 +470,38 @@ cudaError_t rms_forward(const RmsParams& p, bool quant, const LaunchCtx& lc) {
   return aligned ? run_rms_packs<T, true>(q, s, quant, lc) : run_rms_packs<T, false>(q, s, quant, lc);
 }
 
-template <typename T, int VEC, int PACKS, int THREADS>
+template <typename T, int PACKS, bool ALIGNED, int THREADS>
 cudaError_t run_rms_bwd(const RmsParams& p, const RmsShape& s, unsigned* grid_out, const LaunchCtx& lc) {
+  constexpr int VEC = 16 / (int)sizeof(typename Elem<T>::store_t);
   const int groups = s.threads >> s.log_tpr;
   const size_t smem = p.weight_on ? (size_t)groups * p.cols * 4 : 0;
-  auto kern = rmsnorm_bwd_kernel<T, VEC, PACKS, THREADS>;
+  auto kern = rmsnorm_bwd_kernel<T, PACKS, ALIGNED, THREADS>;
   static uint64_t configured = 0;
   cudaError_t e = ensure_dynamic_smem(kern, 80 << 10, &configured);
   if (e != cudaSuccess) return e;
   int per_sm = 1;
   if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, s.threads, smem)) != cudaSuccess) return e;
   const uint64_t work = (p.rows + groups - 1) / groups;
-  *grid_out = (unsigned)std::min<uint64_t>(work, (uint64_t)lc.sm_count * std::max(1, per_sm));
+  uint64_t grid = std::min<uint64_t>(work, (uint64_t)lc.sm_count * std::max(1, per_sm));
+  if (!ALIGNED && grid < work) grid = std::max<uint64_t>(VEC, grid / VEC * VEC);      // a group's rows: the same place in a vector
+  *grid_out = (unsigned)grid;
   return launch_pdl(kern, dim3(*grid_out), s.threads, smem, lc.stream, p);
 }
 
 // The adjoint's groups: a column's weight, its gradient, this row's h, dy, dh and the next row's all stay in registers, so a thread
-// takes two vectors (up to twelve single elements where rows are off the boundaries; 512 threads of 128 registers hold 6144 columns
-// that way) and the group grows to 1024 threads.
-template <typename T, int VEC>
+// takes two vectors and the group grows, to 1024 threads.  (Those have 64 registers each: above 8192 columns of 16 bits, 4096 of f32,
+// some of it is spilled.)
+template <typename T, bool ALIGNED>
 cudaError_t run_rms_bwd_packs(const RmsParams& p, const RmsShape& s, unsigned* grid, const LaunchCtx& lc) {
-  if constexpr (VEC == 1) {
-    if (s.threads == 256) {
-      if (s.packs == 1) return run_rms_bwd<T, 1, 1, 256>(p, s, grid, lc);
-      return s.packs <= 4 ? run_rms_bwd<T, 1, 4, 256>(p, s, grid, lc) : run_rms_bwd<T, 1, 8, 256>(p, s, grid, lc);
-    }
-    if (s.threads == 512) return s.packs <= 4 ? run_rms_bwd<T, 1, 4, 512>(p, s, grid, lc) : run_rms_bwd<T, 1, 12, 512>(p, s, grid, lc);
-    return s.packs <= 8 ? run_rms_bwd<T, 1, 8, 1024>(p, s, grid, lc) : run_rms_bwd<T, 1, 16, 1024>(p, s, grid, lc);
-  } else {
-    if (s.threads == 256) return s.packs == 1 ? run_rms_bwd<T, VEC, 1, 256>(p, s, grid, lc) : run_rms_bwd<T, VEC, 2, 256>(p, s, grid, lc);
-    if (s.threads == 512) return run_rms_bwd<T, VEC, 2, 512>(p, s, grid, lc);
-    if constexpr (sizeof(T) == 4) { if (s.packs > 2) return run_rms_bwd<T, VEC, 4, 1024>(p, s, grid, lc); }
-    return run_rms_bwd<T, VEC, 2, 1024>(p, s, grid, lc);
+  if (s.threads == 256) return s.packs == 1 ? run_rms_bwd<T, 1, ALIGNED, 256>(p, s, grid, lc) : run_rms_bwd<T, 2, ALIGNED, 256>(p, s, grid, lc);
+  if (s.threads == 512) return run_rms_bwd<T, 2, ALIGNED, 512>(p, s, grid, lc);
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (!ALIGNED) { if (s.packs == 8) return run_rms_bwd<T, 8, ALIGNED, 1024>(p, s, grid, lc); }      // 4097 vectors
+    if (s.packs == 4) return run_rms_bwd<T, 4, ALIGNED, 1024>(p, s, grid, lc);
+  } else if constexpr (!ALIGNED) {
+    if (s.packs == 4) return run_rms_bwd<T, 4, ALIGNED, 1024>(p, s, grid, lc);                                   // 2049 vectors
   }
+  return run_rms_bwd<T, 2, ALIGNED, 1024>(p, s, grid, lc);
 }
 
 template <typename T>
@@ -511,13 +510,10 @@ cudaError_t rms_backward(const RmsParams& p, const LaunchCtx& lc) {
   constexpr uint32_t VEC = 16 / sizeof(S);
   RmsParams q = p;
   const bool aligned = p.cols % VEC == 0 && p.ld % VEC == 0;
-  const uint32_t vectors = aligned ? p.cols / VEC : p.cols;
-  RmsShape s = rms_shape(p.rows, vectors, aligned ? 2 : 8, lc.sm_count);
-  if (!aligned && s.log_tpr == 10 && vectors <= 512 * 12) { s.log_tpr = 9; s.threads = 512; }
-  s.packs = (int)((vectors + (1u << s.log_tpr) - 1) >> s.log_tpr);
+  const RmsShape s = rms_shape(p.rows, aligned ? p.cols / VEC : (p.cols + 2 * VEC - 2) / VEC, 2, lc.sm_count);
   q.log_tpr = s.log_tpr;
   unsigned grid = 0;
-  cudaError_t e = aligned ? run_rms_bwd_packs<T, (int)VEC>(q, s, &grid, lc) : run_rms_bwd_packs<T, 1>(q, s, &grid, lc);
+  cudaError_t e = aligned ? run_rms_bwd_packs<T, true>(q, s, &grid, lc) : run_rms_bwd_packs<T, false>(q, s, &grid, lc);
   if (e == cudaSuccess && p.weight_on)
     e = launch_pdl(rmsnorm_dweight_kernel<T>, dim3((p.cols + 31) / 32), 1024, 0, lc.stream, (const float*)q.partial, grid, p.cols, (S*)q.dweight, q.rn);
   return e;
