@@ -290,8 +290,8 @@ typedef struct {
   int32_t  dtype;        /* table, out, dout, dtable: bf16 / f16 / f32 */
   int32_t  id_dtype;     /* ZYXB_I32 or ZYXB_I64 */
   uint64_t tokens, vocab, dim;   /* each below 2^31 */
-  uint64_t ld_table, ld_out;     /* row pitch of table / dtable and of out / dout in elements; 0 = dim.  What lies between dim and
-                                    the pitch is neither read nor written */
+  uint64_t ld_table, ld_out;     /* row pitch of table / dtable and of out / dout in elements; 0 = dim.  What lies between the rows
+                                    is not written */
   float    scale;        /* 0 means 1 */
   int32_t  accumulate;   /* EMBEDDING_BWD only */
 } zyxb_embedding_desc;

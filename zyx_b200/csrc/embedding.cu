@@ -2,7 +2,9 @@
 //   out[i,:]    = scale * table[ids[i],:]                      (zeros for an id outside [0, vocab))
 //   dtable[v,:] = scale * sum_{i : ids[i] = v} dout[i,:]       (+ dtable[v,:])
 //
-// Lookup: a copy, bound by HBM.  A group of threads spans one row's 16-byte vectors and moves four tokens at a time.
+// Lookup: a copy, bound by HBM.  A group of threads spans one row's 16-byte vectors and moves four tokens at a time.  Where rows do
+// not start on vector boundaries (an odd width or pitch), vectors are aligned to the row that is written and shifted out of the
+// two they lie in where they are read.
 //
 // Gradient, three launches and no floating-point atomic:
 //   index    The vocabulary is cut into ranges, one CTA each.  Every CTA scans all token numbers (from L2; 64 KB at 16384 tokens),
@@ -33,40 +35,108 @@ constexpr int FILL_ROWS = 64;          // table rows that a CTA of the sum launc
 
 template <typename ID> __device__ __forceinline__ int64_t id_at(const ID* ids, uint64_t i) { return (int64_t)ids[i]; }
 
-template <typename T, typename ID, int VEC>
+template <typename T> constexpr int emb_vec() { return 16 / (int)sizeof(typename Elem<T>::store_t); }
+
+// entries [from, to) of a vector, one by one
+template <typename T>
+__device__ __forceinline__ void emb_store_some(typename Elem<T>::store_t* at, const RawVec<T, emb_vec<T>()>& r, int from, int to) {
+#pragma unroll
+  for (int k = 0; k < emb_vec<T>(); ++k)
+    if (k >= from && k < to) {
+      if constexpr (sizeof(typename Elem<T>::store_t) == 2) at[k] = (uint16_t)(r.w[k / 2] >> (16 * (k & 1)));
+      else at[k] = __uint_as_float(r.w[k]);
+    }
+}
+
+// VEC values of a row from column c on (may be negative) to memory: as a vector where all of them are the row's, which then starts on
+// a boundary, and one by one at its ends
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void emb_store(typename Elem<T>::store_t* row, int64_t c, uint32_t dim, const RawVec<T, emb_vec<T>()>& r) {
+  constexpr int VEC = emb_vec<T>();
+  if constexpr (ALIGNED) r.store_stream(row + c);
+  else if (c >= 0 && c + VEC <= (int64_t)dim) r.store_stream(row + c);
+  else emb_store_some<T>(row + c, r, (int)max((int64_t)0, -c), (int)min((int64_t)VEC, (int64_t)dim - c));
+}
+
+// A row that starts `off` elements behind a vector boundary (-1: take no notice of boundaries), from the vectors at multiples of VEC columns that neighbouring lanes hold:
+// each lane stores the aligned vector that ends in its own, the first and the last lane their ends one by one.  `active`: lanes of
+// the warp that hold a vector (all of its lanes take part where off is not 0).  Not inlined: five copies of it in the sum kernel's loop
+// did not fit the instruction cache.
+template <typename T>
+__device__ __noinline__ void emb_store_row(typename Elem<T>::store_t* row, uint32_t col, uint32_t dim, int off, uint4 v, int active) {
+  constexpr int VEC = emb_vec<T>();
+  RawVec<T, VEC> r;
+  r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+  const int mine = min(VEC, (int)(dim - col));
+  if (off <= 0) {
+    if (off == 0 && mine == VEC) r.store_stream(row + col);
+    else emb_store_some<T>(row + col, r, 0, mine);
+    return;
+  }
+  const uint32_t mask = active == 32 ? 0xffffffffu : (1u << active) - 1u;
+  const int lane = threadIdx.x & 31;
+  uint32_t w[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { w[j] = __shfl_up_sync(mask, r.w[j], 1); w[4 + j] = r.w[j]; }
+  if (lane > 0 && mine >= VEC - off) {
+    RawVec<T, VEC> out;
+    shift_vector<T, VEC>(out, w, VEC - off);
+    out.store_stream(row + col - off);
+  } else {
+    if (lane > 0) {                       // the row ends inside this vector: the neighbour's end, then this lane's
+      RawVec<T, VEC> before;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) before.w[j] = w[j];
+      emb_store_some<T>(row + col - VEC, before, VEC - off, VEC);
+    }
+    emb_store_some<T>(row + col, r, 0, min(mine, VEC - off));
+  }
+  if (lane == active - 1) emb_store_some<T>(row + col, r, VEC - off, mine);
+}
+
+template <typename T, typename ID, bool ALIGNED>
 __global__ void __launch_bounds__(EMB_THREADS)
 embedding_kernel(const ID* __restrict__ ids, const typename Elem<T>::store_t* __restrict__ table, typename Elem<T>::store_t* __restrict__ out,
-                 uint32_t tokens, uint64_t vocab, uint32_t packs, int log_tpt, uint64_t ld_table, uint64_t ld_out, float scale, int rn) {
+                 uint32_t tokens, uint64_t vocab, uint32_t dim, uint32_t packs, int log_tpt, uint64_t ld_table, uint64_t ld_out, float scale, int rn) {
+  constexpr int VEC = emb_vec<T>();
   const uint32_t tpt = 1u << log_tpt, group = threadIdx.x >> log_tpt, groups = EMB_THREADS >> log_tpt;
   const uint32_t pack = blockIdx.y * tpt + (threadIdx.x & (tpt - 1));
   pdl_trigger();
   pdl_wait();
   if (pack >= packs) return;
   const uint64_t first = (uint64_t)blockIdx.x * groups * EMB_TOKENS + group;
+  // the first column of this thread's vector: vectors are aligned to the row written
+  auto col = [&](uint64_t i) { return (int64_t)pack * VEC - (ALIGNED ? 0 : (int64_t)(i * ld_out % VEC)); };
   int64_t id[EMB_TOKENS];
 #pragma unroll
   for (int u = 0; u < EMB_TOKENS; ++u) {
     const uint64_t i = first + (uint64_t)u * groups;
     id[u] = i < tokens ? id_at(ids, i) : -1;
   }
-  RawVec<T, VEC> r[EMB_TOKENS];
+  std::conditional_t<ALIGNED, RawVec<T, VEC>, Shifted<T, VEC>> from[EMB_TOKENS];
 #pragma unroll
   for (int u = 0; u < EMB_TOKENS; ++u) {
-    r[u].zero();
-    if (id[u] >= 0 && (uint64_t)id[u] < vocab) r[u].load(table + (uint64_t)id[u] * ld_table + (uint64_t)pack * VEC);
+    from[u].zero();
+    if (id[u] >= 0 && (uint64_t)id[u] < vocab) {
+      if constexpr (ALIGNED) from[u].load(table + (uint64_t)id[u] * ld_table + (uint64_t)pack * VEC);
+      else from[u].load(table, id[u] * (int64_t)ld_table + col(first + (uint64_t)u * groups), (vocab - 1) * ld_table + dim);
+    }
   }
 #pragma unroll
   for (int u = 0; u < EMB_TOKENS; ++u) {
     const uint64_t i = first + (uint64_t)u * groups;
-    if (i >= tokens) continue;
+    if (i >= tokens || col(i) >= (int64_t)dim) continue;
+    RawVec<T, VEC> r;
+    if constexpr (ALIGNED) r = from[u];
+    else from[u].get(r);
     if (scale != 1.0f) {
       float v[VEC];
-      r[u].decode(v);
+      r.decode(v);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) v[k] *= scale;
-      round_encode<T, VEC>(r[u], v, rn != 0);
+      round_encode<T, VEC>(r, v, rn != 0);
     }
-    r[u].store_stream(out + i * ld_out + (uint64_t)pack * VEC);
+    emb_store<T, ALIGNED>(out + i * ld_out, col(i), dim, r);
   }
 }
 
@@ -185,15 +255,15 @@ struct EmbGradParams {
   const SortedToken* sorted;
   const uint32_t* starts;      // [vocab + 1]
   float* partial;              // [chunk][2][dim]: 0 the shared run that came in from the chunk before, 1 the one that begins here
-  uint32_t vocab, dim, packs, chunk, chunks, sum_ctas;
+  uint32_t tokens, vocab, dim, packs, chunk, chunks, sum_ctas;
   uint64_t ld_table, ld_out;
   float scale;
   int accumulate, rn;
 };
 
-// scale * acc (+ what the row held) to the table
+// scale * acc (+ what the row held), rounded
 template <typename T, int VEC>
-__device__ __forceinline__ void emb_store_row(typename Elem<T>::store_t* dst, float (&acc)[VEC], const RawVec<T, VEC>& held, const EmbGradParams& p) {
+__device__ __forceinline__ void emb_finish(RawVec<T, VEC>& r, float (&acc)[VEC], const RawVec<T, VEC>& held, const EmbGradParams& p) {
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] *= p.scale;
   if (p.accumulate) {
@@ -202,18 +272,16 @@ __device__ __forceinline__ void emb_store_row(typename Elem<T>::store_t* dst, fl
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] += old[k];
   }
-  RawVec<T, VEC> r;
   round_encode<T, VEC>(r, acc, p.rn != 0);
-  r.store_stream(dst);
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(EMB_THREADS, 4)
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(EMB_THREADS, ALIGNED ? 4 : 3)
 embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typename Elem<T>::store_t* dtable, const EmbGradParams p, int log_tpt) {
-  constexpr int U = VEC >= 4 ? 4 : 8;     // rows in flight per thread; four CTAs per SM
+  constexpr int VEC = emb_vec<T>(), U = 4;                    // rows in flight per thread; four CTAs per SM (three where a row is two vectors)
   const uint32_t tpt = 1u << log_tpt, groups = EMB_THREADS >> log_tpt, group = threadIdx.x >> log_tpt;
   const uint32_t pack = blockIdx.y * tpt + (threadIdx.x & (tpt - 1));
-  const uint64_t col = (uint64_t)pack * VEC;
+  const uint32_t col = pack * VEC;
   pdl_trigger();
   pdl_wait();
   if (pack >= p.packs) return;
@@ -223,7 +291,12 @@ embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typenam
     z.zero();
 #pragma unroll 4
     for (uint32_t r = r0 + group; r < min(p.vocab, r0 + FILL_ROWS); r += groups)
-      if (p.starts[r] == p.starts[r + 1]) z.store_stream(dtable + (uint64_t)r * p.ld_table + col);
+      if (p.starts[r] == p.starts[r + 1]) {
+        auto* row = dtable + (uint64_t)r * p.ld_table;
+        const int off = ALIGNED ? 0 : (int)((uint64_t)r * p.ld_table % VEC);
+        if (ALIGNED || (int64_t)col - off < (int64_t)p.dim) emb_store<T, ALIGNED>(row, (int64_t)col - off, p.dim, z);
+        if (!ALIGNED && pack + 1 == p.packs && (int64_t)col + VEC - off < (int64_t)p.dim) emb_store<T, false>(row, (int64_t)col + VEC - off, p.dim, z);
+      }
     return;
   }
   const uint32_t c = blockIdx.x * groups + group;
@@ -236,17 +309,38 @@ embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typenam
   const uint32_t lo = head.token & (FIRST | SHARED) ? begin : p.starts[head.row + 1];
   const uint32_t hi = tail.token & SHARED ? end : p.starts[tail.row + 1];
   if (lo >= hi) return;
+  // entries behind the row (the last vector of an odd width) are summed with the others and not stored
+  const uint64_t dout_end = ((uint64_t)p.tokens - 1) * p.ld_out + p.dim, table_end = ((uint64_t)p.vocab - 1) * p.ld_table + p.dim;
+  using Loaded = std::conditional_t<ALIGNED, RawVec<T, VEC>, Shifted<T, VEC>>;
+  auto fetch = [&](Loaded& r, const typename Elem<T>::store_t* from, uint64_t at, uint64_t last) {
+    if constexpr (ALIGNED) r.load_stream(from + at);
+    else r.load(from, (int64_t)at, last);
+  };
+  auto vector = [&](const Loaded& l) {
+    RawVec<T, VEC> r;
+    if constexpr (ALIGNED) r = l;
+    else l.get(r);
+    return r;
+  };
+  const int active = (int)min(32u, p.packs - (pack & ~31u));      // lanes of this warp that hold a vector (one group per warp)
   float acc[VEC];
   uint32_t row = 0, slot = (head.token & FIRST) || lo != begin ? 1 : 0;
   bool shared = false;
-  RawVec<T, VEC> held;                    // accumulate: the row as it was, loaded when its run begins
+  Loaded held;                            // accumulate: the row as it was, loaded when its run begins
+  held.zero();
   auto flush = [&] {
     if (shared) {
       float* part = p.partial + ((uint64_t)c * 2 + slot) * p.dim + col;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) part[k] = acc[k];
+      for (int k = 0; k < VEC; ++k)
+        if (ALIGNED || col + k < p.dim) part[k] = acc[k];
     } else {
-      emb_store_row<T, VEC>(dtable + (uint64_t)row * p.ld_table + col, acc, held, p);
+      RawVec<T, VEC> r;
+      emb_finish<T, VEC>(r, acc, vector(held), p);
+      auto* to = dtable + (uint64_t)row * p.ld_table;
+      if (ALIGNED) r.store_stream(to + col);
+      else if (log_tpt >= 5) emb_store_row<T>(to, col, p.dim, (int)((uint64_t)row * p.ld_table % VEC), make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]), active);
+      else emb_store_row<T>(to, col, p.dim, -1, make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]), 0);       // several runs in a warp
     }
     slot = 1;
   };
@@ -254,24 +348,24 @@ embedding_sum_kernel(const typename Elem<T>::store_t* __restrict__ dout, typenam
 #pragma unroll
   for (int u = 0; u < U; ++u) s[u] = p.sorted[min(lo + u, hi - 1)];
   for (uint32_t i = lo; i < hi; i += U) {
-    RawVec<T, VEC> r[U];
+    Loaded r[U];
     SortedToken next[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i + u < hi) r[u].load_stream(dout + (uint64_t)(s[u].token & TOKEN) * p.ld_out + col);
+      if (i + u < hi) fetch(r[u], dout, (uint64_t)(s[u].token & TOKEN) * p.ld_out + col, dout_end);
 #pragma unroll
     for (int u = 0; u < U; ++u) next[u] = p.sorted[min(i + U + u, hi - 1)];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u < hi) {
         float v[VEC];
-        r[u].decode(v);
+        vector(r[u]).decode(v);
         const bool starts_run = (s[u].token & FIRST) || i + u == lo;
         if (starts_run) {
           if (i + u != lo) flush();
           row = s[u].row;
           shared = s[u].token & SHARED;
-          if (p.accumulate && !shared) held.load(dtable + (uint64_t)row * p.ld_table + col);
+          if (p.accumulate && !shared) fetch(held, dtable, (uint64_t)row * p.ld_table + col, table_end);
         }
 #pragma unroll
         for (int k = 0; k < VEC; ++k) acc[k] = starts_run ? v[k] : acc[k] + v[k];
@@ -327,21 +421,23 @@ embedding_combine_kernel(typename Elem<T>::store_t* dtable, const EmbGradParams 
 #pragma unroll
       for (int w = 0; w < CMB_WARPS; ++w) acc[0] += part[w][threadIdx.x];
       auto* dst = dtable + (uint64_t)row * p.ld_table + col;
-      RawVec<T, 1> held;
+      RawVec<T, 1> held, r;
       held.zero();
       if (p.accumulate) held.load(dst);
-      emb_store_row<T, 1>(dst, acc, held, p);
+      emb_finish<T, 1>(r, acc, held, p);
+      r.store(dst);
     }
     __syncthreads();
   }
 }
 
-// the widest vector (in elements) that every row of both matrices can be cut into
-uint32_t emb_vec(const zyxb_embedding_desc& d, uint64_t ld_table, uint64_t ld_out) {
-  const uint64_t all = d.dim | ld_table | ld_out;
-  uint32_t v = (uint32_t)(16 / dtype_size(d.dtype));
-  while (v > 1 && all % v) v >>= 1;
-  return v;
+// whether every row of both matrices starts on a vector boundary and ends on one
+bool emb_aligned(const zyxb_embedding_desc& d, uint64_t ld_table, uint64_t ld_out) {
+  return ((d.dim | ld_table | ld_out) * dtype_size(d.dtype)) % 16 == 0;
+}
+uint32_t emb_packs(const zyxb_embedding_desc& d) {
+  const uint64_t vec = 16 / dtype_size(d.dtype);
+  return (uint32_t)((d.dim + vec - 1) / vec);
 }
 
 int log2_ceil(uint64_t v, int most) {
@@ -355,26 +451,26 @@ bool matrix_fits(uint64_t rows, uint64_t ld, uint64_t dim, uint64_t es, uint64_t
   return (unsigned __int128)es * ((unsigned __int128)(rows - 1) * ld + dim) <= bytes;
 }
 
-template <typename T, typename ID, int VEC>
+template <typename T, typename ID, bool ALIGNED>
 cudaError_t run_embedding(const zyxb_embedding_desc& d, uint64_t ldt, uint64_t ldo, float scale, void* const* args, const LaunchCtx& lc) {
   using S = typename Elem<T>::store_t;
-  const uint32_t packs = (uint32_t)(d.dim / VEC);
+  const uint32_t packs = emb_packs(d) + (ALIGNED ? 0 : 1);          // a row of odd start touches one more
   const int log_tpt = log2_ceil(packs, 8);
   const uint64_t per_cta = (uint64_t)(EMB_THREADS >> log_tpt) * EMB_TOKENS;
   const dim3 grid((unsigned)((d.tokens + per_cta - 1) / per_cta), (unsigned)((packs + (1u << log_tpt) - 1) >> log_tpt));
-  return launch_pdl(embedding_kernel<T, ID, VEC>, grid, EMB_THREADS, 0, lc.stream, (const ID*)args[0], (const S*)args[1], (S*)args[2], (uint32_t)d.tokens,
-                    d.vocab, packs, log_tpt, ldt, ldo, scale, lc.round_nearest ? 1 : 0);
+  return launch_pdl(embedding_kernel<T, ID, ALIGNED>, grid, EMB_THREADS, 0, lc.stream, (const ID*)args[0], (const S*)args[1], (S*)args[2], (uint32_t)d.tokens,
+                    d.vocab, (uint32_t)d.dim, packs, log_tpt, ldt, ldo, scale, lc.round_nearest ? 1 : 0);
 }
 
 struct EmbPlan { uint32_t range, ranges, chunk, chunks; uint64_t starts_off, partial_off; };
 
-template <typename T, typename ID, int VEC>
+template <typename T, typename ID, bool ALIGNED>
 cudaError_t run_embedding_bwd(const zyxb_embedding_desc& d, uint64_t ldt, uint64_t ldo, float scale, const EmbPlan& pl, void* const* args, const LaunchCtx& lc) {
   using S = typename Elem<T>::store_t;
   char* scratch = (char*)lc.scratch;
   EmbGradParams p{};
   p.sorted = (const SortedToken*)scratch; p.starts = (const uint32_t*)(scratch + pl.starts_off); p.partial = (float*)(scratch + pl.partial_off);
-  p.vocab = (uint32_t)d.vocab; p.dim = (uint32_t)d.dim; p.packs = (uint32_t)(d.dim / VEC); p.chunk = pl.chunk;
+  p.tokens = (uint32_t)d.tokens; p.vocab = (uint32_t)d.vocab; p.dim = (uint32_t)d.dim; p.packs = emb_packs(d); p.chunk = pl.chunk;
   p.ld_table = ldt; p.ld_out = ldo; p.scale = scale; p.accumulate = d.accumulate ? 1 : 0; p.rn = lc.round_nearest ? 1 : 0;
   p.chunks = pl.chunks;
   static uint64_t configured = 0;
@@ -388,7 +484,7 @@ cudaError_t run_embedding_bwd(const zyxb_embedding_desc& d, uint64_t ldt, uint64
   p.sum_ctas = (pl.chunks + groups - 1) / groups;
   const unsigned fill = p.accumulate ? 0 : (p.vocab + FILL_ROWS - 1) / FILL_ROWS;
   const dim3 grid(p.sum_ctas + fill, (unsigned)((p.packs + (1u << log_tpt) - 1) >> log_tpt));
-  e = launch_pdl(embedding_sum_kernel<T, VEC>, grid, EMB_THREADS, 0, lc.stream, (const S*)args[1], (S*)args[2], p, log_tpt);
+  e = launch_pdl(embedding_sum_kernel<T, ALIGNED>, grid, EMB_THREADS, 0, lc.stream, (const S*)args[1], (S*)args[2], p, log_tpt);
   if (e != cudaSuccess || d.tokens <= 2 * pl.chunk) return e;
   return launch_pdl(embedding_combine_kernel<T>, dim3((pl.chunks + CMB_WARPS - 1) / CMB_WARPS, (unsigned)((d.dim + CMB_COLS - 1) / CMB_COLS)), CMB_WARPS * 32, 0,
                     lc.stream, (S*)args[2], p);
@@ -410,15 +506,9 @@ int validate_embedding(const zyxb_embedding_desc& d, bool backward, std::string&
   return ZYXB_OK;
 }
 
-#define ZYXB_EMB_VEC(T, ID, F)                                                    \
-  switch (vec) {                                                                  \
-    case 8: if constexpr (sizeof(typename Elem<T>::store_t) == 2) { F(T, ID, 8); } break; \
-    case 4: F(T, ID, 4); break;                                                   \
-    case 2: F(T, ID, 2); break;                                                   \
-    default: F(T, ID, 1); break;                                                  \
-  }
-#define ZYXB_EMB_ID(T, F)                                                         \
-  if (d.id_dtype == ZYXB_I32) { ZYXB_EMB_VEC(T, int32_t, F) } else { ZYXB_EMB_VEC(T, int64_t, F) }
+#define ZYXB_EMB_ID(T, F)                                                                    \
+  if (d.id_dtype == ZYXB_I32) { if (aligned) { F(T, int32_t, true); } else { F(T, int32_t, false); } } \
+  else { if (aligned) { F(T, int64_t, true); } else { F(T, int64_t, false); } }
 #define ZYXB_EMB_DISPATCH(F)                                                      \
   switch (d.dtype) {                                                              \
     case ZYXB_F32: ZYXB_EMB_ID(float, F) break;                                   \
@@ -434,7 +524,7 @@ int launch_embedding(const zyxb_embedding_desc& d, void* const* args, const uint
   ZYXB_CHECK_ARG(matrix_fits(d.tokens, ldo, d.dim, es, arg_bytes[2]), "embedding: out too small");
   ZYXB_CHECK_ARG(args[2] != args[1] && args[2] != args[0], "embedding: out must be a buffer of its own");
   const float scale = d.scale == 0.0f ? 1.0f : d.scale;
-  const uint32_t vec = emb_vec(d, ldt, ldo);
+  const bool aligned = emb_aligned(d, ldt, ldo);
   cudaError_t e = cudaSuccess;
 #define ZYXB_EMB_FWD(T, ID, V) e = run_embedding<T, ID, V>(d, ldt, ldo, scale, args, lc)
   ZYXB_EMB_DISPATCH(ZYXB_EMB_FWD)
@@ -458,8 +548,8 @@ int launch_embedding_bwd(const zyxb_embedding_desc& d, void* const* args, const 
   pl.partial_off = pl.starts_off + ((d.vocab + 1) * 4 + 255) / 256 * 256;
   // few tokens: shorter chunks, so that every SM has three CTAs' worth of them (4099 tokens of 777 f32: 24 -> 22 us; at 16384 of 2048
   // bf16, which 32 places fill, chunks of 8 cost more partials than they save: 61 -> 68 us)
-  const uint32_t vec = emb_vec(d, ldt, ldo);
-  const uint64_t threads_wide = (d.dim / vec + 31) / 32 * 32;
+  const bool aligned = emb_aligned(d, ldt, ldo);
+  const uint64_t threads_wide = (emb_packs(d) + 31) / 32 * 32;
   pl.chunk = CHUNK;
   auto chunks = [&] { return (d.tokens + pl.chunk - 1) / pl.chunk; };
   while (pl.chunk > CHUNK_LEAST && chunks() * threads_wide < (uint64_t)lc.sm_count * 3 * EMB_THREADS) pl.chunk /= 2;

@@ -4,7 +4,7 @@
 //     dx = rstd * dy w - h * rstd^3 * P / cols (+ dh),   dw = sum over rows of dy h rstd
 // Bound by HBM: every element is read once, kept in registers between the sum and the store, and written once.
 //
-// A group of `tpr` threads (a power of two, 8..1024) holds one row as 16-byte vectors, PACKS per thread.  Rows whose start is not
+// A group of `tpr` threads (8, 16 .. 128, or any multiple of 32 up to 1024) holds one row as 16-byte vectors, PACKS per thread.  Rows whose start is not
 // on a 16-byte boundary (odd pitches) are covered by the aligned vectors that contain them: vectors inside the row move as a
 // whole, the two that hang over its ends element by element.  Sums are f32.
 #include <algorithm>
@@ -22,15 +22,16 @@ struct RmsParams {
   const void *x, *residual, *weight, *dy, *dh;
   void *h, *y, *dweight;
   float *scales, *partial;
-  uint64_t rows, ld;
+  uint64_t rows, ld, end;      // end: elements up to the last row's last
   uint32_t cols, group, n_groups;
   float eps, inv_cols;
-  int log_tpr, rn, residual_on, weight_on, dh_on;
+  int log_tpr, tpr, groups;    // threads per row; rows per CTA.  One row: any multiple of 32 threads, log_tpr is 10
+  int rn, residual_on, weight_on, dh_on;
 };
 
 // Sum over a row's threads of up to two values.  `parity` alternates between calls, so one barrier per call is enough.
 template <int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], int log_tpr, float (*buf)[32][N], int parity) {
+__device__ __forceinline__ void row_sum(float (&v)[N], int log_tpr, int wpr, float (*buf)[32][N], int parity) {
   if (log_tpr >= 5) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -44,13 +45,13 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int log_tpr, float (*buf)
     }
   }
   if (log_tpr > 5) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wpr = 1 << (log_tpr - 5);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) buf[parity][warp][i] = v[i];
     }
     __syncthreads();
-    const int first = warp & ~(wpr - 1);
+    const int first = warp & ~((1 << (log_tpr - 5)) - 1);
     float s[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = 0.0f;
@@ -80,14 +81,24 @@ struct RowView {
   __device__ __forceinline__ int col(int pack) const { return pack * VEC - off; }                 // may be negative
   __device__ __forceinline__ bool whole(int pack) const { return ALIGNED || (col(pack) >= 0 && col(pack) + VEC <= cols); }
   __device__ __forceinline__ bool inside(int c) const { return ALIGNED || ((unsigned)c < (unsigned)cols); }
-  // zeros outside the row
-  __device__ __forceinline__ void load(RawVec<T, VEC>& r, const void* base, int pack) const {
+  // Whole vectors wherever the buffer (of `end` elements) has them: what lies outside the row is dropped by mask(), which the caller
+  // applies when it needs the values and not when it starts the load.
+  __device__ __forceinline__ void load(RawVec<T, VEC>& r, const void* base, int pack, uint64_t end) const {
     const S* p = reinterpret_cast<const S*>(base) + start + (uint64_t)pack * VEC;
-    if (whole(pack)) { r.load_stream(p); return; }
+    if (ALIGNED || start + (uint64_t)pack * VEC + VEC <= end) { r.load_stream(p); return; }
     float v[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) v[k] = inside(col(pack) + k) ? Elem<T>::load(p[k]) : 0.0f;
     round_encode<T, VEC>(r, v, true);          // exact: the values are of the storage type
+  }
+  __device__ __forceinline__ void mask(RawVec<T, VEC>& r, int pack) const {
+    if (ALIGNED || whole(pack)) return;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      if (!inside(col(pack) + k)) {
+        if constexpr (sizeof(S) == 2) r.w[k / 2] &= k & 1 ? 0x0000ffffu : 0xffff0000u;
+        else r.w[k] = 0u;
+      }
   }
   __device__ __forceinline__ void store(const typename Nums<VEC>::V (&n)[Nums<VEC>::N], void* base, int pack, bool rn) const {
     S* p = reinterpret_cast<S*>(base) + start + (uint64_t)pack * VEC;
@@ -107,14 +118,8 @@ struct RowView {
   __device__ __forceinline__ void weight(typename Nums<VEC>::V (&n)[Nums<VEC>::N], const void* w, int pack) const {
     const S* p = reinterpret_cast<const S*>(w);
     RawVec<T, VEC> r;
-    if constexpr (ALIGNED) {
-      r.load(p + pack * VEC);
-    } else {
-      float v[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = inside(col(pack) + k) ? Elem<T>::load(p[col(pack) + k]) : 0.0f;
-      round_encode<T, VEC>(r, v, true);
-    }
+    if constexpr (ALIGNED) r.load(p + pack * VEC);
+    else load_shifted<T, VEC>(r, p, col(pack), (uint64_t)cols);
     Nums<VEC>::decode(n, r);
   }
 };
@@ -126,6 +131,14 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 }
 
 constexpr float E4M3_MAX = 448.0f, AMAX_FLOOR = 1e-30f;
+
+// 448 / largest: what y is multiplied by.  The reciprocal is the approximate one (1 ulp): a value next to the border between two 8-bit
+// floats may go to either, as it may by the f32 rounding of y itself.
+__device__ __forceinline__ float e4m3_factor(float amax) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(amax));
+  return r * E4M3_MAX;
+}
 
 // a vector of y as 8-bit floats; scale_of(column): the reciprocal of its scale
 template <typename T, bool ALIGNED, class F>
@@ -139,7 +152,7 @@ __device__ __forceinline__ void put_e4m3(const RowView<T, ALIGNED>& view, const 
   uint32_t w[VEC / 4];
 #pragma unroll
   for (int k = 0; k < VEC / 4; ++k) w[k] = e4m3x2(q[4 * k], q[4 * k + 1]) | (e4m3x2(q[4 * k + 2], q[4 * k + 3]) << 16);
-  if (ALIGNED) {
+  if (ALIGNED || (view.whole(pack) && (row * p.cols + c0) % VEC == 0)) {       // a dense x and the dense y have the same vector boundaries
     if constexpr (VEC == 8) __stcs(reinterpret_cast<uint2*>(out + c0), make_uint2(w[0], w[1]));
     else __stcs(reinterpret_cast<uint32_t*>(out + c0), w[0]);
   } else {
@@ -171,8 +184,8 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsParams p) {
   using Num = Nums<VEC>;
   __shared__ float red[1][32][1];
   extern __shared__ uint32_t amax_bits[];            // QUANT_SHARED: largest |y| of each column group, per row of the CTA, as its bits
-  const int tpr = 1 << p.log_tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & (tpr - 1);
-  const uint64_t row = (uint64_t)blockIdx.x * (blockDim.x >> p.log_tpr) + in_cta;
+  const int tpr = p.tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & ((1 << p.log_tpr) - 1);
+  const uint64_t row = (uint64_t)blockIdx.x * p.groups + in_cta;
   const bool live = row < p.rows;
   const View view(live ? row : 0, p.ld, p.cols);
   pdl_trigger();
@@ -185,15 +198,17 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsParams p) {
       const int pack = t + i * tpr;
       rx[i].zero(); rr[i].zero();
       if (live && view.has(pack)) {
-        view.load(rx[i], p.x, pack);
-        if (p.residual_on) view.load(rr[i], p.residual, pack);
+        view.load(rx[i], p.x, pack, p.end);
+        if (p.residual_on) view.load(rr[i], p.residual, pack, p.end);
       }
     }
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int pack = t + i * tpr;
+      view.mask(rx[i], pack);
       Num::decode(v[i], rx[i]);
       if (p.residual_on) {
+        view.mask(rr[i], pack);
         typename Num::V r[Num::N];
         Num::decode(r, rr[i]);
 #pragma unroll
@@ -205,11 +220,11 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsParams p) {
     }
   }
   if constexpr (QUANT == QUANT_SHARED) {
-    for (uint32_t g = threadIdx.x; g < (blockDim.x >> p.log_tpr) * p.n_groups; g += blockDim.x) amax_bits[g] = __float_as_uint(AMAX_FLOOR);
+    for (uint32_t g = threadIdx.x; g < (uint32_t)p.groups * p.n_groups; g += blockDim.x) amax_bits[g] = __float_as_uint(AMAX_FLOOR);
     if (p.log_tpr <= 5) __syncthreads();             // wider rows pass a barrier in row_sum
   }
   float sum[1] = {Num::sum(sq)};
-  row_sum(sum, p.log_tpr, red, 0);
+  row_sum(sum, p.log_tpr, p.tpr >> 5, red, 0);
   const float rstd = rsqrtf(sum[0] * p.inv_cols + p.eps);
   float h[PACKS][VEC];
 #pragma unroll
@@ -241,7 +256,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsParams p) {
       }
       for (int o = width >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       if (!in) continue;
-      const float scale = m / E4M3_MAX, inv = 1.0f / scale;
+      const float scale = m * (1.0f / E4M3_MAX), inv = e4m3_factor(m);
       put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int) { return inv; });
       if (pack % width == 0) p.scales[row * p.n_groups + pack / width] = scale;
     }
@@ -278,14 +293,17 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_kernel(const RmsParams p) {
       }
     }
     __syncthreads();
+    if (live)
+      for (uint32_t g = t; g < p.n_groups; g += tpr) p.scales[row * p.n_groups + g] = __uint_as_float(mine[g]) * (1.0f / E4M3_MAX);
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
       const int pack = t + i * tpr;
       if (!live || !view.has(pack)) continue;
-      put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int c) { return 1.0f / (__uint_as_float(mine[p.n_groups == 1 ? 0 : (uint32_t)min(max(c, 0), (int)p.cols - 1) / p.group]) / E4M3_MAX); });
+      uint32_t g0 = 0, border = p.cols;
+      if (p.n_groups > 1) { g0 = (uint32_t)max(0, view.col(pack)) / p.group; border = (g0 + 1) * p.group; }
+      const float s0 = e4m3_factor(__uint_as_float(mine[g0])), s1 = border < min(p.cols, (uint32_t)(view.col(pack) + VEC)) ? e4m3_factor(__uint_as_float(mine[g0 + 1])) : s0;
+      put_e4m3<T, ALIGNED>(view, h[i], p, row, pack, [&](int c) { return c < (int)border ? s0 : s1; });
     }
-    if (live)
-      for (uint32_t g = t; g < p.n_groups; g += tpr) p.scales[row * p.n_groups + g] = __uint_as_float(mine[g]) / E4M3_MAX;
   }
 }
 
@@ -301,18 +319,24 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_bwd_kernel(const RmsParams p)
   constexpr int N = Num::N;
   __shared__ float red[2][32][2];
   extern __shared__ float dw_shared[];               // [group of the CTA][cols]
-  const int tpr = 1 << p.log_tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & (tpr - 1), groups = blockDim.x >> p.log_tpr;
+  const int tpr = p.tpr, in_cta = threadIdx.x >> p.log_tpr, t = threadIdx.x & ((1 << p.log_tpr) - 1), groups = p.groups;
   const uint64_t step = (uint64_t)gridDim.x * groups;
   const View first((uint64_t)blockIdx.x * groups + in_cta, p.ld, p.cols);        // stands for all rows where only the place in a vector counts
-  V w[PACKS][N], dw[PACKS][N];
+  // 1024 threads have 64 registers each: no room for the weights and a second row
+  constexpr bool LEAN = THREADS > 512;
+  V w[LEAN ? 1 : PACKS][N], dw[PACKS][N];
+  auto weight = [&](V (&to)[N], int pack) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) to[k] = Num::splat(1.0f);
+    if (p.weight_on && first.has(pack)) first.weight(to, p.weight, pack);
+  };
   pdl_trigger();
   pdl_wait();
 #pragma unroll
   for (int i = 0; i < PACKS; ++i) {
-    const int pack = t + i * tpr;
+    if constexpr (!LEAN) weight(w[i], t + i * tpr);
 #pragma unroll
-    for (int k = 0; k < N; ++k) { w[i][k] = Num::splat(1.0f); dw[i][k] = Num::splat(0.0f); }
-    if (p.weight_on && first.has(pack)) first.weight(w[i], p.weight, pack);
+    for (int k = 0; k < N; ++k) dw[i][k] = Num::splat(0.0f);
   }
   struct Row { RawVec<T, VEC> h[PACKS], g[PACKS], d[PACKS]; };
   auto fetch = [&](Row& r, uint64_t row) {
@@ -322,9 +346,9 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_bwd_kernel(const RmsParams p)
       const int pack = t + i * tpr;
       r.h[i].zero(); r.g[i].zero(); r.d[i].zero();
       if (row < p.rows && view.has(pack)) {
-        view.load(r.h[i], p.h, pack);
-        view.load(r.g[i], p.dy, pack);
-        if (p.dh_on) view.load(r.d[i], p.dh, pack);
+        view.load(r.h[i], p.h, pack, p.end);
+        view.load(r.g[i], p.dy, pack, p.end);
+        if (p.dh_on) view.load(r.d[i], p.dh, pack, p.end);
       }
     }
   };
@@ -333,41 +357,52 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_bwd_kernel(const RmsParams p)
   fetch(now, (uint64_t)blockIdx.x * groups + in_cta);
   for (uint64_t row0 = (uint64_t)blockIdx.x * groups; row0 < p.rows; row0 += step, parity ^= 1) {
     const uint64_t row = row0 + in_cta;
-    V h[PACKS][N], g[PACKS][N], d[PACKS][N], hh = Num::splat(0.0f), gh = Num::splat(0.0f);
+    V hh = Num::splat(0.0f), gh = Num::splat(0.0f);
+    Row cur;
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-      Num::decode(h[i], now.h[i]);
-      Num::decode(g[i], now.g[i]);
-      Num::decode(d[i], now.d[i]);
+      first.mask(now.h[i], t + i * tpr); first.mask(now.g[i], t + i * tpr);
+      cur.h[i] = now.h[i]; cur.g[i] = now.g[i]; cur.d[i] = now.d[i];
     }
-    fetch(now, row + step);                          // in flight during this row's sums
+    if constexpr (!LEAN) fetch(now, row + step);     // in flight during this row's sums
 #pragma unroll
-    for (int i = 0; i < PACKS; ++i)
+    for (int i = 0; i < PACKS; ++i) {
+      V h[N], g[N];
+      Num::decode(h, cur.h[i]);
+      Num::decode(g, cur.g[i]);
+      if constexpr (LEAN) weight(w[0], t + i * tpr);
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        hh = Num::fma(h[i][k], h[i][k], hh);
-        gh = Num::fma(Num::mul(g[i][k], w[i][k]), h[i][k], gh);
+        hh = Num::fma(h[k], h[k], hh);
+        gh = Num::fma(Num::mul(g[k], w[LEAN ? 0 : i][k]), h[k], gh);
       }
+    }
     float s[2] = {Num::sum(hh), Num::sum(gh)};
-    row_sum(s, p.log_tpr, red, parity);
-    if (row >= p.rows) continue;                     // this group's last round; the others' barriers are behind it
-    const View view(row, p.ld, p.cols);
-    const float rstd = rsqrtf(s[0] * p.inv_cols + p.eps);
-    // dx = rstd * (dy w) - h * (rstd^3 * mean(dy w h)) + dh;  dw += dy * h * rstd
-    const V up = Num::splat(rstd), down = Num::splat(-(rstd * rstd * rstd) * (s[1] * p.inv_cols));
+    row_sum(s, p.log_tpr, p.tpr >> 5, red, parity);
+    if (row < p.rows) {
+      const View view(row, p.ld, p.cols);
+      const float rstd = rsqrtf(s[0] * p.inv_cols + p.eps);
+      // dx = rstd * (dy w) - h * (rstd^3 * mean(dy w h)) + dh;  dw += dy * h * rstd
+      const V up = Num::splat(rstd), down = Num::splat(-(rstd * rstd * rstd) * (s[1] * p.inv_cols));
 #pragma unroll
-    for (int i = 0; i < PACKS; ++i) {
-      const int pack = t + i * tpr;
-      if (!view.has(pack)) continue;
-      V o[N];
+      for (int i = 0; i < PACKS; ++i) {
+        const int pack = t + i * tpr;
+        if (!view.has(pack)) continue;
+        V h[N], g[N], d[N], o[N];
+        Num::decode(h, cur.h[i]);
+        Num::decode(g, cur.g[i]);
+        Num::decode(d, cur.d[i]);
+        if constexpr (LEAN) weight(w[0], pack);
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const V gu = Num::mul(g[i][k], up);
-        dw[i][k] = Num::fma(gu, h[i][k], dw[i][k]);
-        o[k] = Num::add(Num::fma(gu, w[i][k], Num::mul(h[i][k], down)), d[i][k]);
+        for (int k = 0; k < N; ++k) {
+          const V gu = Num::mul(g[k], up);
+          dw[i][k] = Num::fma(gu, h[k], dw[i][k]);
+          o[k] = Num::add(Num::fma(gu, w[LEAN ? 0 : i][k], Num::mul(h[k], down)), d[k]);
+        }
+        view.store(o, p.y, pack, p.rn != 0);
       }
-      view.store(o, p.y, pack, p.rn != 0);
     }
+    if constexpr (LEAN) fetch(now, row + step);
   }
   if (!p.weight_on) return;
   // the CTA's groups are added in order, then one row of partials per CTA
@@ -414,25 +449,36 @@ int log2_up(uint64_t v) {
   return l;
 }
 
-struct RmsShape { bool aligned; int log_tpr, packs, threads; };
+struct RmsShape { int log_tpr, tpr, packs, threads, groups; };
 
 // Threads per row and vectors per thread.  A thread's fixed work (addresses, the row's sum) is worth about a vector's, so rows are
-// held by few threads with four vectors each (two for f32: as many bytes in registers) - unless there are too few rows to fill the
-// SMs that way, where a row is spread as wide as it goes.
+// held by few threads with several vectors each (four loads in flight per thread: 8192 x 4096 bf16 with residual and 8-bit output takes
+// 66 us with one vector per thread, 41 with two, 43 with four) - unless there are too few rows to fill the SMs that way, where a row
+// is spread as wide as it goes.
 RmsShape rms_shape(uint64_t rows, uint64_t vectors, int packs_wanted, int sm_count) {
   RmsShape s{};
-  int packs = rows * vectors < (uint64_t)sm_count * 2048 ? 1 : packs_wanted;
-  s.log_tpr = std::min(10, std::max(3, log2_up((vectors + packs - 1) / packs)));
-  const int need = (int)((vectors + (1u << s.log_tpr) - 1) >> s.log_tpr);
-  s.packs = 1;
-  while (s.packs < need) s.packs *= 2;
-  s.threads = std::max(256, 1 << s.log_tpr);
+  const int packs = rows * vectors < (uint64_t)sm_count * 2048 ? 1 : packs_wanted;
+  const uint64_t want = std::min<uint64_t>(1024, (vectors + packs - 1) / packs);
+  if (want <= 128) {
+    s.log_tpr = std::max(3, log2_up(want));
+    s.tpr = 1 << s.log_tpr;
+    s.threads = 256;
+    s.groups = 256 >> s.log_tpr;
+  } else {
+    s.log_tpr = 10;
+    s.tpr = (int)((want + 31) / 32 * 32);
+    s.threads = s.tpr;
+    s.groups = 1;
+  }
+  s.packs = (int)((vectors + s.tpr - 1) / s.tpr);
   return s;
 }
 
+void rms_apply(RmsParams& p, const RmsShape& s) { p.log_tpr = s.log_tpr; p.tpr = s.tpr; p.groups = s.groups; }
+
 template <typename T, int PACKS, bool ALIGNED, int THREADS>
 cudaError_t run_rms(const RmsParams& p, const RmsShape& s, bool quant, const LaunchCtx& lc) {
-  const uint64_t per_cta = (uint64_t)(s.threads >> s.log_tpr);
+  const uint64_t per_cta = (uint64_t)s.groups;
   const unsigned grid = (unsigned)((p.rows + per_cta - 1) / per_cta);
   constexpr uint32_t VEC = 16 / sizeof(typename Elem<T>::store_t);
   const uint32_t width = p.group / VEC;
@@ -440,7 +486,7 @@ cudaError_t run_rms(const RmsParams& p, const RmsShape& s, bool quant, const Lau
     return launch_pdl(rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_NONE, THREADS>, dim3(grid), s.threads, 0, lc.stream, p);
   }
   if constexpr (ALIGNED) {
-    if (p.group % VEC == 0 && (width & (width - 1)) == 0 && width <= 32 && (int)width <= 1 << s.log_tpr) {
+    if (p.group % VEC == 0 && (width & (width - 1)) == 0 && width <= 32 && (int)width <= s.tpr) {
       return launch_pdl(rmsnorm_kernel<T, PACKS, ALIGNED, QUANT_LANES, THREADS>, dim3(grid), s.threads, 0, lc.stream, p);
     }
   }
@@ -449,14 +495,16 @@ cudaError_t run_rms(const RmsParams& p, const RmsShape& s, bool quant, const Lau
 
 template <typename T, bool ALIGNED>
 cudaError_t run_rms_packs(const RmsParams& p, const RmsShape& s, bool quant, const LaunchCtx& lc) {
-  if (s.threads == 256) {
+  if (s.threads <= 256) {
     if (s.packs == 1) return run_rms<T, 1, ALIGNED, 256>(p, s, quant, lc);
     if (s.packs == 2) return run_rms<T, 2, ALIGNED, 256>(p, s, quant, lc);
-    return run_rms<T, 4, ALIGNED, 256>(p, s, quant, lc);
+    if (s.packs <= 4) return run_rms<T, 4, ALIGNED, 256>(p, s, quant, lc);
+    if constexpr (sizeof(T) == 4) return run_rms<T, 8, ALIGNED, 256>(p, s, quant, lc);
   }
   if (s.packs == 1) return run_rms<T, 1, ALIGNED, 1024>(p, s, quant, lc);
   if (s.packs == 2) return run_rms<T, 2, ALIGNED, 1024>(p, s, quant, lc);
-  if constexpr (sizeof(T) == 4 && !ALIGNED) { if (s.packs == 8) return run_rms<T, 8, ALIGNED, 1024>(p, s, quant, lc); }     // 4097 vectors
+  if constexpr (sizeof(T) == 4 && !ALIGNED) { if (s.packs > 4 && s.threads > 512) return run_rms<T, 8, ALIGNED, 1024>(p, s, quant, lc); }     // 4097 vectors, spread wide
+  if constexpr (sizeof(T) == 4) { if (s.packs > 4) return run_rms<T, 8, ALIGNED, 512>(p, s, quant, lc); }
   return run_rms<T, 4, ALIGNED, 1024>(p, s, quant, lc);
 }
 
@@ -465,15 +513,15 @@ cudaError_t rms_forward(const RmsParams& p, bool quant, const LaunchCtx& lc) {
   constexpr uint32_t VEC = 16 / sizeof(typename Elem<T>::store_t);
   RmsParams q = p;
   const bool aligned = p.cols % VEC == 0 && p.ld % VEC == 0;
-  const RmsShape s = rms_shape(p.rows, aligned ? p.cols / VEC : (p.cols + 2 * VEC - 2) / VEC, 4, lc.sm_count);
-  q.log_tpr = s.log_tpr;
+  const RmsShape s = rms_shape(p.rows, aligned ? p.cols / VEC : (p.cols + 2 * VEC - 2) / VEC, p.residual_on ? 2 : 4, lc.sm_count);
+  rms_apply(q, s);
   return aligned ? run_rms_packs<T, true>(q, s, quant, lc) : run_rms_packs<T, false>(q, s, quant, lc);
 }
 
 template <typename T, int PACKS, bool ALIGNED, int THREADS>
 cudaError_t run_rms_bwd(const RmsParams& p, const RmsShape& s, unsigned* grid_out, const LaunchCtx& lc) {
   constexpr int VEC = 16 / (int)sizeof(typename Elem<T>::store_t);
-  const int groups = s.threads >> s.log_tpr;
+  const int groups = s.groups;
   const size_t smem = p.weight_on ? (size_t)groups * p.cols * 4 : 0;
   auto kern = rmsnorm_bwd_kernel<T, PACKS, ALIGNED, THREADS>;
   static uint64_t configured = 0;
@@ -489,19 +537,17 @@ cudaError_t run_rms_bwd(const RmsParams& p, const RmsShape& s, unsigned* grid_ou
 }
 
 // The adjoint's groups: a column's weight, its gradient, this row's h, dy, dh and the next row's all stay in registers, so a thread
-// takes two vectors and the group grows, to 1024 threads.  (Those have 64 registers each: above 8192 columns of 16 bits, 4096 of f32,
-// some of it is spilled.)
+// takes two vectors and the group grows, to 1024 threads - which have 64 registers each, and load the weights anew for every row and
+// the next row after this one.
 template <typename T, bool ALIGNED>
 cudaError_t run_rms_bwd_packs(const RmsParams& p, const RmsShape& s, unsigned* grid, const LaunchCtx& lc) {
-  if (s.threads == 256) return s.packs == 1 ? run_rms_bwd<T, 1, ALIGNED, 256>(p, s, grid, lc) : run_rms_bwd<T, 2, ALIGNED, 256>(p, s, grid, lc);
-  if (s.threads == 512) return run_rms_bwd<T, 2, ALIGNED, 512>(p, s, grid, lc);
-  if constexpr (sizeof(T) == 4) {
-    if constexpr (!ALIGNED) { if (s.packs == 8) return run_rms_bwd<T, 8, ALIGNED, 1024>(p, s, grid, lc); }      // 4097 vectors
-    if (s.packs == 4) return run_rms_bwd<T, 4, ALIGNED, 1024>(p, s, grid, lc);
-  } else if constexpr (!ALIGNED) {
-    if (s.packs == 4) return run_rms_bwd<T, 4, ALIGNED, 1024>(p, s, grid, lc);                                   // 2049 vectors
-  }
-  return run_rms_bwd<T, 2, ALIGNED, 1024>(p, s, grid, lc);
+  if (s.threads <= 256) return s.packs == 1 ? run_rms_bwd<T, 1, ALIGNED, 256>(p, s, grid, lc) : run_rms_bwd<T, 2, ALIGNED, 256>(p, s, grid, lc);
+  if constexpr (sizeof(T) == 4) { if (s.threads <= 512 && s.packs == 3) return run_rms_bwd<T, 3, ALIGNED, 512>(p, s, grid, lc); }
+  if (s.threads <= 512) return run_rms_bwd<T, 2, ALIGNED, 512>(p, s, grid, lc);
+  if (s.packs <= 2) return run_rms_bwd<T, 2, ALIGNED, 1024>(p, s, grid, lc);
+  if constexpr (sizeof(T) == 4 && !ALIGNED) { if (s.packs > 4) return run_rms_bwd<T, 8, ALIGNED, 1024>(p, s, grid, lc); }      // 4097 vectors
+  if constexpr (sizeof(T) == 4 || !ALIGNED) return run_rms_bwd<T, 4, ALIGNED, 1024>(p, s, grid, lc);                           // 16-bit: 2049 vectors
+  else return run_rms_bwd<T, 2, ALIGNED, 1024>(p, s, grid, lc);
 }
 
 template <typename T>
@@ -510,8 +556,11 @@ cudaError_t rms_backward(const RmsParams& p, const LaunchCtx& lc) {
   constexpr uint32_t VEC = 16 / sizeof(S);
   RmsParams q = p;
   const bool aligned = p.cols % VEC == 0 && p.ld % VEC == 0;
-  const RmsShape s = rms_shape(p.rows, aligned ? p.cols / VEC : (p.cols + 2 * VEC - 2) / VEC, 2, lc.sm_count);
-  q.log_tpr = s.log_tpr;
+  const uint64_t vectors = aligned ? p.cols / VEC : (p.cols + 2 * VEC - 2) / VEC;
+  // three vectors of f32 still fit the registers of 512 threads, which hold 6144 columns that way
+  RmsShape s = rms_shape(p.rows, vectors, 2, lc.sm_count);
+  if (sizeof(T) == 4 && s.threads > 512 && vectors <= 3 * 512) s = rms_shape(UINT32_MAX, vectors, 3, lc.sm_count);
+  rms_apply(q, s);
   unsigned grid = 0;
   cudaError_t e = aligned ? run_rms_bwd_packs<T, true>(q, s, &grid, lc) : run_rms_bwd_packs<T, false>(q, s, &grid, lc);
   if (e == cudaSuccess && p.weight_on)
@@ -545,7 +594,7 @@ int launch_rmsnorm(const zyxb_rmsnorm_desc& d, void* const* args, const uint64_t
   ZYXB_CHECK_ARG(n_args == want, "rmsnorm: expected args x [,residual] [,weight] -> [h,] y [,scales]");
   const uint64_t es = dtype_size(d.dtype);
   RmsParams p{};
-  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.eps = d.eps; p.inv_cols = 1.0f / (float)d.cols; p.rn = lc.round_nearest ? 1 : 0;
+  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.end = (d.rows - 1) * p.ld + d.cols; p.eps = d.eps; p.inv_cols = 1.0f / (float)d.cols; p.rn = lc.round_nearest ? 1 : 0;
   p.residual_on = d.has_residual ? 1 : 0; p.weight_on = d.has_weight ? 1 : 0;
   p.group = d.group ? std::min<uint32_t>(d.group, p.cols) : p.cols;
   p.n_groups = (p.cols + p.group - 1) / p.group;
@@ -579,7 +628,7 @@ int launch_rmsnorm_bwd(const zyxb_rmsnorm_desc& d, void* const* args, const uint
   ZYXB_CHECK_ARG(n_args == want, "rmsnorm backward: expected args h, dy [,weight] [,dh] -> dx [,dweight]");
   const uint64_t es = dtype_size(d.dtype);
   RmsParams p{};
-  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.eps = d.eps; p.inv_cols = 1.0f / (float)d.cols; p.rn = lc.round_nearest ? 1 : 0;
+  p.rows = d.rows; p.cols = (uint32_t)d.cols; p.ld = d.ld ? d.ld : d.cols; p.end = (d.rows - 1) * p.ld + d.cols; p.eps = d.eps; p.inv_cols = 1.0f / (float)d.cols; p.rn = lc.round_nearest ? 1 : 0;
   p.weight_on = d.has_weight ? 1 : 0; p.dh_on = d.has_dh ? 1 : 0;
   int i = 0;
   ZYXB_CHECK_ARG(rows_fit(d, p.ld, arg_bytes[i]), "rmsnorm backward: h too small"); p.h = args[i++];

@@ -71,4 +71,73 @@ template <int VEC> struct Nums {
   }
 };
 
+// elements d .. d + VEC of the two vectors in w
+template <typename T, int VEC>
+__device__ __forceinline__ void shift_vector(RawVec<T, VEC>& r, uint32_t (&w)[2 * RawVec<T, VEC>::NW], int d) {
+  constexpr int W = RawVec<T, VEC>::NW, PER = VEC / W;
+  const int s = d / PER;
+  if (s & 2) {
+#pragma unroll
+    for (int j = 0; j < 2 * W - 2; ++j) w[j] = w[j + 2];
+  }
+  if (s & 1) {
+#pragma unroll
+    for (int j = 0; j < 2 * W - 3; ++j) w[j] = w[j + 1];
+  }
+#pragma unroll
+  for (int j = 0; j < W; ++j) r.w[j] = PER == 2 && (d & 1) ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
+}
+
+// A vector from any element on, of a buffer that starts on a vector boundary and has `end` elements: the two aligned vectors that hold
+// it (elements before the buffer or behind its end come as zeros), and how far it lies inside them.  Every lane of a row shifts
+// alike, and the second vector is the next lane's first, so the extra read is an L1 hit.  Loading and shifting are two steps: a
+// thread starts all of its loads before it waits for the first.
+// (its elements at the buffer's ends: rare, and kept out of the way of the loops that inline the rest)
+template <typename T, int VEC>
+__device__ __noinline__ uint4 vector_at_end(const typename Elem<T>::store_t* base, int64_t first, uint64_t end) {
+  constexpr int PER = VEC / 4;
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int k = 0; k < VEC; ++k)
+    if (first + k >= 0 && (uint64_t)(first + k) < end) {
+      if constexpr (PER == 2) w[k / 2] |= (uint32_t)base[first + k] << (16 * (k & 1));
+      else w[k] = __float_as_uint(base[first + k]);
+    }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T, int VEC> struct Shifted {
+  using S = typename Elem<T>::store_t;
+  static constexpr int W = RawVec<T, VEC>::NW, PER = VEC / W;          // words, elements per word
+  static_assert(W == 4, "16-byte vectors");
+  RawVec<T, VEC> half[2];
+  int d;
+  __device__ __forceinline__ void zero() { half[0].zero(); half[1].zero(); d = 0; }
+  __device__ __forceinline__ void load(const S* base, int64_t e, uint64_t end) {
+    const int64_t v = e >= 0 ? e / VEC : -((-e + VEC - 1) / VEC), first = v * VEC;
+    d = (int)(e - first);
+    if (first >= 0 && (uint64_t)first + 2 * VEC <= end) {
+      half[0].load(base + first);
+      half[1].load(base + first + VEC);
+      return;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 q = vector_at_end<T, VEC>(base, first + h * VEC, end);
+      half[h].w[0] = q.x; half[h].w[1] = q.y; half[h].w[2] = q.z; half[h].w[3] = q.w;
+    }
+  }
+  __device__ __forceinline__ void get(RawVec<T, VEC>& r) const {
+    uint32_t w[2 * W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) { w[j] = half[0].w[j]; w[W + j] = half[1].w[j]; }
+    shift_vector<T, VEC>(r, w, d);
+  }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void load_shifted(RawVec<T, VEC>& r, const typename Elem<T>::store_t* base, int64_t e, uint64_t end) {
+  Shifted<T, VEC> s;
+  s.load(base, e, end);
+  s.get(r);
+}
+
 }  // namespace zyxb
