@@ -397,13 +397,14 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
   cudaError_t e = launch_pdl(muon_momentum_kernel<T>, dim3(sums, batch), MUON_THREADS, 0, lc.stream, k, partial);
   if (e == cudaSuccess) e = launch_pdl(muon_normalize_kernel<T, PARTS>, tiles, MUON_THREADS, 0, lc.stream, k, partial, (int)sums, d.eps == 0.0f ? 1e-7f : d.eps, x[0]);
 
-  const int bn_sym = splits > 1 ? 128 : muon::tile_width<PARTS, true>(lo, lo, batch, lc.sm_count), bn_apply = muon::tile_width<PARTS, false>(lo, hi, batch, lc.sm_count);
+  const muon::Shape sym = splits > 1 ? muon::Shape{1, 128} : muon::tile_shape<PARTS, true>(lo, lo, batch, lc.sm_count), square = muon::tile_shape<PARTS, true>(lo, lo, batch, lc.sm_count),
+                    apply = muon::tile_shape<PARTS, false>(lo, hi, batch, lc.sm_count);
   CUtensorMap x_rows[2], x_cols[2], x_k[2], gram_rows, gram_cols, poly_rows;
   bool ok = true;
   for (int j = 0; j < 2; ++j)
-    ok = ok && muon::encode(lc.tma_encode, &x_rows[j], x[j], PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &x_cols[j], x[j], PARTS, batch, bn_sym) &&
+    ok = ok && muon::encode(lc.tma_encode, &x_rows[j], x[j], PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &x_cols[j], x[j], PARTS, batch, (uint32_t)(sym.bn / sym.ctas)) &&
          muon::encode(lc.tma_encode, &x_k[j], x[j], PARTS, batch, 64);
-  ok = ok && muon::encode(lc.tma_encode, &gram_rows, gram, PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &gram_cols, gram, PARTS, batch, bn_sym) &&
+  ok = ok && muon::encode(lc.tma_encode, &gram_rows, gram, PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &gram_cols, gram, PARTS, batch, (uint32_t)(square.bn / square.ctas)) &&
        muon::encode(lc.tma_encode, &poly_rows, poly, PARTS, batch, muon::BM);
   if (!ok) { err = "muon: cuTensorMapEncodeTiled rejected an operand"; return ZYXB_ERR_KERNEL_LAUNCH; }
   float a, b, c;
@@ -419,20 +420,20 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
     if (splits > 1) {
       muon::GemmArgs s = gemm_args(gram, hi);
       s.partial = split_sums; s.splits = splits;
-      e = muon::launch<PARTS, 128, true, false, false, true>(x_rows[from], x_cols[from], s, lc);
+      e = muon::launch<PARTS, 128, 1, true, false, false, true>(x_rows[from], x_cols[from], s, lc);
       const unsigned blocks = (lo + 63) / 64;
       if (e == cudaSuccess)
-        e = launch_pdl(muon::gram_finish_kernel<PARTS>, dim3(blocks, blocks, batch), 256, 0, lc.stream, (const float*)split_sums, splits, muon::tile_count<true>(lo, lo, 128), s);
-    } else e = bn_sym == 128 ? muon::launch<PARTS, 128, true, false, false>(x_rows[from], x_cols[from], gemm_args(gram, hi), lc)
-                      : muon::launch<PARTS, 256, true, false, false>(x_rows[from], x_cols[from], gemm_args(gram, hi), lc);
+        e = launch_pdl(muon::gram_finish_kernel<PARTS>, dim3(blocks, blocks, batch), 256, 0, lc.stream, (const float*)split_sums, splits,
+                       muon::tile_count<true>(lo, lo, 128, 128), s);
+    } else {
+      e = muon::launch<PARTS, true, false, false>(sym, x_rows[from], x_cols[from], gemm_args(gram, hi), lc);
+    }
     if (e != cudaSuccess) break;
     muon::GemmArgs g = gemm_args(poly, lo);
     g.gram = gram.ptr; g.a = a; g.b = b; g.c = c;
-    e = bn_sym == 128 ? muon::launch<PARTS, 128, true, true, false>(gram_rows, gram_cols, g, lc)
-                      : muon::launch<PARTS, 256, true, true, false>(gram_rows, gram_cols, g, lc);
+    e = muon::launch<PARTS, true, true, false>(square, gram_rows, gram_cols, g, lc);
     if (e != cudaSuccess) break;
-    e = bn_apply == 128 ? muon::launch<PARTS, 128, false, false, true>(poly_rows, x_k[from], gemm_args(x[from ^ 1], lo), lc)
-                        : muon::launch<PARTS, 256, false, false, true>(poly_rows, x_k[from], gemm_args(x[from ^ 1], lo), lc);
+    e = muon::launch<PARTS, false, false, true>(apply, poly_rows, x_k[from], gemm_args(x[from ^ 1], lo), lc);
   }
   if (e != cudaSuccess) { err = std::string("muon: ") + cudaGetErrorString(e); return ZYXB_ERR_KERNEL_LAUNCH; }
   e = launch_pdl(muon_step_kernel<T, PARTS>, tiles, MUON_THREADS, 0, lc.stream, k, x[steps & 1], 1.0f - d.lr * d.weight_decay,

@@ -9,6 +9,9 @@
 //
 // The pipeline is the 16-bit matmul's: one persistent CTA per SM, warp 0 loads tiles by TMA, warp 1 issues tcgen05.mma, warps 2..9
 // read the accumulators from TMEM while the next tile is multiplied.  What differs:
+//   pairs     CTAS = 2: two CTAs of a cluster share a tile of 256 rows (cta_group::2).  Each loads its 128 rows of the left operand
+//             and half of the right one's columns, the first issues the instructions for both, each keeps its own rows' accumulator.
+//             A tile's operands then cross L2 and shared memory once per pair: PAIR_NUMBERS
 //   symmetry  only tiles that touch the lower triangle are computed, and stored twice: half of the work of gram and poly.
 //   split     a gram product with few tiles and a long contraction is cut along it: every CTA leaves its f32 sums, and a second
 //             launch adds them in order (129 x 4096 f32: 3 tiles, 64 k-blocks of 0.5 us each).
@@ -49,8 +52,9 @@ struct GemmArgs {
   uint32_t* status;
 };
 
-template <int PARTS, int BN> struct Smem {
-  static constexpr int A_PART = BM * BK * 2, B_PART = BN * BK * 2;
+template <int PARTS, int BN, int CTAS> struct Smem {
+  static constexpr int B_ROWS = BN / CTAS;                       // of the right operand, per CTA
+  static constexpr int A_PART = BM * BK * 2, B_PART = B_ROWS * BK * 2;
   static constexpr int STAGE = PARTS * (A_PART + B_PART);
   static constexpr int STAGES = 196608 / STAGE;
   static constexpr int BAR = STAGES * STAGE;
@@ -63,10 +67,54 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = pack2_t<false>(x - hx, y - hy);
 }
 
-template <int PARTS, int BN, bool SYM, bool POLY, bool B_MN, bool SPLIT>
+// ---- clusters --------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// a load into this CTA's shared memory that reports to a barrier of either CTA of the pair
+__device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int zi, int zo) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(zi), "r"(zo) : "memory");
+}
+template <int CTAS> __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t more) {
+  if constexpr (CTAS == 1) umma_f16(d, a, b, idesc, more);
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(more) : "memory");
+}
+// the barrier at this place in every CTA of the pair
+template <int CTAS> __device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CTAS == 1) umma_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+template <int CTAS> __device__ __forceinline__ void alloc(uint32_t dst_smem, uint32_t cols) {
+  if constexpr (CTAS == 1) tmem_alloc(dst_smem, cols);
+  else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CTAS> __device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t cols) {
+  if constexpr (CTAS == 1) tmem_dealloc(taddr, cols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+
+template <int PARTS, int BN, int CTAS, bool SYM, bool POLY, bool B_MN, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, GemmArgs p) {
-  using SM = Smem<PARTS, BN>;
+  using SM = Smem<PARTS, BN, CTAS>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - raw);
@@ -79,15 +127,18 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr uint32_t TMEM_COLS = 2 * BN;
+  const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
   if (threadIdx.x == 0) {
+    // of a pair, the first CTA's full and tempty barriers count for both; empty and tfull are signalled in both
     for (int s = 0; s < SM::STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), EPI_THREADS / 32); }
+    for (int a = 0; a < 2; ++a) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), CTAS * (EPI_THREADS / 32)); }
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+  if (warp == 1) alloc<CTAS>(smem_u32(tmem_slot), TMEM_COLS);
   tc_fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();
@@ -105,14 +156,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     z = t / p.tiles;
     const uint32_t r = t - z * p.tiles;
     if constexpr (SYM) {
-      // row tm of tiles holds tm / W + 1 of them (W = BN / BM): W rows at a time, q + 1 tiles each, W q (q + 1) / 2 before them
-      constexpr uint32_t W = BN / BM;
-      uint32_t q = (uint32_t)((sqrtf(1.0f + 8.0f * (float)r / W) - 1.0f) * 0.5f);
-      while (W * q * (q + 1) / 2 > r) --q;
-      while (W * (q + 1) * (q + 2) / 2 <= r) ++q;
-      const uint32_t in = r - W * q * (q + 1) / 2;
-      tm = q * W + in / (q + 1);
-      tn = in % (q + 1);
+      // Tiles are R = 128 CTAS rows high.  BN >= R: W = BN / R rows of them at a time have q + 1 tiles each, W q (q + 1) / 2 lie before
+      // them.  BN = R / 2: row q has 2 (q + 1), q (q + 1) lie before it.
+      constexpr uint32_t R = BM * CTAS, W2 = 2 * BN / R, ROWS = W2 >= 2 ? W2 / 2 : 1, EACH = W2 >= 2 ? 1 : 2;
+      constexpr uint32_t TWICE = ROWS * EACH;                  // 2 q (q + 1) / 2 tiles before group q, times this
+      uint32_t q = (uint32_t)((sqrtf(1.0f + 8.0f * (float)r / TWICE) - 1.0f) * 0.5f);
+      while (TWICE * q * (q + 1) / 2 > r) --q;
+      while (TWICE * (q + 1) * (q + 2) / 2 <= r) ++q;
+      const uint32_t in = r - TWICE * q * (q + 1) / 2, per_row = EACH * (q + 1);
+      tm = q * ROWS + in / per_row;
+      tn = in % per_row;
     } else {
       constexpr uint32_t GROUP_M = 16;   // tiles that run together share panels in L2
       const uint32_t group_size = GROUP_M * p.tiles_n, g = r / group_size, first_m = g * GROUP_M;
@@ -126,7 +179,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     if (lane == 0) {
       uint32_t stage = 0, phase = 0, issued = 0;
       bool ok = true;
-      for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      for (uint32_t t = blockIdx.x / CTAS; t < total && ok; t += gridDim.x / CTAS) {
         uint32_t z, tm, tn;
         tile_coords(t, z, tm, tn);
         uint32_t kb0, kb1;
@@ -134,24 +187,28 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         for (uint32_t kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, p.status, ERR_PRODUCER)) { ok = false; break; }
           const uint32_t a_dst = base + stage * SM::STAGE, b_dst = a_dst + PARTS * SM::A_PART;
-          mbar_expect_tx(full_bar(stage), SM::STAGE);
-          const int k0 = (int)(kb * BK);
+          if (rank == 0) mbar_expect_tx(full_bar(stage), CTAS * SM::STAGE);
+          const uint32_t full = CTAS == 2 ? map_to(full_bar(stage), 0) : full_bar(stage);
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, int part) {
+            if constexpr (CTAS == 2) tma_load_4d_pair(dst, map, full, x, y, part, (int)z);
+            else tma_load_4d(dst, map, full, x, y, part, (int)z);
+          };
+          const int k0 = (int)(kb * BK), row_a = (int)((tm * CTAS + rank) * BM), row_b = (int)(tn * BN + rank * SM::B_ROWS);
 #pragma unroll
           for (int q = 0; q < PARTS; ++q) {
-            tma_load_4d(a_dst + q * SM::A_PART, &map_a, full_bar(stage), k0, (int)(tm * BM), q, (int)z);
+            load(a_dst + q * SM::A_PART, &map_a, k0, row_a, q);
             if constexpr (B_MN) {
 #pragma unroll
-              for (int j = 0; j < BN / 64; ++j)
-                tma_load_4d(b_dst + q * SM::B_PART + j * (64 * BK * 2), &map_b, full_bar(stage), (int)(tn * BN) + j * 64, k0, q, (int)z);
+              for (int j = 0; j < SM::B_ROWS / 64; ++j) load(b_dst + q * SM::B_PART + j * (64 * BK * 2), &map_b, row_b + j * 64, k0, q);
             } else {
-              tma_load_4d(b_dst + q * SM::B_PART, &map_b, full_bar(stage), k0, (int)(tn * BN), q, (int)z);
+              load(b_dst + q * SM::B_PART, &map_b, k0, row_b, q);
             }
           }
           ++issued;
           if (++stage == SM::STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      if (!ok) {     // copies in flight land before the CTA goes
+      if (!ok && rank == 0) {     // copies in flight land before the CTA goes (a pair's: both wait for each other at the end)
         uint32_t s = stage, ph = phase;
         const uint32_t n_back = issued < (uint32_t)SM::STAGES ? issued : (uint32_t)SM::STAGES;
         for (uint32_t i = 0; i < n_back; ++i) {
@@ -162,11 +219,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc(false, false, B_MN, BM, BN);
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = make_idesc(false, false, B_MN, BM * CTAS, BN);
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
-      for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      for (uint32_t t = blockIdx.x / CTAS; t < total && ok; t += gridDim.x / CTAS) {
         uint32_t kb0, kb1;
         k_range(t, kb0, kb1);
         for (uint32_t kb = kb0; kb < kb1 && ok; ++kb) {
@@ -188,17 +245,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             };
             const uint32_t more = (in_chunk | (uint32_t)kk) != 0 ? 1u : 0u;
             if constexpr (PARTS == 2) {     // the small products first
-              umma_f16(d_tmem, adesc(1), bdesc(0), idesc, more);
-              umma_f16(d_tmem, adesc(0), bdesc(1), idesc, 1u);
-              umma_f16(d_tmem, adesc(0), bdesc(0), idesc, 1u);
+              mma<CTAS>(d_tmem, adesc(1), bdesc(0), idesc, more);
+              mma<CTAS>(d_tmem, adesc(0), bdesc(1), idesc, 1u);
+              mma<CTAS>(d_tmem, adesc(0), bdesc(0), idesc, 1u);
             } else {
-              umma_f16(d_tmem, adesc(0), bdesc(0), idesc, more);
+              mma<CTAS>(d_tmem, adesc(0), bdesc(0), idesc, more);
             }
           }
-          umma_commit(empty_bar(stage));
+          commit<CTAS>(empty_bar(stage));
           if (++stage == SM::STAGES) { stage = 0; phase ^= 1; }
           if (kb + 1 == kb1 || (PARTS == 2 && in_chunk == CHUNK_BLOCKS - 1)) {
-            umma_commit(tfull_bar(acc));
+            commit<CTAS>(tfull_bar(acc));
             if (++acc == 2) { acc = 0; acc_phase ^= 1; }
           }
         }
@@ -209,9 +266,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const int col_half = (warp - 2) >> 2;
     const uint32_t quarter = (uint32_t)(warp & 3);
     constexpr int HALF = BN / 2, CH = HALF / 32;
+    auto release = [&](uint32_t a) {                       // the accumulator goes back to the issuer
+      if constexpr (CTAS == 2) mbar_arrive_cluster(map_to(tempty_bar(a), 0));
+      else mbar_arrive(tempty_bar(a));
+    };
     uint32_t acc = 0, acc_phase = 0;
     bool ok = true;
-    for (uint32_t t = blockIdx.x; t < total && ok; t += gridDim.x) {
+    for (uint32_t t = blockIdx.x / CTAS; t < total && ok; t += gridDim.x / CTAS) {
       uint32_t z, tm, tn;
       tile_coords(t, z, tm, tn);
       uint32_t kb0, kb1;
@@ -219,7 +280,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       const uint32_t n_chunks = PARTS == 2 ? (kb1 - kb0 + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS : 1;
       uint16_t* out = p.out + z * p.stride;
       const uint16_t* gram = POLY ? p.gram + z * p.stride : nullptr;
-      const uint32_t row0 = tm * BM + quarter * 32, row = row0 + lane;
+      const uint32_t row0 = (tm * CTAS + rank) * BM + quarter * 32, row = row0 + lane;
       // 32 columns from c on of this lane's row
       auto finish = [&](float (&v)[32], uint32_t c) {
         if (c >= p.n || row0 >= p.m) return;
@@ -308,7 +369,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tempty_bar(acc));
+          if (lane == 0) release(acc);
           if (++acc == 2) { acc = 0; acc_phase ^= 1; }
         }
         if (!ok) break;
@@ -334,16 +395,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty_bar(acc));
+        if (lane == 0) release(acc);
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
     }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();                 // the pair's instructions read both CTAs' shared memory
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    dealloc<CTAS>(tmem_base, TMEM_COLS);
   }
 }
 
@@ -423,34 +485,58 @@ inline bool encode(void* fn, CUtensorMap* map, const Operand& o, int parts, uint
   return encode_map(fn, map, false, o.ptr, o.cols, o.rows, o.ld, (uint64_t)parts, parts > 1 ? o.part() : 0, batch, batch > 1 ? o.part() * parts : 0, box_rows);
 }
 
-// Tiles are 128 x 256, or 128 x 128 where those fill the SMs' last round better.  A narrow tile costs more per entry, because both
-// operands' reads from shared memory then run at its rate: 0.83 of a wide tile's time with one part (12.8 against 15.5 us at k = 2048),
-// 0.60 with two (26.2 against 45.9 us: there the tensor core multiplies three times what it reads).
-template <bool SYM> uint32_t tile_count(uint32_t m, uint32_t n, uint32_t bn) {
-  const uint32_t tiles_m = (m + BM - 1) / BM;
+// tiles of `rows` x `bn` that cover a result (of a symmetric one: its lower triangle)
+template <bool SYM> uint32_t tile_count(uint32_t m, uint32_t n, uint32_t rows, uint32_t bn) {
+  const uint32_t tiles_m = (m + rows - 1) / rows;
   if (!SYM) return tiles_m * ((n + bn - 1) / bn);
   uint32_t t = 0;
-  for (uint32_t tm = 0; tm < tiles_m; ++tm) t += tm / (bn / BM) + 1;
+  for (uint32_t tm = 0; tm < tiles_m; ++tm) t += ((tm + 1) * rows - 1) / bn + 1;
   return t;
 }
-template <int PARTS, bool SYM> int tile_width(uint32_t m, uint32_t n, uint32_t batch, int sm_count) {
-  auto rounds = [&](uint32_t bn) { return (tile_count<SYM>(m, n, bn) * (uint64_t)batch + sm_count - 1) / sm_count; };
-  return (PARTS == 1 ? 83 : 60) * rounds(128) < 100 * rounds(256) ? 128 : 256;
+
+// Tile shapes: one CTA 128 x 128, a pair 256 x 128 or 256 x 256.  COST: TILE_NUMBERS
+struct Shape { int ctas, bn; };
+template <int PARTS, bool SYM> Shape tile_shape(uint32_t m, uint32_t n, uint32_t batch, int sm_count) {
+  auto time = [&](int ctas, int bn, int cost) {
+    const uint64_t slots = (uint64_t)sm_count / ctas;
+    return (tile_count<SYM>(m, n, 128 * ctas, bn) * (uint64_t)batch + slots - 1) / slots * cost;
+  };
+  const uint64_t one = time(1, 128, PARTS == 1 ? 83 : 60), narrow = time(2, 128, 60), wide = time(2, 256, 100);
+  if (one <= narrow && one <= wide) return {1, 128};
+  return narrow < wide ? Shape{2, 128} : Shape{2, 256};
 }
 
-template <int PARTS, int BN, bool SYM, bool POLY, bool B_MN, bool SPLIT = false>
+template <int PARTS, int BN, int CTAS, bool SYM, bool POLY, bool B_MN, bool SPLIT = false>
 cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mb, GemmArgs p, const LaunchCtx& lc) {
-  using SM = Smem<PARTS, BN>;
+  using SM = Smem<PARTS, BN, CTAS>;
   static uint64_t configured = 0;
-  auto kern = gemm_kernel<PARTS, BN, SYM, POLY, B_MN, SPLIT>;
+  auto kern = gemm_kernel<PARTS, BN, CTAS, SYM, POLY, B_MN, SPLIT>;
   cudaError_t e = ensure_dynamic_smem(kern, SM::TOTAL, &configured);
   if (e != cudaSuccess) return e;
-  p.tiles_m = (p.m + BM - 1) / BM;
+  p.tiles_m = (p.m + BM * CTAS - 1) / (BM * CTAS);
   p.tiles_n = (p.n + BN - 1) / BN;
-  p.tiles = tile_count<SYM>(p.m, p.n, BN);
+  p.tiles = tile_count<SYM>(p.m, p.n, BM * CTAS, BN);
   p.status = lc.status_word;
-  const unsigned grid = (unsigned)std::min<uint64_t>((uint64_t)p.tiles * p.batch * (SPLIT ? p.splits : 1), (uint64_t)lc.sm_count);
+  const unsigned grid = CTAS * (unsigned)std::min<uint64_t>((uint64_t)p.tiles * p.batch * (SPLIT ? p.splits : 1), (uint64_t)lc.sm_count / CTAS);
+  if constexpr (CTAS == 2) {
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SM::TOTAL; cfg.stream = lc.stream;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, ma, mb, p);
+  }
   return launch_pdl(kern, dim3(grid), THREADS, SM::TOTAL, lc.stream, ma, mb, p);
+}
+
+template <int PARTS, bool SYM, bool POLY, bool B_MN>
+cudaError_t launch(Shape s, const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& p, const LaunchCtx& lc) {
+  if (s.ctas == 1) return launch<PARTS, 128, 1, SYM, POLY, B_MN>(ma, mb, p, lc);
+  if (s.bn == 128) return launch<PARTS, 128, 2, SYM, POLY, B_MN>(ma, mb, p, lc);
+  return launch<PARTS, 256, 2, SYM, POLY, B_MN>(ma, mb, p, lc);
 }
 
 }  // namespace muon
