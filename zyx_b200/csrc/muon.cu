@@ -397,15 +397,13 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
   cudaError_t e = launch_pdl(muon_momentum_kernel<T>, dim3(sums, batch), MUON_THREADS, 0, lc.stream, k, partial);
   if (e == cudaSuccess) e = launch_pdl(muon_normalize_kernel<T, PARTS>, tiles, MUON_THREADS, 0, lc.stream, k, partial, (int)sums, d.eps == 0.0f ? 1e-7f : d.eps, x[0]);
 
-  const muon::Shape sym = splits > 1 ? muon::Shape{1, 128} : muon::tile_shape<PARTS, true>(lo, lo, batch, lc.sm_count), square = muon::tile_shape<PARTS, true>(lo, lo, batch, lc.sm_count),
-                    apply = muon::tile_shape<PARTS, false>(lo, hi, batch, lc.sm_count);
-  CUtensorMap x_rows[2], x_cols[2], x_k[2], gram_rows, gram_cols, poly_rows;
+  // CTAs per tile of the three products; each CTA's share of either operand is 128 rows (or 128 columns, as two boxes of 64) either way
+  const int square = muon::tile_ctas<PARTS, true>(lo, lo, batch, lc.sm_count), apply = muon::tile_ctas<PARTS, false>(lo, hi, batch, lc.sm_count);
+  CUtensorMap x_rows[2], x_k[2], gram_rows, poly_rows;
   bool ok = true;
   for (int j = 0; j < 2; ++j)
-    ok = ok && muon::encode(lc.tma_encode, &x_rows[j], x[j], PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &x_cols[j], x[j], PARTS, batch, (uint32_t)(sym.bn / sym.ctas)) &&
-         muon::encode(lc.tma_encode, &x_k[j], x[j], PARTS, batch, 64);
-  ok = ok && muon::encode(lc.tma_encode, &gram_rows, gram, PARTS, batch, muon::BM) && muon::encode(lc.tma_encode, &gram_cols, gram, PARTS, batch, (uint32_t)(square.bn / square.ctas)) &&
-       muon::encode(lc.tma_encode, &poly_rows, poly, PARTS, batch, muon::BM);
+    ok = ok && muon::encode(lc.tma_encode, &x_rows[j], x[j], PARTS, batch, 128) && muon::encode(lc.tma_encode, &x_k[j], x[j], PARTS, batch, 64);
+  ok = ok && muon::encode(lc.tma_encode, &gram_rows, gram, PARTS, batch, 128) && muon::encode(lc.tma_encode, &poly_rows, poly, PARTS, batch, 128);
   if (!ok) { err = "muon: cuTensorMapEncodeTiled rejected an operand"; return ZYXB_ERR_KERNEL_LAUNCH; }
   float a, b, c;
   muon_coefficients(d, a, b, c);
@@ -420,18 +418,18 @@ int muon_run(const zyxb_muon_desc& d, const uint64_t* rows, const uint64_t* cols
     if (splits > 1) {
       muon::GemmArgs s = gemm_args(gram, hi);
       s.partial = split_sums; s.splits = splits;
-      e = muon::launch<PARTS, 128, 1, true, false, false, true>(x_rows[from], x_cols[from], s, lc);
+      e = muon::launch<PARTS, 128, 1, true, false, false, true>(x_rows[from], x_rows[from], s, lc);
       const unsigned blocks = (lo + 63) / 64;
       if (e == cudaSuccess)
         e = launch_pdl(muon::gram_finish_kernel<PARTS>, dim3(blocks, blocks, batch), 256, 0, lc.stream, (const float*)split_sums, splits,
-                       muon::tile_count<true>(lo, lo, 128, 128), s);
+                       muon::tile_count<true>(lo, lo, 128), s);
     } else {
-      e = muon::launch<PARTS, true, false, false>(sym, x_rows[from], x_cols[from], gemm_args(gram, hi), lc);
+      e = muon::launch<PARTS, true, false, false>(square, x_rows[from], x_rows[from], gemm_args(gram, hi), lc);
     }
     if (e != cudaSuccess) break;
     muon::GemmArgs g = gemm_args(poly, lo);
     g.gram = gram.ptr; g.a = a; g.b = b; g.c = c;
-    e = muon::launch<PARTS, true, true, false>(square, gram_rows, gram_cols, g, lc);
+    e = muon::launch<PARTS, true, true, false>(square, gram_rows, gram_rows, g, lc);
     if (e != cudaSuccess) break;
     e = muon::launch<PARTS, false, false, true>(apply, poly_rows, x_k[from], gemm_args(x[from ^ 1], lo), lc);
   }

@@ -11,7 +11,8 @@
 // read the accumulators from TMEM while the next tile is multiplied.  What differs:
 //   pairs     CTAS = 2: two CTAs of a cluster share a tile of 256 rows (cta_group::2).  Each loads its 128 rows of the left operand
 //             and half of the right one's columns, the first issues the instructions for both, each keeps its own rows' accumulator.
-//             A tile's operands then cross L2 and shared memory once per pair: PAIR_NUMBERS
+//             A tile's operands then cross L2 and shared memory once per pair: 4 x [2048 x 2048 x 2048] takes 55.5 us against 61.9 of
+//             single CTAs with 128 x 256 tiles.
 //   symmetry  only tiles that touch the lower triangle are computed, and stored twice: half of the work of gram and poly.
 //   split     a gram product with few tiles and a long contraction is cut along it: every CTA leaves its f32 sums, and a second
 //             launch adds them in order (129 x 4096 f32: 3 tiles, 64 k-blocks of 0.5 us each).
@@ -156,16 +157,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     z = t / p.tiles;
     const uint32_t r = t - z * p.tiles;
     if constexpr (SYM) {
-      // Tiles are R = 128 CTAS rows high.  BN >= R: W = BN / R rows of them at a time have q + 1 tiles each, W q (q + 1) / 2 lie before
-      // them.  BN = R / 2: row q has 2 (q + 1), q (q + 1) lie before it.
-      constexpr uint32_t R = BM * CTAS, W2 = 2 * BN / R, ROWS = W2 >= 2 ? W2 / 2 : 1, EACH = W2 >= 2 ? 1 : 2;
-      constexpr uint32_t TWICE = ROWS * EACH;                  // 2 q (q + 1) / 2 tiles before group q, times this
-      uint32_t q = (uint32_t)((sqrtf(1.0f + 8.0f * (float)r / TWICE) - 1.0f) * 0.5f);
-      while (TWICE * q * (q + 1) / 2 > r) --q;
-      while (TWICE * (q + 1) * (q + 2) / 2 <= r) ++q;
-      const uint32_t in = r - TWICE * q * (q + 1) / 2, per_row = EACH * (q + 1);
-      tm = q * ROWS + in / per_row;
-      tn = in % per_row;
+      // square tiles (128 or 256): row tm has tm + 1 of them, tm (tm + 1) / 2 lie before it
+      tm = (uint32_t)((sqrtf(1.0f + 8.0f * (float)r) - 1.0f) * 0.5f);
+      while (tm * (tm + 1) / 2 > r) --tm;
+      while ((tm + 1) * (tm + 2) / 2 <= r) ++tm;
+      tn = r - tm * (tm + 1) / 2;
     } else {
       constexpr uint32_t GROUP_M = 16;   // tiles that run together share panels in L2
       const uint32_t group_size = GROUP_M * p.tiles_n, g = r / group_size, first_m = g * GROUP_M;
@@ -278,6 +274,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       uint32_t kb0, kb1;
       k_range(t, kb0, kb1);
       const uint32_t n_chunks = PARTS == 2 ? (kb1 - kb0 + CHUNK_BLOCKS - 1) / CHUNK_BLOCKS : 1;
+      const uint32_t col0 = tn * BN;
       uint16_t* out = p.out + z * p.stride;
       const uint16_t* gram = POLY ? p.gram + z * p.stride : nullptr;
       const uint32_t row0 = (tm * CTAS + rank) * BM + quarter * 32, row = row0 + lane;
@@ -285,7 +282,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       auto finish = [&](float (&v)[32], uint32_t c) {
         if (c >= p.n || row0 >= p.m) return;
         if constexpr (SPLIT) {
-          float4* to = reinterpret_cast<float4*>(p.partial + ((uint64_t)t * BM + quarter * 32 + lane) * BN + (c - tn * BN));
+          float4* to = reinterpret_cast<float4*>(p.partial + ((uint64_t)t * BM + quarter * 32 + lane) * BN + (c - col0));
 #pragma unroll
           for (int q = 0; q < 8; ++q) to[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
           return;
@@ -378,7 +375,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           float v[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = sum[ch * 32 + i];
-          finish(v, tn * BN + (col_half * CH + ch) * 32);
+          finish(v, col0 + (col_half * CH + ch) * 32);
         }
       } else {
         if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, p.status, ERR_EPILOGUE)) { ok = false; break; }
@@ -391,7 +388,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           float v[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-          finish(v, tn * BN + (col_half * CH + ch) * 32);
+          finish(v, col0 + (col_half * CH + ch) * 32);
         }
         tc_fence_before();
         __syncwarp();
@@ -485,25 +482,19 @@ inline bool encode(void* fn, CUtensorMap* map, const Operand& o, int parts, uint
   return encode_map(fn, map, false, o.ptr, o.cols, o.rows, o.ld, (uint64_t)parts, parts > 1 ? o.part() : 0, batch, batch > 1 ? o.part() * parts : 0, box_rows);
 }
 
-// tiles of `rows` x `bn` that cover a result (of a symmetric one: its lower triangle)
-template <bool SYM> uint32_t tile_count(uint32_t m, uint32_t n, uint32_t rows, uint32_t bn) {
-  const uint32_t tiles_m = (m + rows - 1) / rows;
-  if (!SYM) return tiles_m * ((n + bn - 1) / bn);
-  uint32_t t = 0;
-  for (uint32_t tm = 0; tm < tiles_m; ++tm) t += ((tm + 1) * rows - 1) / bn + 1;
-  return t;
+// square tiles that cover a result (of a symmetric one: its lower triangle)
+template <bool SYM> uint32_t tile_count(uint32_t m, uint32_t n, uint32_t size) {
+  const uint32_t tiles_m = (m + size - 1) / size;
+  return SYM ? tiles_m * (tiles_m + 1) / 2 : tiles_m * ((n + size - 1) / size);
 }
-
-// Tile shapes: one CTA 128 x 128, a pair 256 x 128 or 256 x 256.  COST: TILE_NUMBERS
-struct Shape { int ctas, bn; };
-template <int PARTS, bool SYM> Shape tile_shape(uint32_t m, uint32_t n, uint32_t batch, int sm_count) {
-  auto time = [&](int ctas, int bn, int cost) {
-    const uint64_t slots = (uint64_t)sm_count / ctas;
-    return (tile_count<SYM>(m, n, 128 * ctas, bn) * (uint64_t)batch + slots - 1) / slots * cost;
-  };
-  const uint64_t one = time(1, 128, PARTS == 1 ? 83 : 60), narrow = time(2, 128, 60), wide = time(2, 256, 100);
-  if (one <= narrow && one <= wide) return {1, 128};
-  return narrow < wide ? Shape{2, 128} : Shape{2, 256};
+// 1: tiles of 128 x 128, a CTA each; 2: 256 x 256, a pair.  A round of single CTAs' tiles takes 0.92 of a round of the pairs' with one
+// part, 0.59 with two, where the tensor core works longest on what it reads (k = 2048: 12.7 against 13.9 us, 25.3 against 42.5).
+// (Pairs' tiles of 256 x 128 lose to single CTAs' either way; the last round's tiles in halves changed no whole update: they run
+// under the power limit.)
+template <int PARTS, bool SYM> int tile_ctas(uint32_t m, uint32_t n, uint32_t batch, int sm_count) {
+  const uint32_t pairs = (uint32_t)sm_count / 2, single = tile_count<SYM>(m, n, 128) * batch, wide = tile_count<SYM>(m, n, 256) * batch;
+  if (single <= (uint32_t)sm_count) return 1;            // one round either way; a pair's start costs a microsecond more
+  return (uint64_t)((single + sm_count - 1) / sm_count) * (PARTS == 1 ? 92 : 59) <= (uint64_t)((wide + pairs - 1) / pairs) * 100 ? 1 : 2;
 }
 
 template <int PARTS, int BN, int CTAS, bool SYM, bool POLY, bool B_MN, bool SPLIT = false>
@@ -515,9 +506,11 @@ cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mb, GemmArgs p, con
   if (e != cudaSuccess) return e;
   p.tiles_m = (p.m + BM * CTAS - 1) / (BM * CTAS);
   p.tiles_n = (p.n + BN - 1) / BN;
-  p.tiles = tile_count<SYM>(p.m, p.n, BM * CTAS, BN);
+  static_assert(BN == BM * CTAS, "square tiles");
+  p.tiles = tile_count<SYM>(p.m, p.n, BN);
   p.status = lc.status_word;
-  const unsigned grid = CTAS * (unsigned)std::min<uint64_t>((uint64_t)p.tiles * p.batch * (SPLIT ? p.splits : 1), (uint64_t)lc.sm_count / CTAS);
+  const uint64_t items = (uint64_t)p.tiles * p.batch * (SPLIT ? p.splits : 1);
+  const unsigned grid = CTAS * (unsigned)std::min<uint64_t>(items, (uint64_t)lc.sm_count / CTAS);
   if constexpr (CTAS == 2) {
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -533,10 +526,8 @@ cudaError_t launch(const CUtensorMap& ma, const CUtensorMap& mb, GemmArgs p, con
 }
 
 template <int PARTS, bool SYM, bool POLY, bool B_MN>
-cudaError_t launch(Shape s, const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& p, const LaunchCtx& lc) {
-  if (s.ctas == 1) return launch<PARTS, 128, 1, SYM, POLY, B_MN>(ma, mb, p, lc);
-  if (s.bn == 128) return launch<PARTS, 128, 2, SYM, POLY, B_MN>(ma, mb, p, lc);
-  return launch<PARTS, 256, 2, SYM, POLY, B_MN>(ma, mb, p, lc);
+cudaError_t launch(int ctas, const CUtensorMap& ma, const CUtensorMap& mb, const GemmArgs& p, const LaunchCtx& lc) {
+  return ctas == 1 ? launch<PARTS, 128, 1, SYM, POLY, B_MN>(ma, mb, p, lc) : launch<PARTS, 256, 2, SYM, POLY, B_MN>(ma, mb, p, lc);
 }
 
 }  // namespace muon
