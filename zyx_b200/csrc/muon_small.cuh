@@ -61,6 +61,12 @@ __device__ __forceinline__ uint32_t unit_at(uint32_t row, uint32_t unit) {
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void stmatrix4(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 __device__ __forceinline__ void stmatrix4_trans(uint32_t addr, const uint32_t (&r)[4]) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
@@ -139,8 +145,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     }
   };
 
-  // U items at a time, so that their loads are in flight together: f(first, loaded) for each
-  constexpr uint32_t U = 4;
+  // U items at a time, so that their loads are in flight together (four: 63 us at 128 x 784 f32, two: 61)
+  constexpr uint32_t U = 2;
   // at: the first element; r, c: its place in X; n: how many of the eight are this item's
   struct Item { uint64_t at; uint32_t r, c, n; };
   auto item_at = [&](uint32_t i) {
@@ -159,6 +165,50 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     return t;
   };
 
+  // an item's eight entries of X, packed in pairs per part, to and from shared memory
+  auto x_at = [&](uint32_t s, uint32_t r, uint32_t c) { return smem + SM::X + ((c >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(r, c & 63); };
+  auto put = [&](const Item& t, const uint32_t (&w)[2][4]) {
+    if (!m.tall) {
+#pragma unroll
+      for (int s = 0; s < PARTS; ++s) *reinterpret_cast<uint4*>(x_at(s, t.r, t.c)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+      return;
+    }
+    uint32_t r = t.r, c = t.c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j < (int)t.n) {
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) *reinterpret_cast<uint16_t*>(x_at(s, r, c)) = (uint16_t)(w[s][j / 2] >> (16 * (j & 1)));
+      }
+      if (++r == p.lo) { r = 0; ++c; }
+    }
+  };
+  auto take = [&](const Item& t, uint32_t (&w)[2][4]) {
+    if (!m.tall) {
+#pragma unroll
+      for (int s = 0; s < PARTS; ++s) {
+        const uint4 q = *reinterpret_cast<const uint4*>(x_at(s, t.r, t.c));
+        w[s][0] = q.x; w[s][1] = q.y; w[s][2] = q.z; w[s][3] = q.w;
+      }
+      return;
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[s][j] = 0u;
+    uint32_t r = t.r, c = t.c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j < (int)t.n) {
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) w[s][j / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(x_at(s, r, c)) << (16 * (j & 1));
+      }
+      if (++r == p.lo) { r = 0; ++c; }
+    }
+  };
+
+  // Two parts, lying: between the passes the direction waits in X's place (standing, its entries lie apart: it is read again).
+  const bool stash = PARTS == 2 && !m.tall;
   // momentum, and the sum of squares of the direction (64 bits: see muon.cu)
   double sum = 0.0;
   for (uint32_t i0 = threadIdx.x; i0 < items; i0 += U * SMALL_THREADS) {
@@ -182,6 +232,17 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
         sum += (double)u[e][j] * (double)u[e][j];
       }
       if (b) save(f[e], b, t[e].at, t[e].n, true);          // exact: rounded above
+      if (stash && t[e].n) {
+        // The direction waits for its norm in X's own place: the upper half of its bits where the high part will be, the lower half in
+        // the low part's.
+        uint32_t w[2][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[0][j] = __byte_perm(__float_as_uint(u[e][2 * j]), __float_as_uint(u[e][2 * j + 1]), 0x7632);
+          w[1][j] = __byte_perm(__float_as_uint(u[e][2 * j]), __float_as_uint(u[e][2 * j + 1]), 0x5410);
+        }
+        put(t[e], w);
+      }
     }
   }
   sum = warp_reduce(sum, OpSum());
@@ -202,44 +263,40 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
 #pragma unroll
     for (uint32_t e = 0; e < U; ++e) {
       t[e] = item_at(i0 + e * SMALL_THREADS);
-      load(u[e], g, t[e].at, t[e].n);
-      if (b) load(f[e], b, t[e].at, t[e].n);                // what this thread stored
+      if (!stash) {
+        load(u[e], g, t[e].at, t[e].n);
+        if (b) load(f[e], b, t[e].at, t[e].n);              // what this thread stored
+      }
     }
 #pragma unroll
     for (uint32_t e = 0; e < U; ++e) {
       if (t[e].n == 0) continue;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        u[e][j] *= p.grad_scale;
-        if (b) u[e][j] = p.nesterov ? u[e][j] + p.momentum * f[e][j] : f[e][j];
-        u[e][j] *= inv;
-      }
       uint32_t w[2][4];
+      if (stash) {
+        take(t[e], w);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) split2(u[e][2 * j], u[e][2 * j + 1], w[0][j], w[1][j]);
-      if (!m.tall) {
-#pragma unroll
-        for (int s = 0; s < PARTS; ++s)
-          *reinterpret_cast<uint4*>(smem + SM::X + ((t[e].c >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(t[e].r, t[e].c & 63)) = make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+        for (int j = 0; j < 4; ++j) {
+          u[e][2 * j] = __uint_as_float(__byte_perm(w[1][j], w[0][j], 0x5410)) * inv;
+          u[e][2 * j + 1] = __uint_as_float(__byte_perm(w[1][j], w[0][j], 0x7632)) * inv;
+        }
       } else {
-        uint32_t r = t[e].r, c = t[e].c;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (j < (int)t[e].n) {
-#pragma unroll
-            for (int s = 0; s < PARTS; ++s)
-              *reinterpret_cast<uint16_t*>(smem + SM::X + ((c >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(r, c & 63)) = (uint16_t)(w[s][j / 2] >> (16 * (j & 1)));
-          }
-          if (++r == p.lo) { r = 0; ++c; }
+          u[e][j] *= p.grad_scale;
+          if (b) u[e][j] = p.nesterov ? u[e][j] + p.momentum * f[e][j] : f[e][j];
+          u[e][j] *= inv;
         }
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split2(u[e][2 * j], u[e][2 * j + 1], w[0][j], w[1][j]);
+      put(t[e], w);
     }
   }
   fence_proxy_async_all();
   tc_fence_before();
   __syncthreads();
 
-  constexpr uint32_t gram_idesc = make_idesc(false, false, false, 128, 128);
+  constexpr uint32_t gram_idesc = make_idesc(false, false, false, 128, 128), poly_idesc = make_idesc(false, false, true, 128, 128);
   const uint32_t tiles = p.cols / 64, x_base = base + SM::X, a_base = base + SM::A, stage = base + SM::STAGE;
   const uint32_t quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane, lane_addr = (quarter * 32u) << 16;
   uint32_t phase = 0;
@@ -261,6 +318,21 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     tc_fence_after();
   };
   auto a_byte = [&](uint32_t s, uint32_t r, uint32_t c) { return (s * 2 + (c >> 6)) * SM::TILE_BYTES + tile_at(r, c & 63); };     // of A
+
+  // where this warp's blocks of the mirror image lie: the same in every step
+  constexpr uint32_t WARPS = SMALL_THREADS / 32, MIRRORS = (30 * PARTS + WARPS - 1) / WARPS;
+  uint32_t mirror_from[MIRRORS], mirror_to[MIRRORS];
+#pragma unroll
+  for (uint32_t e = 0; e < MIRRORS; ++e) {
+    const uint32_t op = min(warp + e * WARPS, 30u * PARTS - 1), part = op / 30, t = op % 30 * 4 + (lane >> 3);
+    uint32_t bi = (uint32_t)((1.0f + sqrtf(1.0f + 8.0f * (float)t)) * 0.5f);        // bi (bi - 1) / 2 <= t
+    while (bi * (bi + 1) / 2 <= t) ++bi;
+    while (bi * (bi - 1) / 2 > t) --bi;
+    const uint32_t bj = t - bi * (bi - 1) / 2, in = lane & 7;
+    mirror_from[e] = a_base + a_byte(part, bi * 8 + in, bj * 8);
+    mirror_to[e] = a_base + a_byte(part, bj * 8 + in, bi * 8);
+  }
+  const uint32_t diagonal_block = (warp & 3) * 4 + (lane >> 3), on_diagonal = a_base + a_byte(warp < 4 ? 0 : 1, diagonal_block * 8 + (lane & 7), diagonal_block * 8);
 
   for (int it = 0; it < p.steps; ++it) {
     // ---- gram: two parts: an accumulator per 128 of k (24 additions), as in muon_gemm.cuh
@@ -299,46 +371,55 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
     cluster_sync();
     // the C-th part of the units each
     const uint32_t share = (STAGE_UNITS + ctas - 1) / ctas;
-    for (uint32_t i = rank * share + threadIdx.x; i < min(STAGE_UNITS, (rank + 1) * share); i += SMALL_THREADS) {
-      float4 f[SMALL_CTAS];
+    const uint32_t last = min(STAGE_UNITS, (rank + 1) * share);
+    for (uint32_t i0 = rank * share + threadIdx.x; i0 < last; i0 += 2 * SMALL_THREADS) {      // two at a time: 264 units on 256 threads
+      float4 f[2][SMALL_CTAS];
 #pragma unroll
-      for (uint32_t k = 0; k < SMALL_CTAS; ++k)
-        if (k < ctas) f[k] = ld_cluster4(map_to(stage + i * 16, k));
-      uint32_t q4 = (uint32_t)((sqrtf(1.0f + 2.0f * (float)i) - 1.0f) * 0.5f);       // 2 q (q + 1) <= i
-      while (2 * (q4 + 1) * (q4 + 2) <= i) ++q4;
-      while (2 * q4 * (q4 + 1) > i) --q4;
-      const uint32_t in = i - 2 * q4 * (q4 + 1), rr = q4 * 4 + in / (q4 + 1), q = in % (q4 + 1);
-      float4 s = f[0];
+      for (uint32_t e = 0; e < 2; ++e)
 #pragma unroll
-      for (uint32_t k = 1; k < SMALL_CTAS; ++k)
-        if (k < ctas) { s.x += f[k].x; s.y += f[k].y; s.z += f[k].z; s.w += f[k].w; }
-      uint32_t w[2][2];
-      split2(s.x * UNSCALE, s.y * UNSCALE, w[0][0], w[1][0]);
-      split2(s.z * UNSCALE, s.w * UNSCALE, w[0][1], w[1][1]);
+        for (uint32_t k = 0; k < SMALL_CTAS; ++k)
+          if (k < ctas && i0 + e * SMALL_THREADS < last) f[e][k] = ld_cluster4(map_to(stage + (i0 + e * SMALL_THREADS) * 16, k));
 #pragma unroll
-      for (int part = 0; part < PARTS; ++part) {
-        const uint32_t to = a_base + a_byte(part, rr, q * 4);
-        for (uint32_t k = 0; k < ctas; ++k) st_cluster2(map_to(to, k), w[part][0], w[part][1]);
+      for (uint32_t e = 0; e < 2; ++e) {
+        const uint32_t i = i0 + e * SMALL_THREADS;
+        if (i >= last) break;
+        uint32_t q4 = (uint32_t)((sqrtf(1.0f + 2.0f * (float)i) - 1.0f) * 0.5f);       // 2 q (q + 1) <= i
+        while (2 * (q4 + 1) * (q4 + 2) <= i) ++q4;
+        while (2 * q4 * (q4 + 1) > i) --q4;
+        const uint32_t in = i - 2 * q4 * (q4 + 1), rr = q4 * 4 + in / (q4 + 1), q = in % (q4 + 1);
+        float4 s = f[e][0];
+#pragma unroll
+        for (uint32_t k = 1; k < SMALL_CTAS; ++k)
+          if (k < ctas) { s.x += f[e][k].x; s.y += f[e][k].y; s.z += f[e][k].z; s.w += f[e][k].w; }
+        uint32_t w[2][2];
+        split2(s.x * UNSCALE, s.y * UNSCALE, w[0][0], w[1][0]);
+        split2(s.z * UNSCALE, s.w * UNSCALE, w[0][1], w[1][1]);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          const uint32_t to = a_base + a_byte(part, rr, q * 4);
+          for (uint32_t k = 0; k < ctas; ++k) st_cluster2(map_to(to, k), w[part][0], w[part][1]);
+        }
       }
     }
     cluster_sync();
     // the upper triangle: the 120 blocks of 8 x 8 below the diagonal, four per instruction, loaded and stored transposed ...
-    for (uint32_t op = warp; op < 30 * PARTS; op += SMALL_THREADS / 32) {
-      const uint32_t part = op / 30, t = op % 30 * 4 + (lane >> 3);
-      uint32_t bi = (uint32_t)((1.0f + sqrtf(1.0f + 8.0f * (float)t)) * 0.5f);        // bi (bi - 1) / 2 <= t
-      while (bi * (bi + 1) / 2 <= t) ++bi;
-      while (bi * (bi - 1) / 2 > t) --bi;
-      const uint32_t bj = t - bi * (bi - 1) / 2, in = lane & 7;
-      uint32_t r[4];
-      ldmatrix4(r, a_base + a_byte(part, bi * 8 + in, bj * 8));
-      stmatrix4_trans(a_base + a_byte(part, bj * 8 + in, bi * 8), r);
-    }
-    // ... and the blocks on it, a row per thread
-    if (threadIdx.x < 128 * PARTS) {
-      const uint32_t part = threadIdx.x >> 7, r = threadIdx.x & 127, d = r & ~7u;
 #pragma unroll
-      for (uint32_t c = 0; c < 7; ++c)
-        if (d + c < r) *reinterpret_cast<uint16_t*>(smem + SM::A + a_byte(part, d + c, r)) = *reinterpret_cast<const uint16_t*>(smem + SM::A + a_byte(part, r, d + c));
+    for (uint32_t e = 0; e < MIRRORS; ++e) {
+      if (warp + e * WARPS >= 30 * PARTS) break;
+      uint32_t r[4];
+      ldmatrix4(r, mirror_from[e]);
+      stmatrix4_trans(mirror_to[e], r);
+    }
+    // ... and the 16 on it, each put together from itself and its transpose
+    if (warp < 4 * PARTS) {
+      uint32_t r[4], t[4];
+      ldmatrix4(r, on_diagonal);
+      ldmatrix4_trans(t, on_diagonal);
+      const uint32_t row8 = lane >> 2, col8 = (lane & 3) * 2;          // this lane's two entries of each block
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = col8 + 1 <= row8 ? r[j] : col8 <= row8 ? __byte_perm(r[j], t[j], 0x7610) : t[j];
+      __syncwarp();
+      stmatrix4(on_diagonal, r);
     }
     fence_proxy_async_all();
     tc_fence_before();
@@ -349,8 +430,8 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
       tc_fence_after();
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
-        const uint32_t at = a_base + (kk >> 2) * SM::TILE_BYTES + (kk & 3) * 32;
-        multiply(tmem, at, 2 * SM::TILE_BYTES, at, 2 * SM::TILE_BYTES, 16, gram_idesc, kk != 0);
+        // A is symmetric: as the right operand it is read down its rows (66 clocks a product against 93 of the other reading)
+        multiply(tmem, a_base + (kk >> 2) * SM::TILE_BYTES + (kk & 3) * 32, 2 * SM::TILE_BYTES, a_base + kk * 2048, 2 * SM::TILE_BYTES, SM::TILE_BYTES, poly_idesc, kk != 0);
       }
       umma_commit(bar);
     }
@@ -441,29 +522,17 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
 #pragma unroll
     for (uint32_t e = 0; e < U; ++e) {
       if (t[e].n == 0) continue;
-      float x[8] = {};
-      if (m.tall) {
-        uint32_t r = t[e].r, c = t[e].c;
+      uint32_t w[2][4];
+      take(t[e], w);
+      float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j < (int)t[e].n) {
+      for (int s = 0; s < PARTS; ++s)
 #pragma unroll
-            for (int s = 0; s < PARTS; ++s)
-              x[j] += f16_to_f32(*reinterpret_cast<const uint16_t*>(smem + SM::X + ((c >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(r, c & 63)));
-          }
-          if (++r == p.lo) { r = 0; ++c; }
+        for (int j = 0; j < 4; ++j) {
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[s][j]));
+          x[2 * j] = s ? x[2 * j] + v.x : v.x;
+          x[2 * j + 1] = s ? x[2 * j + 1] + v.y : v.y;
         }
-      } else {
-#pragma unroll
-        for (int s = 0; s < PARTS; ++s) {
-          RawVec<f16_t, 8> q;
-          q.load(reinterpret_cast<const uint16_t*>(smem + SM::X + ((t[e].c >> 6) * PARTS + s) * SM::TILE_BYTES + tile_at(t[e].r, t[e].c & 63)));
-          float v[8];
-          q.decode(v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] += v[j];
-        }
-      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[e][j] = f[e][j] * p.decay - step * x[j];
       save(f[e], pw, t[e].at, t[e].n, p.rn != 0);
