@@ -113,6 +113,13 @@ def test_many_matrices_of_mixed_shapes(gsess, dtype):
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES, ids=R.NAMES.get)
+@pytest.mark.parametrize("shape", [(330, 650), (328, 648)])
+def test_more_tiles_than_a_launch_has_ctas(gsess, dtype, shape):
+    """24 matrices of 66 tiles of 64 x 64 each, lying and standing: the CTAs that lay out X take several."""
+    check(gsess, dtype, [shape, shape[::-1]] * 12, np.random.default_rng(12))
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.NAMES.get)
 def test_zero_and_odd_gradients(gsess, dtype):
     """A zero gradient moves p by the decay only; tiny and huge ones are normed like others; a NaN stays in its own matrix."""
     rng = np.random.default_rng(2)
