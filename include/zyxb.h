@@ -285,11 +285,13 @@ typedef struct {
  *   EMBEDDING      out[i,:] = scale * table[ids[i],:]          (scale 1: the table's bits)
  *   EMBEDDING_BWD  dtable[v,:] = scale * sum over the i with ids[i] = v of dout[i,:]   (+ dtable[v,:] when accumulate is set)
  * The sums are f32, over the tokens in an order that depends on ids alone: the same input gives the same bits.  Without accumulate
- * every row of dtable is written (zeros where no token names it); with it only the named rows are read and written. */
+ * every row of dtable is written (zeros where no token names it); with it only the named rows are read and written.  The output
+ * overlaps no input. */
 typedef struct {
   int32_t  dtype;        /* table, out, dout, dtable: bf16 / f16 / f32 */
   int32_t  id_dtype;     /* ZYXB_I32 or ZYXB_I64 */
-  uint64_t tokens, vocab, dim;   /* each below 2^31 */
+  uint64_t tokens, vocab;        /* below 2^31; EMBEDDING_BWD: at most 2^24 */
+  uint64_t dim;                  /* at most 2^20 */
   uint64_t ld_table, ld_out;     /* row pitch of table / dtable and of out / dout in elements; 0 = dim.  What lies between the rows
                                     is not written */
   float    scale;        /* 0 means 1 */
@@ -306,7 +308,8 @@ typedef struct {
  * Backward (h as stored): xh = h / sqrt(mean(h^2) + eps), g = dy * weight, dx = (g - xh * mean(g * xh)) / sqrt(mean(h^2) + eps) [+ dh],
  * dweight = sum over rows of dy * xh (f32, in a fixed order).  dx is the gradient of x and of residual alike; dh is the gradient
  * that reaches the residual stream behind the norm.
- * An output may be the buffer of an input of its type and shape. */
+ * Squares and sums are f32: entries above 1e19 leave its range, with eps = 0 those below 1e-19 too.
+ * An output may be the buffer of an input of its type and shape; arguments overlap in no other way. */
 typedef struct {
   int32_t  dtype;        /* bf16 / f16 / f32; weight, dweight too */
   int32_t  quant;        /* RMSNORM only: 1 = y as e4m3 bytes [rows, cols] (dense) and scales [rows, ceil(cols / group)] */
@@ -341,7 +344,8 @@ typedef struct {
   float    grad_scale;     /* gradients are multiplied by this first; 0 means 1 */
   int32_t  adjust;         /* ZYXB_MUON_ADJUST_* */
 } zyxb_muon_desc;
-/* ZYXB_KIND_MUON  args (updated in place): p[0..n), g[0..n) [, buf[0..n) when momentum != 0]; p and buf each name n different buffers.
+/* ZYXB_KIND_MUON  args (updated in place): p[0..n), g[0..n) [, buf[0..n) when momentum != 0]; p and buf name 2 n different buffers, g none
+ * of them; they do not overlap.
  * The program owns the memory its products need (allocated at creation, given back at release): a graph that captured its launch
  * must be released before it. */
 

@@ -641,7 +641,7 @@ int launch_rmsnorm_bwd(const zyxb_rmsnorm_desc& d, void* const* args, const uint
     ZYXB_CHECK_ARG(p.y != p.weight && p.dweight != p.y && p.dweight != p.h && p.dweight != p.dy && p.dweight != p.dh,
                    "rmsnorm backward: dx must not be the weight's buffer, dweight no other argument's but the weight's");
   }
-  p.partial = (float*)lc.scratch;
+  p.partial = (float*)lc.scratch;      // a row of cols per CTA: 2048 threads per SM hold at most 32768 columns, 20 MB in all
   cudaError_t e;
   switch (d.dtype) {
     case ZYXB_F32: e = rms_backward<float>(p, lc); break;
