@@ -179,11 +179,17 @@ embedding_index_kernel(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, u
   constexpr uint32_t STEP = 128 * IDX_BATCH;
   const uint32_t slice = ((n + IDX_WARPS - 1) / IDX_WARPS + 127) / 128 * 128;
   const uint32_t begin = min(n, warp * slice), end = min(n, begin + slice);
-  uint32_t below = 0;
-  for (uint32_t i0 = begin; i0 < end; i0 += STEP) {
-    int v[IDX_BATCH][4];
+  int v[IDX_BATCH][4];
+  uint32_t held = 0xffffffffu;                    // where v begins
+  auto fetch = [&](uint32_t i0) {
+    if (held == i0) return;                       // up to 16384 tokens: the second pass finds the first one's still there
+    held = i0;
 #pragma unroll
     for (int q = 0; q < IDX_BATCH; ++q) load4(ids, i0 + q * 128 + lane * 4, end, v[q]);
+  };
+  uint32_t below = 0;
+  for (uint32_t i0 = begin; i0 < end; i0 += STEP) {
+    fetch(i0);
 #pragma unroll
     for (int q = 0; q < IDX_BATCH; ++q)
 #pragma unroll
@@ -224,9 +230,7 @@ embedding_index_kernel(const ID* __restrict__ ids, uint32_t n, uint32_t vocab, u
   __syncthreads();
   // second pass: equal rows of a warp's 32 lanes take consecutive places
   for (uint32_t i0 = begin; i0 < end; i0 += STEP) {
-    int v[IDX_BATCH][4];
-#pragma unroll
-    for (int q = 0; q < IDX_BATCH; ++q) load4(ids, i0 + q * 128 + lane * 4, end, v[q]);
+    fetch(i0);
 #pragma unroll
     for (int q = 0; q < IDX_BATCH; ++q)
 #pragma unroll
@@ -386,13 +390,14 @@ embedding_combine_kernel(typename Elem<T>::store_t* dtable, const EmbGradParams 
   __shared__ float part[CMB_WARPS][CMB_COLS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  const uint32_t n = p.starts[p.vocab], c = blockIdx.x * CMB_WARPS + warp;
+  const uint32_t c = blockIdx.x * CMB_WARPS + warp;
   const uint64_t begin = (uint64_t)c * p.chunk, end = begin + p.chunk;
   if (lane == 0) {
     found[warp][2] = 0;
-    if (end < n) {
-      const SortedToken s = p.sorted[end - 1];
-      if (s.token & SHARED) {
+    if (end < p.tokens) {
+      const SortedToken s = p.sorted[end - 1];       // behind the n named ones (not every token names a row) it holds nothing
+      const uint32_t n = p.starts[p.vocab];
+      if (end < n && (s.token & SHARED)) {
         const uint32_t r0 = p.starts[s.row], r1 = p.starts[s.row + 1];
         if (r0 >= begin) { found[warp][0] = s.row; found[warp][1] = c; found[warp][2] = (r1 - 1) / p.chunk; }
       }
