@@ -433,8 +433,14 @@ __global__ void __launch_bounds__(1024) rmsnorm_dweight_kernel(const float* part
   pdl_wait();
   float sum = 0.0f;
   if (c < cols) {
-#pragma unroll 8
-    for (uint32_t i = warp; i < n; i += 32) sum += partial[(uint64_t)i * cols + c];
+    constexpr int U = 12;                          // loads in flight: 384 CTAs' partials in one go
+    for (uint32_t i0 = warp; i0 < n; i0 += 32 * U) {
+      float v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = i0 + 32 * u < n ? partial[(uint64_t)(i0 + 32 * u) * cols + c] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) sum += v[u];
+    }
   }
   part[warp][lane] = sum;
   __syncthreads();
