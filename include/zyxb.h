@@ -404,12 +404,6 @@ int32_t zyxb_buffer_bytes(zyxb_ctx* ctx, int32_t dev, uint32_t buf, uint64_t* ou
  * plan's `Alias` instruction shares storage (zyx/src/graph/plan.rs:47-54).  Freeing a view releases
  * only the id; the parent must outlive its views. */
 int32_t zyxb_buffer_view(zyxb_ctx* ctx, int32_t dev, uint32_t parent, uint64_t offset, uint64_t bytes, uint32_t* out_buf);
-/* An id for device memory that another library of this process owns (a tensor of it, say): programs then read and write it in
- * place.  device_ptr is 256-byte aligned and [device_ptr, device_ptr + bytes) lies inside one allocation on this device.
- * zyxb_free releases only the id; the owner keeps the memory alive until this library's work on it has finished.  The library's
- * streams know nothing of the owner's: synchronise with the owner's stream before a launch, and with this device (zyxb_sync /
- * zyxb_device_sync) before the owner reads what a launch wrote. */
-int32_t zyxb_buffer_import(zyxb_ctx* ctx, int32_t dev, void* device_ptr, uint64_t bytes, uint32_t* out_buf);
 /* blocking; destroys the events */
 int32_t zyxb_sync(zyxb_ctx* ctx, int32_t dev, const zyxb_event* events, int32_t n);
 /* non-blocking destroy */

@@ -134,7 +134,6 @@ SIGNATURES = {
     "zyxb_memset": (C.c_int32, [_CTX, C.c_int32, C.c_uint32, C.c_uint64, C.c_int32, C.c_uint64]),
     "zyxb_buffer_bytes": (C.c_int32, [_CTX, C.c_int32, C.c_uint32, C.POINTER(C.c_uint64)]),
     "zyxb_buffer_view": (C.c_int32, [_CTX, C.c_int32, C.c_uint32, C.c_uint64, C.c_uint64, _U32_P]),
-    "zyxb_buffer_import": (C.c_int32, [_CTX, C.c_int32, C.c_void_p, C.c_uint64, _U32_P]),
     "zyxb_sync": (C.c_int32, [_CTX, C.c_int32, _EV_P, C.c_int32]),
     "zyxb_release_events": (C.c_int32, [_CTX, C.c_int32, _EV_P, C.c_int32]),
     "zyxb_device_sync": (C.c_int32, [_CTX, C.c_int32]),
@@ -169,6 +168,10 @@ SIGNATURES = {
     "zyxb_comm_option": (C.c_int32, [_CTX, C.c_int32, C.c_int32, C.c_int32]),
     "zyxb_comm_destroy": (C.c_int32, [_CTX, C.c_int32]),
 }
+# ... and include/zyxb_interop.h
+INTEROP_SIGNATURES = {
+    "zyxb_buffer_import": (C.c_int32, [_CTX, C.c_int32, C.c_void_p, C.c_uint64, _U32_P]),
+}
 
 _lib = None
 
@@ -182,7 +185,7 @@ def load():
         raise ImportError("zyx_b200: %s is missing — build it with `python -m zyx_b200.build` "
                           "(there is no CPU or PyTorch fallback)" % LIB_PATH)
     lib = C.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **INTEROP_SIGNATURES}.items():
         fn = getattr(lib, name)   # AttributeError if the library does not export it
         fn.restype = res
         fn.argtypes = args

@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "comm.h"
+#include "../../include/zyxb_interop.h"
 #include "internal.h"
 
 using namespace zyxb;
