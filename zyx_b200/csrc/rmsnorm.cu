@@ -482,8 +482,13 @@ RmsShape rms_shape(uint64_t rows, uint64_t vectors, int packs_wanted, int sm_cou
 
 void rms_apply(RmsParams& p, const RmsShape& s) { p.log_tpr = s.log_tpr; p.tpr = s.tpr; p.groups = s.groups; }
 
+// A kernel of PACKS vectors per thread and THREADS threads covers a row of this shape: what it would leave out, it would leave out
+// silently, so both directions ask before they launch.
+template <int PACKS, int THREADS> bool rms_covers(const RmsShape& s) { return s.packs <= PACKS && s.threads <= THREADS; }
+
 template <typename T, int PACKS, bool ALIGNED, int THREADS>
 cudaError_t run_rms(const RmsParams& p, const RmsShape& s, bool quant, const LaunchCtx& lc) {
+  if (!rms_covers<PACKS, THREADS>(s)) return cudaErrorInvalidConfiguration;
   const uint64_t per_cta = (uint64_t)s.groups;
   const unsigned grid = (unsigned)((p.rows + per_cta - 1) / per_cta);
   constexpr uint32_t VEC = 16 / sizeof(typename Elem<T>::store_t);
@@ -526,6 +531,7 @@ cudaError_t rms_forward(const RmsParams& p, bool quant, const LaunchCtx& lc) {
 
 template <typename T, int PACKS, bool ALIGNED, int THREADS>
 cudaError_t run_rms_bwd(const RmsParams& p, const RmsShape& s, unsigned* grid_out, const LaunchCtx& lc) {
+  if (!rms_covers<PACKS, THREADS>(s)) return cudaErrorInvalidConfiguration;
   constexpr int VEC = 16 / (int)sizeof(typename Elem<T>::store_t);
   const int groups = s.groups;
   const size_t smem = p.weight_on ? (size_t)groups * p.cols * 4 : 0;
@@ -563,9 +569,10 @@ cudaError_t rms_backward(const RmsParams& p, const LaunchCtx& lc) {
   RmsParams q = p;
   const bool aligned = p.cols % VEC == 0 && p.ld % VEC == 0;
   const uint64_t vectors = aligned ? p.cols / VEC : (p.cols + 2 * VEC - 2) / VEC;
-  // three vectors of f32 still fit the registers of 512 threads, which hold 6144 columns that way
+  // Three vectors of f32 still fit the registers of 512 threads, which hold 6144 columns that way; rows of at most 3 * 256 vectors,
+  // which few rows spread over more than 512 threads too, would come back with 256 threads and stay as they are: no form of 256 threads has three
   RmsShape s = rms_shape(p.rows, vectors, 2, lc.sm_count);
-  if (sizeof(T) == 4 && s.threads > 512 && vectors <= 3 * 512) s = rms_shape(UINT32_MAX, vectors, 3, lc.sm_count);
+  if (sizeof(T) == 4 && s.threads > 512 && vectors > 3 * 256 && vectors <= 3 * 512) s = rms_shape(UINT32_MAX, vectors, 3, lc.sm_count);
   rms_apply(q, s);
   unsigned grid = 0;
   cudaError_t e = aligned ? run_rms_bwd_packs<T, true>(q, s, &grid, lc) : run_rms_bwd_packs<T, false>(q, s, &grid, lc);
