@@ -204,6 +204,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           if (++stage == SM::STAGES) { stage = 0; phase ^= 1; }
         }
       }
+      // Every stage's last release is waited for before the CTA goes: the issuer's commits arrive in both CTAs of a pair, tfull's says
+      // nothing of the ones before it, and the shared memory has to be there when they come.
+      for (uint32_t i = 0, s = stage, ph = phase; i < (uint32_t)SM::STAGES && ok; ++i) {
+        ok = mbar_wait(empty_bar(s), ph ^ 1, abort_flag, p.status, ERR_PRODUCER);
+        if (++s == SM::STAGES) { s = 0; ph ^= 1; }
+      }
       if (!ok && rank == 0) {     // copies in flight land before the CTA goes (a pair's: both wait for each other at the end)
         uint32_t s = stage, ph = phase;
         const uint32_t n_back = issued < (uint32_t)SM::STAGES ? issued : (uint32_t)SM::STAGES;
