@@ -8,7 +8,6 @@
 //   compute : every kernel, d2h, memset            (in-order: a launch sees all earlier launches)
 //   copy    : h2d, so uploads can overlap kernels  (ordered against compute by events)
 //   comm    : NCCL collectives                      (ordered against compute by events)
-#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdio.h>
 #include <string.h>
@@ -21,6 +20,7 @@
 
 #include "comm.h"
 #include "../../include/zyxb_interop.h"
+#include "import_range.h"
 #include "internal.h"
 
 using namespace zyxb;
@@ -435,13 +435,8 @@ int32_t zyxb_buffer_import(zyxb_ctx* ctx, int32_t dev, void* device_ptr, uint64_
   cudaError_t e = cudaPointerGetAttributes(&at, device_ptr);
   if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "buffer_import", e); }
   if (at.type != cudaMemoryTypeDevice || at.device != D.cuda_id) return fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "buffer_import: not memory of this device");
-  if (D.address_range) {      // the whole range belongs to the allocation the address lies in
-    CUdeviceptr base = 0;
-    size_t size = 0;
-    if (reinterpret_cast<CUresult (*)(CUdeviceptr*, size_t*, CUdeviceptr)>(D.address_range)(&base, &size, (CUdeviceptr)device_ptr) != CUDA_SUCCESS ||
-        !range_ok((uint64_t)((CUdeviceptr)device_ptr - base), bytes, size))
-      return fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, "buffer_import: range exceeds the allocation");
-  }
+  if (const char* why = import_refusal(D.address_range, (uint64_t)(uintptr_t)device_ptr, bytes))
+    return fail(ctx, ZYXB_ERR_MEMORY_ALLOCATION, std::string("buffer_import: ") + why);
   uint32_t id;
   if (!D.free_buffer_ids.empty()) { id = D.free_buffer_ids.back(); D.free_buffer_ids.pop_back(); }
   else { id = (uint32_t)D.buffers.size(); D.buffers.emplace_back(); }
