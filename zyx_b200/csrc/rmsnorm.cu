@@ -509,13 +509,11 @@ cudaError_t run_rms_packs(const RmsParams& p, const RmsShape& s, bool quant, con
   if (s.threads <= 256) {
     if (s.packs == 1) return run_rms<T, 1, ALIGNED, 256>(p, s, quant, lc);
     if (s.packs == 2) return run_rms<T, 2, ALIGNED, 256>(p, s, quant, lc);
-    if (s.packs <= 4) return run_rms<T, 4, ALIGNED, 256>(p, s, quant, lc);
-    if constexpr (sizeof(T) == 4) return run_rms<T, 8, ALIGNED, 256>(p, s, quant, lc);
+    return run_rms<T, 4, ALIGNED, 256>(p, s, quant, lc);
   }
   if (s.packs == 1) return run_rms<T, 1, ALIGNED, 1024>(p, s, quant, lc);
   if (s.packs == 2) return run_rms<T, 2, ALIGNED, 1024>(p, s, quant, lc);
-  if constexpr (sizeof(T) == 4 && !ALIGNED) { if (s.packs > 4 && s.threads > 512) return run_rms<T, 8, ALIGNED, 1024>(p, s, quant, lc); }     // 4097 vectors, spread wide
-  if constexpr (sizeof(T) == 4) { if (s.packs > 4) return run_rms<T, 8, ALIGNED, 512>(p, s, quant, lc); }
+  if constexpr (sizeof(T) == 4 && !ALIGNED) { if (s.packs > 4) return run_rms<T, 8, ALIGNED, 1024>(p, s, quant, lc); }     // 4097 vectors, spread wide
   return run_rms<T, 4, ALIGNED, 1024>(p, s, quant, lc);
 }
 
