@@ -169,8 +169,10 @@ SIGNATURES = {
     "zyxb_comm_destroy": (C.c_int32, [_CTX, C.c_int32]),
 }
 # ... and include/zyxb_interop.h
+OWN_STREAM = C.c_void_p(-1).value
 INTEROP_SIGNATURES = {
     "zyxb_buffer_import": (C.c_int32, [_CTX, C.c_int32, C.c_void_p, C.c_uint64, _U32_P]),
+    "zyxb_use_stream": (C.c_int32, [_CTX, C.c_int32, C.c_void_p]),
 }
 
 _lib = None

@@ -151,7 +151,7 @@ class MemoryPool:
 
     def import_device(self, device_ptr, nbytes):
         """An id for device memory that another library of this process owns (256-byte aligned, on this device); the caller keeps it
-        alive and orders its own stream against this library's (zyxb_buffer_import).  deallocate releases only the id."""
+        alive and orders its own stream against this library's (zyxb_buffer_import; Device.use_stream).  deallocate releases only the id."""
         buf = C.c_uint32()
         self.be._check(self.be.lib.zyxb_buffer_import(self.be.ctx, self.dev, C.c_void_p(int(device_ptr)), int(nbytes), C.byref(buf)))
         return buf.value
@@ -232,6 +232,11 @@ class Device:
         t = C.c_uint64()
         self.be._check(self.be.lib.zyxb_program_get_step(self.be.ctx, self.dev, program_id, C.byref(t)))
         return t.value
+
+    def use_stream(self, stream):
+        """Launches go to `stream` (a cudaStream_t as an integer, 0 the legacy default stream: what torch calls cuda_stream) from here
+        on, in order with what others put there; None: the context's own stream again (zyxb_use_stream)."""
+        self.be._check(self.be.lib.zyxb_use_stream(self.be.ctx, self.dev, L.OWN_STREAM if stream is None else int(stream)))
 
     def sync(self):
         self.be._check(self.be.lib.zyxb_device_sync(self.be.ctx, self.dev))

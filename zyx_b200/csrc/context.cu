@@ -5,7 +5,7 @@
 // (zyx/src/lib.rs:96), possibly from different OS threads.  Instead of the reference CUDA
 // backend's worker thread per device (zyx/src/backend/cuda.rs:475-519) every call here makes
 // its device current and enqueues on that device's streams:
-//   compute : every kernel, d2h, memset            (in-order: a launch sees all earlier launches)
+//   compute : every kernel, d2h, memset            (in-order: a launch sees all earlier launches); a caller's stream after zyxb_use_stream
 //   copy    : h2d, so uploads can overlap kernels  (ordered against compute by events)
 //   comm    : NCCL collectives                      (ordered against compute by events)
 #include <cuda_runtime.h>
@@ -52,6 +52,7 @@ struct Device {
   int cuda_id = 0;
   cudaDeviceProp prop{};
   cudaStream_t compute = nullptr, copy = nullptr, comm_stream = nullptr;
+  cudaStream_t own_compute = nullptr;     // compute is this one, or a caller's (zyxb_use_stream)
   std::vector<Buffer> buffers;
   std::vector<uint32_t> free_buffer_ids;
   std::vector<Program> programs;
@@ -269,6 +270,7 @@ int32_t zyxb_init(const zyxb_config* config, zyxb_ctx** out_ctx) {
         (e = cudaStreamCreateWithFlags(&D.comm_stream, cudaStreamNonBlocking)) != cudaSuccess) {
       delete ctx; return cuda_fail(nullptr, ZYXB_ERR_INITIALIZATION, "stream creation", e);
     }
+    D.own_compute = D.compute;
     D.scratch_bytes = 320ull << 20;   // partials of split reductions, prepared operands of the f32 tensor-core matmul
     if ((e = cudaMalloc(&D.scratch, D.scratch_bytes)) != cudaSuccess || (e = cudaMalloc((void**)&D.status_word, 256)) != cudaSuccess) {
       delete ctx; return cuda_fail(nullptr, ZYXB_ERR_MEMORY_ALLOCATION, "scratch allocation", e);
@@ -312,7 +314,7 @@ int32_t zyxb_shutdown(zyxb_ctx* ctx) {
     if (D.scratch) cudaFree(D.scratch);
     if (D.status_word) cudaFree(D.status_word);
     if (D.flush_buf) cudaFree(D.flush_buf);
-    cudaStreamDestroy(D.compute); cudaStreamDestroy(D.copy); cudaStreamDestroy(D.comm_stream);
+    cudaStreamDestroy(D.own_compute); cudaStreamDestroy(D.copy); cudaStreamDestroy(D.comm_stream);
   }
   for (auto& kv : ctx->registered) cudaHostUnregister(kv.first);
   delete ctx;
@@ -445,6 +447,25 @@ int32_t zyxb_buffer_import(zyxb_ctx* ctx, int32_t dev, void* device_ptr, uint64_
   b.ptr = device_ptr; b.bytes = bytes; b.capacity = bytes; b.live = true;
   b.is_view = true; b.parent = id;       // like a view: freeing it releases the id, the owner keeps the memory
   *out_buf = id;
+  return ZYXB_OK;
+}
+
+int32_t zyxb_use_stream(zyxb_ctx* ctx, int32_t dev, void* stream) {
+  DEV_OR_FAIL(ZYXB_ERR_INITIALIZATION);
+  NOT_WHILE_CAPTURING("zyxb_use_stream", ZYXB_ERR_INITIALIZATION);
+  cudaStream_t next = stream == ZYXB_OWN_STREAM ? D.own_compute : (cudaStream_t)stream;
+  if (next == cudaStreamPerThread) return fail(ctx, ZYXB_ERR_INITIALIZATION, "use_stream: the per-thread default stream is another one in every thread");
+  if (next == cudaStreamLegacy) next = nullptr;      // one name for the legacy default stream
+  if (next == D.compute) return ZYXB_OK;
+  int on = D.cuda_id;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(next, &capture);
+  if (e == cudaSuccess && capture != cudaStreamCaptureStatusNone) return fail(ctx, ZYXB_ERR_INITIALIZATION, "use_stream: the stream is being captured");
+  if (e == cudaSuccess && next) e = cudaStreamGetDevice(next, &on);
+  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, ZYXB_ERR_INITIALIZATION, "use_stream", e); }
+  if (on != D.cuda_id) return fail(ctx, ZYXB_ERR_INITIALIZATION, "use_stream: the stream belongs to another device");
+  if (int st = order_streams(ctx, D.compute, next, ZYXB_ERR_INITIALIZATION)) return st;
+  D.compute = next;
   return ZYXB_OK;
 }
 
@@ -763,7 +784,7 @@ int32_t zyxb_capture_begin(zyxb_ctx* ctx, int32_t dev) {
   DEV_OR_FAIL(ZYXB_ERR_KERNEL_LAUNCH);
   if (D.capturing) return fail(ctx, ZYXB_ERR_KERNEL_LAUNCH, "capture_begin: a capture is already open");
   cudaError_t e = cudaStreamBeginCapture(D.compute, cudaStreamCaptureModeThreadLocal);
-  if (e != cudaSuccess) return cuda_fail(ctx, ZYXB_ERR_KERNEL_LAUNCH, "cudaStreamBeginCapture", e);
+  if (e != cudaSuccess) { cudaGetLastError(); return cuda_fail(ctx, ZYXB_ERR_KERNEL_LAUNCH, "cudaStreamBeginCapture", e); }
   D.capturing = true;
   D.capture_launch_base = D.launch_count;
   return ZYXB_OK;
