@@ -124,7 +124,8 @@ MUON = dict(lr=0.02, weight_decay=0.01, momentum=0.95)
 
 
 class _Program:
-    """A program of the package on tensors of this process: they are imported as pool buffers, in the order of its arguments."""
+    """A program of the package on tensors of this process: they are imported as pool buffers, in the order of its arguments, and the
+    launches go to torch's stream, in order with what fills the tensors before and reads or frees them after."""
 
     def __init__(self, desc, tensors):
         from zyx_b200.ops import Session
@@ -132,6 +133,7 @@ class _Program:
             _Program.session = Session(device_ids=[torch.cuda.current_device()], round_nearest=True)
         s = _Program.session
         self.pool, self.device = s.pool, s.device
+        self.device.use_stream(torch.cuda.current_stream().cuda_stream)
         self.prog = self.device.create_program(desc)
         self.args = [self.pool.import_device(x.data_ptr(), x.numel() * x.element_size()) for x in tensors]
 
