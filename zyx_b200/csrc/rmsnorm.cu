@@ -133,7 +133,8 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 constexpr float E4M3_MAX = 448.0f, AMAX_FLOOR = 1e-30f;
 
 // 448 / largest: what y is multiplied by.  The reciprocal is the approximate one (1 ulp): a value next to the border between two 8-bit
-// floats may go to either, as it may by the f32 rounding of y itself.
+// floats may go to either, as it may by the f32 rounding of y itself.  At 8192 x 4096 with groups of 128, 975 of 33.6 million values are on
+// the other side than in 64 bits, and 949 with a division rounded once, which costs 4 us of 41.
 __device__ __forceinline__ float e4m3_factor(float amax) {
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(amax));
