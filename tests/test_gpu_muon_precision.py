@@ -64,8 +64,9 @@ def test_step_of_several(gsess, dtype):
 
 @pytest.mark.parametrize("dtype", [L.F32, L.BF16], ids=R.NAMES.get)
 @pytest.mark.parametrize("shape", [(40, 72), (72, 40), (300, 260), (260, 300), (300, 261)])
-@pytest.mark.parametrize("scale,eps", [(1e25, 0.0), (1e-3, 0.0), (1e-20, 1e-30), (1e-30, 1e-30)])
+@pytest.mark.parametrize("scale,eps", [(1e25, 0.0), (2e37, 0.0), (1e-3, 0.0), (1e-20, 1e-30), (1e-30, 1e-30)])
 def test_large_and_small_gradients_are_normed_like_others(gsess, dtype, shape, scale, eps):
+    """The norm of the gradients of 2e37 lies outside f32."""
     check(gsess, dtype, [shape], scale=scale, eps=eps)
 
 

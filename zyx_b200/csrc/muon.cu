@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(MUON_THREADS) muon_normalize_kernel(const __gr
     double s = 0.0;
 #pragma unroll
     for (int w = 0; w < MUON_THREADS / 32; ++w) s += part[w];
-    return muon::SCALE / ((float)sqrt(s) + eps);
+    return (float)(muon::SCALE / (sqrt(s) + (double)eps));       // the norm itself may lie outside f32
   };
   auto put = [&](const float (&v)[8], uint32_t y, uint32_t q, float inv) {
     uint32_t w[2][4];

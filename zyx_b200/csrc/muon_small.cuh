@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
   cluster_sync();
   double total = 0.0;
   for (uint32_t q = 0; q < ctas; ++q) total += ld_cluster_f64(map_to(smem_u32(sums), q));
-  const float inv = SCALE / ((float)sqrt(total) + p.eps);
+  const float inv = (float)(SCALE / (sqrt(total) + (double)p.eps));      // the norm itself may lie outside f32
   for (uint32_t i0 = threadIdx.x; i0 < items; i0 += U * SMALL_THREADS) {
     Item t[U];
     float u[U][8], f[U][8];
