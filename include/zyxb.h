@@ -346,8 +346,8 @@ typedef struct {
 } zyxb_muon_desc;
 /* ZYXB_KIND_MUON  args (updated in place): p[0..n), g[0..n) [, buf[0..n) when momentum != 0]; p and buf name 2 n different buffers, g none
  * of them; they do not overlap.
- * The program owns the memory its products need (allocated at creation, given back at release): a graph that captured its launch
- * must be released before it. */
+ * The program owns the memory its products need (allocated at creation, given back at release): its release is refused while a graph
+ * lives that captured its launch. */
 
 typedef struct {
   int32_t kind;  /* ZYXB_KIND_* */

@@ -44,6 +44,7 @@ struct Program {
   std::vector<uint64_t> numel;  // optimizer programs: copy of desc.u.optim.numel; Muon: rows, then cols of its matrices
   void* workspace = nullptr;    // Muon: memory of its products, owned by the program
   uint64_t workspace_bytes = 0;
+  std::vector<uint32_t> graphs; // graphs that captured a launch of it and with it the workspace's address
   uint64_t step = 0;            // optimizer programs: AdamW::t
   bool live = false;
 };
@@ -680,6 +681,9 @@ int32_t zyxb_program_release(zyxb_ctx* ctx, int32_t dev, uint32_t prog) {
   if (prog == 0 || prog >= D.programs.size() || !D.programs[prog].live) return fail(ctx, ZYXB_ERR_KERNEL_COMPILATION, "release: unknown program");
   if (D.programs[prog].workspace) {
     NOT_WHILE_CAPTURING("zyxb_program_release of a Muon program", ZYXB_ERR_KERNEL_COMPILATION);
+    for (uint32_t g : D.programs[prog].graphs)      // a replay would write to memory that has a new owner
+      if (g <= D.graphs.size() && D.graphs[g - 1].first)
+        return fail(ctx, ZYXB_ERR_KERNEL_COMPILATION, "release: graph " + std::to_string(g) + " captured a launch of this program and its workspace; release the graph first");
     recycle_block(D, D.programs[prog].workspace, D.programs[prog].workspace_bytes);
   }
   D.programs[prog] = Program();
@@ -752,6 +756,8 @@ int32_t zyxb_launch(zyxb_ctx* ctx, int32_t dev, uint32_t prog, const uint32_t* a
       break;
     default: st = ZYXB_ERR_KERNEL_LAUNCH; err = "launch: unknown kernel kind";
   }
+  const uint32_t next_graph = (uint32_t)D.graphs.size() + 1;       // the number that the open capture will get
+  if (D.capturing && P.workspace && st != ZYXB_ERR_INCORRECT_KERNEL_ARG && (P.graphs.empty() || P.graphs.back() != next_graph)) P.graphs.push_back(next_graph);
   if (st) return fail(ctx, st, err);
   if (ctx->debug & 1) fprintf(stderr, "[zyxb] launch program %u kind %d\n", prog, P.desc.kind);
   return record_event(ctx, D, D.compute, out_event, ZYXB_ERR_KERNEL_LAUNCH);
@@ -794,6 +800,7 @@ int32_t zyxb_capture_end(zyxb_ctx* ctx, int32_t dev, uint32_t* out_graph) {
   DEV_OR_FAIL(ZYXB_ERR_KERNEL_LAUNCH);
   if (!D.capturing || !out_graph) return fail(ctx, ZYXB_ERR_KERNEL_LAUNCH, "capture_end: no capture is open");
   D.capturing = false;
+  D.graphs.emplace_back(nullptr, 0);           // a number even if the capture fails: programs may have noted it
   cudaGraph_t graph = nullptr;
   cudaError_t e = cudaStreamEndCapture(D.compute, &graph);
   if (e != cudaSuccess || !graph) { cudaGetLastError(); return cuda_fail(ctx, ZYXB_ERR_KERNEL_LAUNCH, "cudaStreamEndCapture", e); }
@@ -803,7 +810,7 @@ int32_t zyxb_capture_end(zyxb_ctx* ctx, int32_t dev, uint32_t* out_graph) {
   if (e != cudaSuccess) return cuda_fail(ctx, ZYXB_ERR_KERNEL_COMPILATION, "cudaGraphInstantiate", e);
   const uint64_t kernels = D.launch_count - D.capture_launch_base;
   D.launch_count = D.capture_launch_base;      // captured launches have not run yet; replays are counted
-  D.graphs.emplace_back(exec, kernels);
+  D.graphs.back() = {exec, kernels};
   *out_graph = (uint32_t)D.graphs.size();      // ids start at 1
   return ZYXB_OK;
 }
