@@ -284,9 +284,11 @@ typedef struct {
  * no gradient.
  *   EMBEDDING      out[i,:] = scale * table[ids[i],:]          (scale 1: the table's bits)
  *   EMBEDDING_BWD  dtable[v,:] = scale * sum over the i with ids[i] = v of dout[i,:]   (+ dtable[v,:] when accumulate is set)
- * The sums are f32, over the tokens in an order that depends on ids alone: the same input gives the same bits.  Without accumulate
- * every row of dtable is written (zeros where no token names it); with it only the named rows are read and written.  The output
- * overlaps no input. */
+ * The sums are f32, in an order that the descriptor, the ids and the device fix: the same call gives the same bits (another dim, type or
+ * GPU may cut a row's tokens into other partial sums).  Without accumulate every row of dtable is written (zeros where no token names
+ * it); with it only the named rows are read and written.  The output overlaps no input.
+ * EMBEDDING_BWD reads all ids once for each 1024 rows of the vocabulary (once per SM below some 150 000 rows): 1 ms at 2^20 tokens and
+ * 2^20 rows, and with the product of the two from there, so that its limits take a quarter of a second. */
 typedef struct {
   int32_t  dtype;        /* table, out, dout, dtable: bf16 / f16 / f32 */
   int32_t  id_dtype;     /* ZYXB_I32 or ZYXB_I64 */

@@ -14,7 +14,9 @@
 //            of the runs that begin in its chunk in f32 registers; a run of more than two chunks is shared by the chunks it
 //            crosses, each leaving f32 partials.  The same launch writes the rows of zeros.
 //   combine  Adds the partials of each shared run, in chunk order.
-// The order of every sum depends on ids alone.
+// The order of every sum is fixed by ids and by where the chunks end, which the launch chooses by extents, type, SMs and scratch memory.
+// The index launch reads all token numbers in every CTA: 0.04 ms at 2^16 tokens and rows, 0.12 at 2^18, 1.0 at 2^20, and as tokens x
+// rows from there.
 #include <algorithm>
 
 #include "internal.h"
