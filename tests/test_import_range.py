@@ -41,3 +41,14 @@ def test_the_library_asks(refusal):
     text = open(os.path.join(ROOT, "zyx_b200", "csrc", "context.cu")).read()
     body = text[text.index("int32_t zyxb_buffer_import("):text.index("int32_t zyxb_buffer_bytes(")]
     assert "import_refusal(D.address_range" in body and "if (D.address_range)" not in body
+
+
+def test_the_interop_header_and_binding_agree():
+    import re
+    from zyx_b200 import _lib, build
+    build.build()
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "zyxb_interop.h")).read(), flags=re.S)
+    declared = sorted(set(re.findall(r"\b(zyxb_[a-z0-9_]+)\s*\(", text)))
+    assert declared == sorted(_lib.INTEROP_SIGNATURES)
+    lib = _lib.load()
+    assert all(hasattr(lib, name) for name in declared)
